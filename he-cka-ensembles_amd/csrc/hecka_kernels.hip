@@ -7,28 +7,12 @@
 #include <stdio.h>
 #include <stdlib.h>
 
-#include "../../include/hecka.h"
+#include "hecka_host.hpp"
 #include "gemm_mfma.hpp"
 #include "gemm_bf16x6.hpp"
 #include "gemm_f16x3_k32.hpp"
 
 namespace hecka {
-
-static thread_local char g_err[256] = "";
-
-static int fail(int code, const char* fmt, const char* a = "", long long x = 0, long long y = 0) {
-  snprintf(g_err, sizeof(g_err), fmt, a, x, y);
-  return code;
-}
-static int check_launch(const char* what) {
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return fail(HECKA_ELAUNCH, "%s: launch failed (%lld)", what, (long long)e);
-  return HECKA_OK;
-}
-// hipGetLastError is sticky per thread: drop whatever an earlier, unrelated runtime call left behind so
-// that check_launch reports only this launch.
-static inline void clear_error() { (void)hipGetLastError(); }
-static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // ------------------------------------------------------------------------------------------
 // (1) column mean: sbar[m,p] = mean_b X[m,b,p].   HBM-bound: reads X once (4 B / element).
