@@ -1,0 +1,56 @@
+// 8-bit blocks: 128 consecutive elements of a row share one power of two s = 2^q, the smallest with max |x| <= 448 s over the
+// block's finite elements (q >= -126; 0 for a block of zeros), and each is kept as the e4m3 code nearest to x / s, ties to
+// even.  The division by a power of two is exact, so a code is off by half a step of its own binade: 2^-4 of the value, or
+// 2^-10 s where the value is below 2^-6 s.  A NaN or an infinity is kept as NaN (code 0x7f) and leaves its neighbours' scale
+// alone; a finite element stays finite: with the topmost scale, 2^120, codes end at 240 (256 2^120 is no fp32 number).  A scale is kept as the byte q + 127 - the form in which the scaled matrix instructions take it.
+#pragma once
+#include "hecka_vec.hpp"
+
+namespace hecka {
+
+static constexpr int kBlock = 128;
+
+// max |.| with non-finite elements left out
+__device__ __forceinline__ float finite_abs(float x) {
+  const float a = fabsf(x);
+  return a <= 3.402823466e38f ? a : 0.f;      // false for NaN
+}
+
+// scale byte of a block whose largest finite magnitude is `amax`: 448 = 0.875 * 2^9
+__device__ __forceinline__ int scale_byte(float amax) {
+  int e;
+  const float m = frexpf(amax, &e);
+  const int q = e - 9 + (m > 0.875f ? 1 : 0);
+  return amax > 0.f ? (q < -126 ? 1 : q + 127) : 127;
+}
+__device__ __forceinline__ float scale_of(int byte) { return __uint_as_float((unsigned)byte << 23); }            // 2^q
+__device__ __forceinline__ float inverse_scale(int byte) { return __uint_as_float((unsigned)(254 - byte) << 23); }  // 2^-q
+
+// four elements as codes, `inv` = 2^-q; |x inv| <= 448, so the conversion never meets its overflow
+__device__ __forceinline__ unsigned encode4(float a, float b, float c, float d, float inv) {
+  int r = __builtin_amdgcn_cvt_pk_fp8_f32(a * inv, b * inv, 0, false);
+  r = __builtin_amdgcn_cvt_pk_fp8_f32(c * inv, d * inv, r, true);
+  return (unsigned)r;
+}
+// What the conversion is given for x: an infinity must not reach it (it may clamp), so NaN takes its place, and magnitudes past
+// 240 2^120 - which only the topmost scale meets - are held there.
+__device__ __forceinline__ float encodable(float x) {
+  const float top = 0x1.ep+127f;      // 240 2^120
+  const float a = fabsf(x);
+  return a <= top ? x : a <= 3.402823466e38f ? copysignf(top, x) : __uint_as_float(0x7fc00000u);
+}
+
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void decode4(unsigned c, float s, float* v) {
+  const f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);
+  v[0] = lo[0] * s;
+  v[1] = lo[1] * s;
+  v[2] = hi[0] * s;
+  v[3] = hi[1] * s;
+}
+
+// blocks along a row of K elements, and the row of scale bytes up to whole dwords
+__host__ __device__ __forceinline__ int row_blocks(int K) { return (K + kBlock - 1) / kBlock; }
+__host__ __device__ __forceinline__ int scale_stride(int K) { return (row_blocks(K) + 3) & ~3; }
+
+}  // namespace hecka

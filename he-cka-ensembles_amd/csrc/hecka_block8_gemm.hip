@@ -1,0 +1,568 @@
+// Products of 8-bit blocks (block8.hpp) on the matrix cores (hecka_block8_linear / _linear_token / _wgrad; include/hecka.h).
+#include "block8.hpp"
+#include "hecka_host.hpp"
+
+namespace hecka {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4v __attribute__((ext_vector_type(4)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) void* lds_ptr;
+typedef __attribute__((address_space(3))) i16x4* lds_i16x4;
+typedef const __attribute__((address_space(1))) void* global_ptr;
+
+// eight codes as bf16 times their scale: exact, a code has four significant bits (and 2^-133, the smallest bf16, is below 2^-9 2^-124)
+__device__ __forceinline__ bf16x8 widen8(unsigned lo, unsigned hi, float s) {
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, true);
+  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, true);
+  bf16x8 r = {a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+  return r;
+}
+
+// Workgroup id -> tile.  Ids go round the eight XCDs; each XCD gets a contiguous run of tiles, walked in bands of up to eight
+// row tiles, so that the operands which the tiles in flight on one XCD share stay in that XCD's L2.
+__device__ __forceinline__ void place(int id, int total, int tn, int to, int& m, int& in, int& io) {
+  const int q = total >> 3, r = total & 7, xcd = id & 7, at = id >> 3;
+  int t = xcd < r ? xcd * (q + 1) + at : r * (q + 1) + (xcd - r) * q + at;
+  const int per = tn * to;
+  m = t / per;
+  t -= m * per;
+  const int band = t / (8 * to), first = band * 8, rows = tn - first < 8 ? tn - first : 8;
+  t -= band * 8 * to;
+  in = first + t % rows;
+  io = t / rows;
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// y[m][n][o] = alpha sum_k x8[m][n][k] w8[m][o][k] + beta bias[m][o]
+//
+// A workgroup of WO x WN waves owns BO x BN outputs; per step, 128 codes (one block) of each of its rows come straight from
+// memory into LDS (no registers), one step ahead of the products.  LDS rows are 128 bytes; the 16-byte piece c of row r sits
+// at piece c ^ (r & 7), so that the sixteen rows which a fragment read touches fall on different banks.
+// The weights are the first operand, so that a lane ends up with four neighbouring outputs of one row.
+// EXACT = false: the scaled fp8 instruction takes both scales as bytes.  It adds groups of eight products aligned to the
+//   largest, keeping 13 bits below its leading one (measured; 1.5e-5 of the result for normal values, whatever K), against
+//   a half step of 2^-8 of a bf16 result and 2^-11 of an fp16 one - so 16-bit results take it.
+// EXACT = true (fp32 results): the codes are widened to bf16 on their way out of LDS - exact - and the bf16 instruction
+//   adds their products in fp32 (1.4e-7 at K = 8192), at half the rate.
+// ------------------------------------------------------------------------------------------------------------------
+template <class T, bool EXACT, int BO, int BN, int WO, int WN>
+__global__ __launch_bounds__(64 * WO * WN) void block8_linear_kernel(
+    const unsigned char* __restrict__ x, const unsigned char* __restrict__ xs, long long xstride, long long xsstride,
+    const unsigned char* __restrict__ w, const unsigned char* __restrict__ ws, int N, int O, int nblk,
+    const float* __restrict__ bias, float alpha, float beta, T* __restrict__ y, int tiles_n, int tiles_o) {
+  constexpr int NWAVE = WO * WN, TO = BO / WO / 16, TN = BN / WN / 16;
+  static_assert(BO / WO <= kBlock, "a wave's weight rows lie in one 128 x 128 block");
+  __shared__ __attribute__((aligned(1024))) unsigned char sm[2][(BO + BN) * kBlock];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wo = wave % WO, wn = wave / WO, l16 = lane & 15, g = lane >> 4;
+  int m, tn, to;
+  place(blockIdx.x, gridDim.x, tiles_n, tiles_o, m, tn, to);
+  const int n0 = tn * BN, o0 = to * BO, sstride = (nblk + 3) & ~3;
+  const long long K = (long long)nblk * kBlock;
+  x += m * xstride;
+  xs += m * xsstride;
+  w += (long long)m * O * K;
+  ws += (long long)m * ((O + kBlock - 1) / kBlock) * sstride;
+
+  // what this lane loads: row (i NWAVE + wave) 8 + lane / 8 of each operand's tile, rows behind the end repeat the last one
+  constexpr int LO = BO / 8 / NWAVE, LN = BN / 8 / NWAVE;
+  const unsigned char *pw[LO], *px[LN];
+  const int piece = ((lane & 7) ^ (lane >> 3)) * 16;
+#pragma unroll
+  for (int i = 0; i < LO; ++i) {
+    const int o = o0 + (i * NWAVE + wave) * 8 + (lane >> 3);
+    pw[i] = w + (long long)(o < O ? o : O - 1) * K + piece;
+  }
+#pragma unroll
+  for (int i = 0; i < LN; ++i) {
+    const int n = n0 + (i * NWAVE + wave) * 8 + (lane >> 3);
+    px[i] = x + (long long)(n < N ? n : N - 1) * K + piece;
+  }
+  auto fetch = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < LO; ++i) {
+      __builtin_amdgcn_global_load_lds((global_ptr)pw[i], (lds_ptr)(sm[buf] + (i * NWAVE + wave) * 1024), 16, 0, 0);
+      pw[i] += kBlock;
+    }
+#pragma unroll
+    for (int i = 0; i < LN; ++i) {
+      __builtin_amdgcn_global_load_lds((global_ptr)px[i], (lds_ptr)(sm[buf] + BO * kBlock + (i * NWAVE + wave) * 1024), 16, 0, 0);
+      px[i] += kBlock;
+    }
+  };
+  // scales: four steps' bytes per dword, one dword per row tile and lane (x), one for the wave's weight block
+  const unsigned* pxs[TN];
+  unsigned sx[TN];
+#pragma unroll
+  for (int j = 0; j < TN; ++j) {
+    const int n = n0 + (wn * TN + j) * 16 + l16;
+    pxs[j] = reinterpret_cast<const unsigned*>(xs + (long long)(n < N ? n : N - 1) * sstride);
+  }
+  int ob = (o0 + wo * TO * 16) / kBlock;
+  if (ob * kBlock >= O) ob = (O - 1) / kBlock;
+  const unsigned* pws = reinterpret_cast<const unsigned*>(ws + (long long)ob * sstride);
+  unsigned sw = 0;
+
+  f32x4v acc[TO][TN];
+#pragma unroll
+  for (int i = 0; i < TO; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = f32x4v{0.f, 0.f, 0.f, 0.f};
+
+  fetch(0);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  for (int kb = 0; kb < nblk; ++kb) {
+    const int buf = kb & 1, sh = (kb & 3) * 8;
+    if ((kb & 3) == 0) {
+#pragma unroll
+      for (int j = 0; j < TN; ++j) sx[j] = pxs[j][kb >> 2];
+      sw = pws[kb >> 2];
+    }
+    if (kb + 1 < nblk) fetch(buf ^ 1);
+    const unsigned char* fo = sm[buf] + (wo * TO * 16 + l16) * kBlock + ((g ^ (l16 & 7)) * 16);
+    const unsigned char* fn = sm[buf] + BO * kBlock + (wn * TN * 16 + l16) * kBlock + ((g ^ (l16 & 7)) * 16);
+    const int flip = ((g ^ (l16 & 7)) & 4) ? -64 : 64;      // piece g + 4 of the same row
+    if constexpr (!EXACT) {
+      i32x8 fx[TN];
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const i32x4 a = *reinterpret_cast<const i32x4*>(fn + j * 2048), b = *reinterpret_cast<const i32x4*>(fn + flip + j * 2048);
+        fx[j] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+      }
+#pragma unroll
+      for (int i = 0; i < TO; ++i) {
+        const i32x4 a = *reinterpret_cast<const i32x4*>(fo + i * 2048), b = *reinterpret_cast<const i32x4*>(fo + flip + i * 2048);
+        const i32x8 fw = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw, fx[j], acc[i][j], 0, 0, 0, (int)(sw >> sh), 0, (int)(sx[j] >> sh));
+      }
+    } else {
+      const float vw = scale_of((sw >> sh) & 255);
+      float vx[TN];
+#pragma unroll
+      for (int j = 0; j < TN; ++j) vx[j] = scale_of((sx[j] >> sh) & 255);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        i32x4 cx[TN];
+#pragma unroll
+        for (int j = 0; j < TN; ++j) cx[j] = *reinterpret_cast<const i32x4*>(fn + h * flip + j * 2048);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          bf16x8 bx[TN];
+#pragma unroll
+          for (int j = 0; j < TN; ++j) bx[j] = widen8(cx[j][2 * q], cx[j][2 * q + 1], vx[j]);
+#pragma unroll
+          for (int i = 0; i < TO; ++i) {
+            const uint2 c = *reinterpret_cast<const uint2*>(fo + h * flip + i * 2048 + q * 8);
+            const bf16x8 bw = widen8(c.x, c.y, vw);
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bw, bx[j], acc[i][j], 0, 0, 0);
+          }
+        }
+      }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // the next step's codes are in LDS once every wave is here
+    __syncthreads();
+  }
+
+#pragma unroll
+  for (int i = 0; i < TO; ++i) {
+    const int o = o0 + (wo * TO + i) * 16 + 4 * g;
+    float bv[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) bv[e] = bias && o + e < O ? beta * bias[(long long)m * O + o + e] : 0.f;
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const int n = n0 + (wn * TN + j) * 16 + l16;
+      if (n >= N || o >= O) continue;
+      T* yr = y + ((long long)m * N + n) * O + o;
+      struct { T e[4]; } out;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) narrow(fmaf(alpha, acc[i][j][e], bv[e]), out.e[e]);
+      if (o + 4 <= O) {
+        __builtin_memcpy(yr, &out, sizeof(out));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (o + e < O) yr[e] = out.e[e];
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// The same product for up to sixteen rows x (fp32 / bf16 / fp16) that are not in codes yet: one launch.  It reads every weight
+// code once, which is what bounds it, so nothing is staged: a wave takes 16 NT weight rows, its four-way share of the blocks
+// of K, and reads 32 codes per lane and row; each wave makes the codes of x for its blocks by itself (the same codes as
+// hecka_block8_quantize: 32 elements per lane, the maximum over the four lanes of a row).  All products in bf16, exact.
+// The four waves' sums are added in order.
+// ------------------------------------------------------------------------------------------------------------------
+template <class T, int NT>
+__global__ __launch_bounds__(256) void block8_token_kernel(const T* __restrict__ x, long long xstride, int N, int K,
+                                                           const unsigned char* __restrict__ w, const unsigned char* __restrict__ ws,
+                                                           int O, const float* __restrict__ bias, float alpha, float beta,
+                                                           T* __restrict__ y) {
+  __shared__ f32x4v red[4][NT][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g = lane >> 4;
+  const int nblk = row_blocks(K), sstride = scale_stride(K), o0 = blockIdx.x * 16 * NT;
+  const long long m = blockIdx.y, Kp = (long long)nblk * kBlock;
+  x += m * xstride + (long long)(l16 < N ? l16 : N - 1) * K;
+  w += m * O * Kp;
+  const unsigned char* pw[NT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+    const int o = o0 + i * 16 + l16;
+    pw[i] = w + (long long)(o < O ? o : O - 1) * Kp + g * 32;
+  }
+  ws += (m * ((O + kBlock - 1) / kBlock) + o0 / kBlock) * sstride;      // 16 NT <= 128 rows of one block
+  f32x4v acc[NT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) acc[i] = f32x4v{0.f, 0.f, 0.f, 0.f};
+  for (int kb = wave; kb < nblk; kb += 4) {
+    i32x4 c[NT][2];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      c[i][0] = *reinterpret_cast<const i32x4*>(pw[i] + (long long)kb * kBlock);
+      c[i][1] = *reinterpret_cast<const i32x4*>(pw[i] + (long long)kb * kBlock + 16);
+    }
+    float v[32], a = 0.f;
+#pragma unroll
+    for (int j = 0; j < 32 / Piece<T>::N; ++j) {
+      const Piece<T> p = load_piece(x, kb * kBlock + g * 32 + j * Piece<T>::N, K);
+#pragma unroll
+      for (int i = 0; i < Piece<T>::N; ++i) {
+        v[j * Piece<T>::N + i] = widen(p.e[i]);
+        a = fmaxf(a, finite_abs(v[j * Piece<T>::N + i]));
+      }
+    }
+    a = fmaxf(a, __shfl_xor(a, 16));
+    a = fmaxf(a, __shfl_xor(a, 32));
+    const int byte = scale_byte(a);
+    const float inv = inverse_scale(byte), sx = scale_of(byte), sw = scale_of(ws[kb]);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[q * 8 + i] = encodable(v[q * 8 + i]);
+      const bf16x8 bx = widen8(encode4(v[q * 8], v[q * 8 + 1], v[q * 8 + 2], v[q * 8 + 3], inv),
+                               encode4(v[q * 8 + 4], v[q * 8 + 5], v[q * 8 + 6], v[q * 8 + 7], inv), sx);
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const bf16x8 bw = widen8(c[i][q >> 1][(q & 1) * 2], c[i][q >> 1][(q & 1) * 2 + 1], sw);
+        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bw, bx, acc[i], 0, 0, 0);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NT; ++i) red[wave][i][lane] = acc[i];
+  __syncthreads();
+  for (int i = wave; i < NT; i += 4) {
+    f32x4v s = red[0][i][lane];
+#pragma unroll
+    for (int k = 1; k < 4; ++k) s += red[k][i][lane];
+    const int o = o0 + i * 16 + 4 * g;
+    if (l16 < N) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (o + e < O) narrow(fmaf(alpha, s[e], bias ? beta * bias[m * O + o + e] : 0.f), y[(m * N + l16) * O + o + e]);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// dW[m][o][i] = alpha sum_n dy[m][n][o] x8[m][n][i],  db[m][o] = beta sum_n dy[m][n][o]
+//
+// The sum runs down the rows of both operands.  A step stages 32 rows n of each in LDS as bf16, row major, and the
+// transposing LDS read hands every lane four rows of its column at a time.  x8's codes are widened times their scale (exact);
+// dy is split exactly into TERMS bf16 terms by cutting (bf16 1, fp16 2, fp32 3 terms of eight significant bits), every term
+// multiplies x: the products are exact and added in fp32.  db: the sums of dy are one more product with a column of ones, made
+// by the waves that hold the first columns i.
+// LDS rows hold units of 16 columns (32 bytes); unit u of row n sits at u ^ (n & 3): a transposing read takes one unit of
+// four rows, which then lie on different banks.
+// Few tiles (small O x I): the rows are cut into pieces by blockIdx.y, whose sums a second kernel adds up in order.
+// ------------------------------------------------------------------------------------------------------------------
+template <int TERMS>
+__device__ __forceinline__ void cut(const float* v, unsigned (*out)[2]) {      // four floats -> TERMS x four bf16
+  float r[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+  for (int t = 0; t < TERMS; ++t) {
+    out[t][0] = __builtin_amdgcn_perm(__float_as_uint(r[1]), __float_as_uint(r[0]), 0x07060302);
+    out[t][1] = __builtin_amdgcn_perm(__float_as_uint(r[3]), __float_as_uint(r[2]), 0x07060302);
+    if (t + 1 < TERMS) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r[i] -= __uint_as_float(__float_as_uint(r[i]) & 0xffff0000u);
+    }
+  }
+}
+
+template <class T, int TERMS, int BO, int BI, int WO, int WI>
+__global__ __launch_bounds__(64 * WO * WI) void block8_wgrad_kernel(
+    const T* __restrict__ dy, const unsigned char* __restrict__ x, const unsigned char* __restrict__ xs, long long xstride,
+    long long xsstride, int N, int O, int I, float alpha, float beta, float* __restrict__ dW, float* __restrict__ db,
+    int tiles_o, int tiles_i, int rows_per, long long slab, long long bslab) {
+  constexpr int NT = 64 * WO * WI, KS = 32, TO = BO / WO / 16, TI = BI / WI / 16;
+  constexpr int SZ = (TERMS * BO + BI) * KS * 2;
+  __shared__ __attribute__((aligned(16))) unsigned char sm[2][SZ];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), tid = threadIdx.x;
+  const int wi = wave % WI, wo = wave / WI, l16 = lane & 15, g = lane >> 4;
+  int m, to, ti;
+  place(blockIdx.x, gridDim.x, tiles_o, tiles_i, m, to, ti);
+  const int o0 = to * BO, i0 = ti * BI, nblk = row_blocks(I), sstride = scale_stride(I);
+  const int first = blockIdx.y * rows_per, last = first + rows_per < N ? first + rows_per : N;
+  const long long Kp = (long long)nblk * kBlock;
+  dy += (long long)m * N * O;
+  x += m * xstride;
+  xs += m * xsstride;
+  dW += blockIdx.y * slab + (long long)m * O * I;
+  if (db) db += blockIdx.y * bslab + (long long)m * O;
+  const bool sums = db && ti == 0 && wi == 0;
+
+  // staging: dy in 16-byte pieces, codes sixteen at a time
+  constexpr int P = Piece<T>::N, DPR = BO / P, DL = KS * DPR / NT, XPR = BI / 16, XL = KS * XPR / NT;
+  Piece<T> rd[DL];
+  i32x4 rx[XL];
+  int rs[XL];
+  auto load = [&](int k0) {
+#pragma unroll
+    for (int j = 0; j < DL; ++j) {
+      const int t = j * NT + tid, n = first + k0 + t / DPR, o = o0 + (t % DPR) * P;
+      rd[j] = load_piece(dy + (long long)(n < last ? n : 0) * O, n < last ? o : O, O);
+    }
+#pragma unroll
+    for (int j = 0; j < XL; ++j) {
+      const int t = j * NT + tid, n = first + k0 + t / XPR, i = i0 + (t % XPR) * 16;
+      const bool in = n < last && i < Kp;
+      rx[j] = in ? *reinterpret_cast<const i32x4*>(x + n * Kp + i) : i32x4{0, 0, 0, 0};
+      rs[j] = in ? xs[(long long)n * sstride + (i >> 7)] : 127;
+    }
+  };
+  auto stage = [&](int buf) {
+#pragma unroll
+    for (int j = 0; j < DL; ++j) {
+      const int t = j * NT + tid, n = t / DPR, o = (t % DPR) * P;
+      unsigned char* at = sm[buf] + n * BO * 2 + (((o >> 4) ^ (n & 3)) * 32) + (o & 15) * 2;
+      if constexpr (TERMS == 1) {
+        *reinterpret_cast<Piece<T>*>(at) = rd[j];
+      } else {
+#pragma unroll
+        for (int h = 0; h < P / 4; ++h) {
+          float v[4];
+          unsigned c[TERMS][2];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = widen(rd[j].e[h * 4 + e]);
+          cut<TERMS>(v, c);
+#pragma unroll
+          for (int q = 0; q < TERMS; ++q) *reinterpret_cast<uint2*>(at + q * KS * BO * 2 + h * 8) = make_uint2(c[q][0], c[q][1]);
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < XL; ++j) {
+      const int t = j * NT + tid, n = t / XPR, u = t % XPR;
+      const float s = scale_of(rs[j]);
+      bf16x8* at = reinterpret_cast<bf16x8*>(sm[buf] + TERMS * KS * BO * 2 + n * BI * 2 + ((u ^ (n & 3)) * 32));
+      at[0] = widen8(rx[j][0], rx[j][1], s);
+      at[1] = widen8(rx[j][2], rx[j][3], s);
+    }
+  };
+
+  f32x4v acc[TO][TI], accb[TO];
+#pragma unroll
+  for (int i = 0; i < TO; ++i) {
+    accb[i] = f32x4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < TI; ++j) acc[i][j] = f32x4v{0.f, 0.f, 0.f, 0.f};
+  }
+  bf16x8 ones;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) ones[i] = (__bf16)1.0f;
+
+  // fragment of 16 columns (unit u) out of a tile whose rows are `width` columns: rows 4 g .. 4 g + 3 and 16 more down
+  const int fr = g * 4 + (l16 >> 2), sw = l16 >> 2;
+  auto frag = [&](const unsigned char* tile, int width, int u) {
+    const unsigned char* at = tile + fr * width * 2 + ((u ^ sw) * 32) + (l16 & 3) * 8;
+    const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(at));
+    const i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(at + 16 * width * 2));
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+
+  const int steps = (last - first + KS - 1) / KS;
+  load(0);
+  stage(0);
+  __syncthreads();
+  for (int k = 0; k < steps; ++k) {
+    const int buf = k & 1;
+    if (k + 1 < steps) load((k + 1) * KS);
+    bf16x8 fx[TI];
+#pragma unroll
+    for (int j = 0; j < TI; ++j) fx[j] = frag(sm[buf] + TERMS * KS * BO * 2, BI, wi * TI + j);
+#pragma unroll
+    for (int q = 0; q < TERMS; ++q) {
+#pragma unroll
+      for (int i = 0; i < TO; ++i) {
+        const bf16x8 fd = frag(sm[buf] + q * KS * BO * 2, BO, wo * TO + i);
+#pragma unroll
+        for (int j = 0; j < TI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fx[j], fd, acc[i][j], 0, 0, 0);
+        if (sums) accb[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, fd, accb[i], 0, 0, 0);
+      }
+    }
+    if (k + 1 < steps) stage(buf ^ 1);
+    __syncthreads();
+  }
+
+#pragma unroll
+  for (int i = 0; i < TO; ++i) {
+    const int o = o0 + (wo * TO + i) * 16 + l16;
+    if (o >= O) continue;
+    if (sums && g == 0) db[o] = beta * accb[i][0];
+#pragma unroll
+    for (int j = 0; j < TI; ++j) {
+      const int c = i0 + (wi * TI + j) * 16 + 4 * g;
+      f32x4v v = acc[i][j] * alpha;
+      float* at = dW + (long long)o * I + c;
+      if (c + 4 <= I) {
+        __builtin_memcpy(at, &v, 16);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (c + e < I) at[e] = v[e];
+      }
+    }
+  }
+}
+
+// out[e] = sum over S slabs, in order
+__global__ __launch_bounds__(256) void block8_slabs_kernel(const float* __restrict__ part, int S, long long n, float* __restrict__ out) {
+  for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < n; e += (long long)gridDim.x * 256) {
+    float s = part[e];
+    for (int i = 1; i < S; ++i) s += part[i * n + e];
+    out[e] = s;
+  }
+}
+
+static int cdiv(int a, int b) { return (a + b - 1) / b; }
+
+template <class T, bool EXACT>
+static int linear_run(const void* x, const void* xs, long long xstride, long long xsstride, const void* w, const void* ws, int M,
+                      int N, int O, int nblk, const float* bias, float alpha, float beta, void* y, hipStream_t st) {
+  const int tn = cdiv(N, 128), to = cdiv(O, 128);
+  block8_linear_kernel<T, EXACT, 128, 128, 2, 2><<<dim3((unsigned)(M * tn * to)), 256, 0, st>>>(
+      (const unsigned char*)x, (const unsigned char*)xs, xstride, xsstride, (const unsigned char*)w, (const unsigned char*)ws, N, O,
+      nblk, bias, alpha, beta, (T*)y, tn, to);
+  return check_launch("block8_linear");
+}
+
+template <class T>
+static int token_run(const void* x, long long xstride, int M, int N, int K, const void* w, const void* ws, int O,
+                     const float* bias, float alpha, float beta, void* y, hipStream_t st) {
+  block8_token_kernel<T, 2><<<dim3(cdiv(O, 32), M), 256, 0, st>>>((const T*)x, xstride, N, K, (const unsigned char*)w,
+                                                               (const unsigned char*)ws, O, bias, alpha, beta, (T*)y);
+  return check_launch("block8_token");
+}
+
+struct WgradPlan { int to, ti, splits, rows; };
+static WgradPlan wgrad_plan(int M, int N, int O, int I) {
+  WgradPlan p;
+  p.to = cdiv(O, 128);
+  p.ti = cdiv(I, 128);
+  const long long tiles = (long long)M * p.to * p.ti;
+  // fewer tiles than two per CU: pieces of at least 256 rows until there are
+  long long s = tiles >= 512 ? 1 : 512 / tiles;
+  const int most = cdiv(N, 256);
+  p.splits = (int)(s < most ? s : most);
+  p.rows = cdiv(cdiv(N, p.splits), 32) * 32;
+  p.splits = cdiv(N, p.rows);
+  return p;
+}
+
+template <class T, int TERMS>
+static int wgrad_run(const void* dy, const void* x, const void* xs, long long xstride, long long xsstride, int M, int N, int O,
+                     int I, float alpha, float beta, float* dW, float* db, float* ws, hipStream_t st) {
+  const WgradPlan p = wgrad_plan(M, N, O, I);
+  const long long nw = (long long)M * O * I, nb = (long long)M * O;
+  const bool cut = p.splits > 1;
+  block8_wgrad_kernel<T, TERMS, 128, 128, 2, 2><<<dim3((unsigned)(M * p.to * p.ti), p.splits), 256, 0, st>>>(
+      (const T*)dy, (const unsigned char*)x, (const unsigned char*)xs, xstride, xsstride, N, O, I, alpha, beta, cut ? ws : dW,
+      db ? (cut ? ws + p.splits * nw : db) : nullptr, p.to, p.ti, p.rows, nw, nb);
+  if (cut) {
+    block8_slabs_kernel<<<dim3((unsigned)((nw + 255) / 256 < 2048 ? (nw + 255) / 256 : 2048)), 256, 0, st>>>(ws, p.splits, nw, dW);
+    if (db) block8_slabs_kernel<<<dim3((unsigned)((nb + 255) / 256 < 2048 ? (nb + 255) / 256 : 2048)), 256, 0, st>>>(ws + p.splits * nw, p.splits, nb, db);
+  }
+  return check_launch("block8_wgrad");
+}
+
+static bool bad_type(int dtype) { return dtype != HECKA_DT_F32 && dtype != HECKA_DT_BF16 && dtype != HECKA_DT_F16; }
+// sizes for which every index that the kernels keep in 32 bits fits: sizes below 2^22, tiles below 2^31
+static bool bad_sizes(int M, int N, int O, int I) {
+  const int most = 1 << 22;
+  return M <= 0 || N <= 0 || O <= 0 || I <= 0 || M > 65535 || N > most || O > most || I > most ||
+         (long long)M * cdiv(N, 128) * cdiv(O, 128) > 0x7fffffffLL || (long long)M * cdiv(O, 128) * cdiv(I, 128) > 0x7fffffffLL;
+}
+
+}  // namespace hecka
+
+using namespace hecka;
+
+extern "C" {
+
+int hecka_block8_linear(const void* x, const void* xscales, int x_members, const void* w, const void* wscales, int M, int N, int O,
+                        int I, const float* bias, float alpha, float beta, void* y, int dtype, void* stream) {
+  if (bad_type(dtype)) return fail(HECKA_EINVAL, "block8_linear: unknown dtype%s");
+  if (bad_sizes(M, N, O, I)) return fail(HECKA_EINVAL, "%sblock8_linear: bad size (N = %lld, O = %lld)", "", N, O);
+  if (x_members != M && x_members != 1) return fail(HECKA_EINVAL, "%sblock8_linear: codes of %lld members for %lld", "", x_members, M);
+  if (!x || !xscales || !w || !wscales || !y) return fail(HECKA_EINVAL, "block8_linear: null pointer%s");
+  if (!aligned16(x) || !aligned16(w) || (reinterpret_cast<uintptr_t>(xscales) & 3) || (reinterpret_cast<uintptr_t>(wscales) & 3))
+    return fail(HECKA_EINVAL, "block8_linear: codes need 16-byte alignment, scales 4-byte%s");
+  clear_error();
+  const int nblk = row_blocks(I);
+  const long long xst = x_members == 1 ? 0 : (long long)N * nblk * kBlock, sst = x_members == 1 ? 0 : (long long)N * scale_stride(I);
+  hipStream_t st = (hipStream_t)stream;
+  return dtype == HECKA_DT_F32 ? linear_run<float, true>(x, xscales, xst, sst, w, wscales, M, N, O, nblk, bias, alpha, beta, y, st)
+         : dtype == HECKA_DT_BF16 ? linear_run<Bf16, false>(x, xscales, xst, sst, w, wscales, M, N, O, nblk, bias, alpha, beta, y, st)
+                                  : linear_run<F16, false>(x, xscales, xst, sst, w, wscales, M, N, O, nblk, bias, alpha, beta, y, st);
+}
+
+int hecka_block8_linear_token(const void* x, int dtype, int x_members, const void* w, const void* wscales, int M, int N, int O, int I,
+                              const float* bias, float alpha, float beta, void* y, void* stream) {
+  if (bad_type(dtype)) return fail(HECKA_EINVAL, "block8_linear_token: unknown dtype%s");
+  if (bad_sizes(M, N, O, I) || N > 16) return fail(HECKA_EINVAL, "%sblock8_linear_token: bad size (N = %lld, O = %lld)", "", N, O);
+  if (x_members != M && x_members != 1) return fail(HECKA_EINVAL, "%sblock8_linear_token: rows of %lld members for %lld", "", x_members, M);
+  if (!x || !w || !wscales || !y) return fail(HECKA_EINVAL, "block8_linear_token: null pointer%s");
+  if (!aligned16(w)) return fail(HECKA_EINVAL, "block8_linear_token: codes need 16-byte alignment%s");
+  clear_error();
+  const long long xst = x_members == 1 ? 0 : (long long)N * I;
+  hipStream_t st = (hipStream_t)stream;
+  return dtype == HECKA_DT_F32 ? token_run<float>(x, xst, M, N, I, w, wscales, O, bias, alpha, beta, y, st)
+         : dtype == HECKA_DT_BF16 ? token_run<Bf16>(x, xst, M, N, I, w, wscales, O, bias, alpha, beta, y, st)
+                                  : token_run<F16>(x, xst, M, N, I, w, wscales, O, bias, alpha, beta, y, st);
+}
+
+size_t hecka_block8_wgrad_workspace_bytes(int M, int N, int O, int I) {
+  if (bad_sizes(M, N, O, I)) return 0;
+  const WgradPlan p = wgrad_plan(M, N, O, I);
+  return p.splits > 1 ? (size_t)p.splits * M * O * ((size_t)I + 1) * sizeof(float) : 0;
+}
+
+int hecka_block8_wgrad(const void* dy, int dtype, const void* x, const void* xscales, int x_members, int M, int N, int O, int I,
+                       float alpha, float beta, float* dW, float* db, void* ws, size_t ws_bytes, void* stream) {
+  if (bad_type(dtype)) return fail(HECKA_EINVAL, "block8_wgrad: unknown dtype%s");
+  if (bad_sizes(M, N, O, I)) return fail(HECKA_EINVAL, "%sblock8_wgrad: bad size (N = %lld, O = %lld)", "", N, O);
+  if (x_members != M && x_members != 1) return fail(HECKA_EINVAL, "%sblock8_wgrad: codes of %lld members for %lld", "", x_members, M);
+  if (!dy || !x || !xscales || !dW) return fail(HECKA_EINVAL, "block8_wgrad: null pointer%s");
+  if (!aligned16(x)) return fail(HECKA_EINVAL, "block8_wgrad: codes need 16-byte alignment%s");
+  if ((ws ? ws_bytes : 0) < hecka_block8_wgrad_workspace_bytes(M, N, O, I))
+    return fail(HECKA_EWORKSPACE, "%sblock8_wgrad: workspace too small (%lld bytes given)", "", (long long)ws_bytes);
+  clear_error();
+  const long long xst = x_members == 1 ? 0 : (long long)N * row_blocks(I) * kBlock, sst = x_members == 1 ? 0 : (long long)N * scale_stride(I);
+  hipStream_t st = (hipStream_t)stream;
+  return dtype == HECKA_DT_F32 ? wgrad_run<float, 3>(dy, x, xscales, xst, sst, M, N, O, I, alpha, beta, dW, db, (float*)ws, st)
+         : dtype == HECKA_DT_BF16 ? wgrad_run<Bf16, 1>(dy, x, xscales, xst, sst, M, N, O, I, alpha, beta, dW, db, (float*)ws, st)
+                                  : wgrad_run<F16, 2>(dy, x, xscales, xst, sst, M, N, O, I, alpha, beta, dW, db, (float*)ws, st);
+}
+
+}  // extern "C"

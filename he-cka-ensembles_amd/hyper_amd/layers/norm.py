@@ -6,10 +6,11 @@ and return their gradients as one tensor, and the forward kernel updates the run
 is selected in order; otherwise the selected members' statistics are updated with a handful of [members, C] tensor ops."""
 import torch
 import torch.nn as nn
+from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from ..config import knobs
-from .module import GenModule, ParametersGroup
+from .module import GenModule, ParametersGroup, register_gen_module
 
 
 class _NormAffine(ParametersGroup):
@@ -242,6 +243,135 @@ class _BatchNorm(_NormBase):
                 bufs.update('mean', mean, factor)
                 bufs.update('var', var * (cnt / max(cnt - 1, 1)), factor)
         return self.track_feature(y), y
+
+
+_NORM_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+class _LayerNorm(torch.autograd.Function):
+    """Layer norm of x [G, R, D] (libhecka hecka_layernorm_*).  weight / bias [G, D] fp32; packed: `weight` is the flat
+    parameter row [G, 2 D] (weight | bias), read in place, its gradient returned as one tensor."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, packed):
+        G, R, D = x.shape
+        y = torch.empty_like(x)
+        want = any(ctx.needs_input_grad[:3])
+        mean = torch.empty((G, R), device=x.device, dtype=torch.float32) if want else None
+        rstd = torch.empty_like(mean) if want else None
+        w_ptr = weight.data_ptr() if weight is not None else None
+        b_ptr = w_ptr + 4 * D if packed else bias.data_ptr() if bias is not None else None
+        ptr = lambda t: t.data_ptr() if t is not None else None   # noqa: E731
+        if x.numel():
+            with torch.cuda.device(x.device):
+                _lib.check(_lib.lib().hecka_layernorm_fwd(
+                    x.data_ptr(), _NORM_DTYPES[x.dtype], G, R, D, w_ptr, b_ptr, 2 * D if packed else D, float(eps), y.data_ptr(),
+                    ptr(mean), ptr(rstd), torch.cuda.current_stream(x.device).cuda_stream), 'layernorm_fwd')
+        ctx.save_for_backward(x, mean, rstd, weight)
+        ctx.cfg = (packed, bias is not None)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, mean, rstd, weight = ctx.saved_tensors
+        packed, has_bias = ctx.cfg
+        G, R, D = x.shape
+        dy = dy.contiguous()
+        f32 = dict(device=x.device, dtype=torch.float32)
+        dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
+        dw = db = None
+        if weight is not None and ctx.needs_input_grad[1]:
+            dw = torch.empty((G, 2 * D if packed else D), **f32)
+        if has_bias and ctx.needs_input_grad[2]:
+            db = torch.empty((G, D), **f32)
+        if x.numel() == 0:
+            return dx, dw.zero_() if dw is not None else None, db.zero_() if db is not None else None, None, None
+        ptr = lambda t: t.data_ptr() if t is not None else None   # noqa: E731
+        L = _lib.lib()
+        nbytes = L.hecka_layernorm_bwd_workspace_bytes(G, R, D) if dw is not None or db is not None else 0
+        ws = torch.empty((nbytes // 4,), **f32) if nbytes else None
+        with torch.cuda.device(x.device):
+            _lib.check(L.hecka_layernorm_bwd(
+                dy.data_ptr(), x.data_ptr(), _NORM_DTYPES[x.dtype], mean.data_ptr(), rstd.data_ptr(), G, R, D, ptr(weight),
+                2 * D if packed else D, ptr(dx), ptr(dw), dw.data_ptr() + 4 * D if packed and dw is not None else ptr(db),
+                2 * D if packed else D, ptr(ws), nbytes, torch.cuda.current_stream(x.device).cuda_stream), 'layernorm_bwd')
+        return dx, dw, db, None, None
+
+
+def _check_layer_norm(x, affine):
+    if not torch.is_tensor(x) or not x.is_cuda:
+        raise RuntimeError('hyper_amd layer norm needs GPU tensors; there is no CPU path')
+    if x.dtype not in _NORM_DTYPES:
+        raise TypeError('layer norm takes float32, bfloat16 or float16, got %s' % x.dtype)
+    if x.dim() < 1 or not 0 < x.shape[-1] <= 16384:
+        raise ValueError('layer norm takes rows of 1 to 16384 elements, got %s' % (tuple(x.shape),))
+    for name, t in affine:
+        if t is None:
+            continue
+        if t.device != x.device:
+            raise RuntimeError('layer norm: x on %s, %s on %s' % (x.device, name, t.device))
+        if t.dtype != torch.float32:
+            raise TypeError('layer norm: %s has to be float32, got %s' % (name, t.dtype))
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """Layer norm over the last axis (1 to 16384 elements) of x, fp32 / bf16 / fp16 on the GPU; statistics in fp32.  weight / bias
+    fp32: [D] shared by every row, or [M, D] with x [M, ..., D], a row for each member.  Gradients for x (its dtype), weight and
+    bias (fp32; a shared one's is the sum over the members)."""
+    _check_layer_norm(x, (('weight', weight), ('bias', bias)))
+    D = x.shape[-1]
+    given = [t for t in (weight, bias) if t is not None]
+    if weight is None and bias is not None:
+        raise ValueError('layer norm: a bias needs a weight')
+    if any(t.shape != given[0].shape for t in given):
+        raise ValueError('layer norm: weight %s and bias %s' % (tuple(weight.shape), tuple(bias.shape)))
+    G = 1
+    if given and weight.dim() == 2:
+        if x.dim() < 2 or tuple(weight.shape) != (x.shape[0], D):
+            raise ValueError('layer norm: weight has to be (%d,) or (%s, %d), got %s' % (D, x.shape[0] if x.dim() > 1 else '-', D, tuple(weight.shape)))
+        G = x.shape[0]
+    elif given and tuple(weight.shape) != (D,):
+        raise ValueError('layer norm: weight has to be (%d,) or (members, %d), got %s' % (D, D, tuple(weight.shape)))
+    if G > 65535:
+        raise ValueError('layer norm: at most 65535 members, got %d' % G)
+    row = lambda t: t.reshape(G, D).contiguous() if t is not None else None   # noqa: E731
+    rows = x.numel() // (G * D) if G else 0
+    return _LayerNorm.apply(x.contiguous().view(G, rows, D), row(weight), row(bias), eps, False).view(x.shape)
+
+
+@register_gen_module('layer_norm')
+class LayerNorm(GenModule):
+    """Batched layer norm, every member with its own weight and bias (affine): x [members, samples, ..., num_features].  The
+    reference has none; parameters and naming follow its batched norms (hyper/layers/norm.py:12-46)."""
+
+    def __init__(self, num_features, eps=1e-5, affine=True, track=True):
+        super().__init__(track=track)
+        if not 0 < num_features <= 16384:
+            raise ValueError('LayerNorm takes rows of 1 to 16384 elements, got %d' % num_features)
+        self.num_features, self.eps, self.affine = num_features, eps, affine
+        self.affine_module = _NormAffine(num_features) if affine else None
+
+    def define_generated_modules(self):
+        mod = super().define_generated_modules()
+        if self.affine:
+            mod['affine'] = self.affine_module.define_generated_modules()
+        return mod
+
+    def forward(self, params, input):
+        flat = params['affine']['self'] if self.affine else None
+        _check_layer_norm(input, (('params', flat),))
+        if input.dim() < 2 or input.shape[-1] != self.num_features:
+            raise ValueError('expected (members, ..., %d) input (got %s)' % (self.num_features, tuple(input.shape)))
+        if flat is not None and tuple(flat.shape) != (input.shape[0], 2 * self.num_features):
+            raise ValueError('expected parameters (%d, %d) (got %s)' % (input.shape[0], 2 * self.num_features, tuple(flat.shape)))
+        M = input.shape[0]
+        x = input.contiguous().view(M, input.numel() // max(M * self.num_features, 1), self.num_features)
+        y = _LayerNorm.apply(x, flat.contiguous() if flat is not None else None, None, self.eps, flat is not None).view(input.shape)
+        return self.track_feature(y), y
+
+    def extra_repr(self):
+        return '{num_features}, eps={eps}, affine={affine}'.format(**self.__dict__)
 
 
 class BatchNorm1d(_BatchNorm):

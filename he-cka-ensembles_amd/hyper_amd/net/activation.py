@@ -3,6 +3,7 @@ activation_gamma :48); stock torch elementwise ops."""
 import math
 
 import torch
+from torch.autograd.function import once_differentiable
 
 _H = math.sqrt(2.0) / 2.0
 _C = _H + 0.008274364699
@@ -75,6 +76,36 @@ def crater_maxpool2_eligible(x, kwargs):
 
 def crater_maxpool2(x):
     return _CraterMaxPool2.apply(x)
+
+
+class _Checkpointed(torch.autograd.Function):
+    """y = act(x) in one pass that leaves x in 8-bit blocks; the backward takes the slope at the blocks' values."""
+
+    @staticmethod
+    def forward(ctx, x, act):
+        from .. import block8
+        q, y = block8._quantize(x, act)
+        ctx.save_for_backward(q.codes, q.scales)
+        ctx.cfg = (q.shape, q.dtype, act)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        from .. import block8
+        shape, dtype, act = ctx.cfg
+        return block8._values(block8.Rows8(*ctx.saved_tensors, shape, dtype), dtype, act, dy.contiguous()), None
+
+
+def checkpointed(name, x):
+    """act(x) for 'gelu' (erf form), 'silu', 'tanh', 'sigmoid' or 'crater', its input kept for the backward pass in 8-bit blocks
+    (block8: a byte per element instead of 2 or 4; y is exact, only the slope is taken at the rounded input).  x: fp32 / bf16 /
+    fp16 on the GPU, any shape; blocks run along the last axis."""
+    from .. import block8
+    if name not in block8.ACTIVATIONS:
+        raise ValueError('no 8-bit checkpoint for activation %r: please select from %s' % (name, sorted(block8.ACTIVATIONS)))
+    block8._check(x, 'checkpointed')
+    return _Checkpointed.apply(x, block8.ACTIVATIONS[name])
 
 
 def softstep(x, k=0.2, clamp=True):

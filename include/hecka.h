@@ -522,6 +522,57 @@ int hecka_gram_bwd_multi_f32(int L, const float* const* W, const float* const* X
                              const float* const* xmax, const float* gate, int M, int B, const int* P, float* const* dX,
                              int slice_rows, int slice_members, int gemm_mode, void* stream);
 
+/* Layer norm over the last axis of x [G, R, D] (dtype HECKA_DT_*; D <= 16384), the statistics in fp32:
+ *   y = (x - mean) rstd weight + bias, rstd = 1 / sqrt(mean (x - mean)^2 + eps).
+ * weight / bias (may be NULL): fp32, group g's row at weight + g * wstride (wstride 0: one row for all groups).
+ * mean / rstd (both or neither): [G, R], kept for the backward.  The reference has no layer norm; the batched module beside
+ * its norms (hyper/layers/norm.py:129-224) is hyper_amd.layers.LayerNorm.
+ * backward: dx (dtype), dweight / dbias (fp32 [G, D], rows gstride apart), each may be NULL; ws: hecka_layernorm_bwd_
+ * workspace_bytes (needed when dweight or dbias is given); sums over rows in a fixed order, no atomics. */
+int hecka_layernorm_fwd(const void* x, int dtype, int G, long long R, int D, const float* weight, const float* bias,
+                        long long wstride, float eps, void* y, float* mean, float* rstd, void* stream);
+size_t hecka_layernorm_bwd_workspace_bytes(int G, long long R, int D);
+int hecka_layernorm_bwd(const void* dy, const void* x, int dtype, const float* mean, const float* rstd, int G, long long R,
+                        int D, const float* weight, long long wstride, void* dx, float* dweight, float* dbias,
+                        long long gstride, void* ws, size_t ws_bytes, void* stream);
+
+/* ---- 8-bit blocks: activation checkpoints and products.  No counterpart in the reference (fp32 only). ----
+ * 128 consecutive elements of a row share one power of two s = 2^q, the smallest with max |x| <= 448 s over the block's finite
+ * elements (q >= -126; 0 for a block of zeros); an element is kept as the e4m3 code (OCP, no infinities) nearest to x / s,
+ * ties to even, a NaN or an infinity as NaN; a finite element stays finite (codes end at 240 with the topmost scale, 2^120;
+ * 65536 comes back as 65504 in fp16).  Codes [R, Kp], Kp = K up to whole blocks (zero codes behind K), 16-byte
+ * aligned; scale bytes q + 127 [R, S], S = Kp / 128 up to a multiple of 4 (127 behind the last block).
+ * Weights [M, O, I] share one s over 128 x 128 elements: codes [M, O, Ip], scale bytes [M, ceil(O / 128), S(I)]. */
+#define HECKA_ACT_NONE 0
+#define HECKA_ACT_GELU 1     /* erf form */
+#define HECKA_ACT_SILU 2
+#define HECKA_ACT_TANH 3
+#define HECKA_ACT_SIGMOID 4
+#define HECKA_ACT_CRATER 5   /* hyper/net/activation.py:10 */
+/* codes and scales of R rows of K elements, ld elements apart; act != NONE: also y [R, K] = act(x), in x's dtype. */
+int hecka_block8_quantize(const void* x, int dtype, long long R, int K, long long ld, int act, void* codes, void* scales,
+                          void* y, void* stream);
+/* act == NONE: out [R, K] (dtype) = the values of the codes; else out = dy * act'(values), dy [R, K] (dtype). */
+int hecka_block8_values(const void* codes, const void* scales, const void* dy, int dtype, long long R, int K, int act,
+                        void* out, void* stream);
+/* codes of weights W [M, O, I]; codes_t / scales_t (both or neither): the same codes transposed, [M, I, Op] and
+ * [M, ceil(I / 128), S(O)], for the product with W^T. */
+int hecka_block8_weight(const void* W, int dtype, int M, int O, int I, void* codes, void* scales, void* codes_t,
+                        void* scales_t, void* stream);
+/* y[m][n][o] = alpha sum_i x[m][n][i] w[m][o][i] + beta bias[m][o] (bias fp32, may be NULL) of rows in codes (x_members: M,
+ * or 1 for rows that all members share) and weights in codes; y in dtype.  HECKA_DT_F32: exact products, added in fp32;
+ * 16-bit: fp8 matrix instructions (about 1.5e-5 of the result before its rounding).  Sizes up to 2^22. */
+int hecka_block8_linear(const void* x, const void* xscales, int x_members, const void* w, const void* wscales, int M, int N, int O,
+                        int I, const float* bias, float alpha, float beta, void* y, int dtype, void* stream);
+/* The same from rows x [x_members, N, I] (dtype) that are put into codes on the way, N <= 16: one launch. */
+int hecka_block8_linear_token(const void* x, int dtype, int x_members, const void* w, const void* wscales, int M, int N, int O, int I,
+                              const float* bias, float alpha, float beta, void* y, void* stream);
+/* dW [M, O, I] (fp32) = alpha dy^T x, db [M, O] (fp32, may be NULL) = beta sum_n dy; dy [M, N, O] (dtype), x in codes.  Exact
+ * products, added in fp32, in a fixed order.  ws: hecka_block8_wgrad_workspace_bytes. */
+size_t hecka_block8_wgrad_workspace_bytes(int M, int N, int O, int I);
+int hecka_block8_wgrad(const void* dy, int dtype, const void* x, const void* xscales, int x_members, int M, int N, int O, int I,
+                       float alpha, float beta, float* dW, float* db, void* ws, size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
