@@ -135,7 +135,7 @@ __global__ __launch_bounds__(256) void block8_values_kernel(const unsigned char*
 // maximum, and writes the codes along the rows and - through LDS - along the columns, so that the same codes serve the
 // product with W and the one with its transpose.  LDS rows of 132 bytes: the byte-wise column writes spread over the banks.
 template <class T>
-__global__ __launch_bounds__(256) void block8_weight_kernel(const T* __restrict__ W, int O, int I, unsigned char* __restrict__ codes,
+__global__ __launch_bounds__(256) void block8_weight_kernel(const T* __restrict__ W, int O, int I, long long mstride, unsigned char* __restrict__ codes,
                                                             unsigned char* __restrict__ scales, unsigned char* __restrict__ codes_t,
                                                             unsigned char* __restrict__ scales_t) {
   __shared__ float red[4];
@@ -143,7 +143,7 @@ __global__ __launch_bounds__(256) void block8_weight_kernel(const T* __restrict_
   const int nI = row_blocks(I), nO = row_blocks(O), bi = blockIdx.x, bo = blockIdx.y;
   const long long m = blockIdx.z;
   const int lane16 = threadIdx.x & 15, r0 = threadIdx.x >> 4;      // 16 rows at a time, eight columns per lane
-  const T* Wm = W + m * (long long)O * I;
+  const T* Wm = W + m * mstride;
   float v[8][8], a = 0.f;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
@@ -231,9 +231,9 @@ static int values_run(const void* codes, const void* scales, const void* dy, lon
   return check_launch("block8_values");
 }
 template <class T>
-static int weight_run(const void* W, int M, int O, int I, void* codes, void* scales, void* codes_t, void* scales_t, hipStream_t st) {
+static int weight_run(const void* W, int M, int O, int I, long long mstride, void* codes, void* scales, void* codes_t, void* scales_t, hipStream_t st) {
   block8_weight_kernel<T><<<dim3(row_blocks(I), row_blocks(O), M), 256, 0, st>>>(
-      (const T*)W, O, I, (unsigned char*)codes, (unsigned char*)scales, (unsigned char*)codes_t, (unsigned char*)scales_t);
+      (const T*)W, O, I, mstride, (unsigned char*)codes, (unsigned char*)scales, (unsigned char*)codes_t, (unsigned char*)scales_t);
   return check_launch("block8_weight");
 }
 
@@ -275,18 +275,19 @@ int hecka_block8_values(const void* codes, const void* scales, const void* dy, i
                                   : values_run<F16>(codes, scales, dy, R, K, act, out, st);
 }
 
-int hecka_block8_weight(const void* W, int dtype, int M, int O, int I, void* codes, void* scales, void* codes_t,
+int hecka_block8_weight(const void* W, int dtype, int M, int O, int I, long long mstride, void* codes, void* scales, void* codes_t,
                         void* scales_t, void* stream) {
   if (bad_type(dtype)) return fail(HECKA_EINVAL, "block8_weight: unknown dtype%s");
   if (M <= 0 || M > 65535 || O <= 0 || I <= 0 || O > (65535 << 7) || I > (1 << 30))
     return fail(HECKA_EINVAL, "%sblock8_weight: bad size (O = %lld, I = %lld)", "", O, I);
+  if (M > 1 && mstride < (long long)O * I) return fail(HECKA_EINVAL, "%sblock8_weight: members %lld elements apart", "", mstride);
   if (!W || !codes || !scales || !codes_t != !scales_t) return fail(HECKA_EINVAL, "block8_weight: null pointer%s");
   if (!aligned16(codes) || !aligned16(codes_t)) return fail(HECKA_EINVAL, "block8_weight: codes need 16-byte alignment%s");
   clear_error();
   hipStream_t st = (hipStream_t)stream;
-  return dtype == HECKA_DT_F32 ? weight_run<float>(W, M, O, I, codes, scales, codes_t, scales_t, st)
-         : dtype == HECKA_DT_BF16 ? weight_run<Bf16>(W, M, O, I, codes, scales, codes_t, scales_t, st)
-                                  : weight_run<F16>(W, M, O, I, codes, scales, codes_t, scales_t, st);
+  return dtype == HECKA_DT_F32 ? weight_run<float>(W, M, O, I, mstride, codes, scales, codes_t, scales_t, st)
+         : dtype == HECKA_DT_BF16 ? weight_run<Bf16>(W, M, O, I, mstride, codes, scales, codes_t, scales_t, st)
+                                  : weight_run<F16>(W, M, O, I, mstride, codes, scales, codes_t, scales_t, st);
 }
 
 }  // extern "C"

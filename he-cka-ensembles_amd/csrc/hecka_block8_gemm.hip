@@ -53,7 +53,7 @@ template <class T, bool EXACT, int BO, int BN, int WO, int WN>
 __global__ __launch_bounds__(64 * WO * WN) void block8_linear_kernel(
     const unsigned char* __restrict__ x, const unsigned char* __restrict__ xs, long long xstride, long long xsstride,
     const unsigned char* __restrict__ w, const unsigned char* __restrict__ ws, int N, int O, int nblk,
-    const float* __restrict__ bias, float alpha, float beta, T* __restrict__ y, int tiles_n, int tiles_o) {
+    const float* __restrict__ bias, long long bstride, float alpha, float beta, T* __restrict__ y, int tiles_n, int tiles_o) {
   constexpr int NWAVE = WO * WN, TO = BO / WO / 16, TN = BN / WN / 16;
   static_assert(BO / WO <= kBlock, "a wave's weight rows lie in one 128 x 128 block");
   __shared__ __attribute__((aligned(1024))) unsigned char sm[2][(BO + BN) * kBlock];
@@ -176,7 +176,7 @@ __global__ __launch_bounds__(64 * WO * WN) void block8_linear_kernel(
     const int o = o0 + (wo * TO + i) * 16 + 4 * g;
     float bv[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) bv[e] = bias && o + e < O ? beta * bias[(long long)m * O + o + e] : 0.f;
+    for (int e = 0; e < 4; ++e) bv[e] = bias && o + e < O ? beta * bias[m * bstride + o + e] : 0.f;
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
       const int n = n0 + (wn * TN + j) * 16 + l16;
@@ -206,7 +206,7 @@ __global__ __launch_bounds__(64 * WO * WN) void block8_linear_kernel(
 template <class T, int NT>
 __global__ __launch_bounds__(256) void block8_token_kernel(const T* __restrict__ x, long long xstride, int N, int K,
                                                            const unsigned char* __restrict__ w, const unsigned char* __restrict__ ws,
-                                                           int O, const float* __restrict__ bias, float alpha, float beta,
+                                                           int O, const float* __restrict__ bias, long long bstride, float alpha, float beta,
                                                            T* __restrict__ y) {
   __shared__ f32x4v red[4][NT][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g = lane >> 4;
@@ -269,7 +269,7 @@ __global__ __launch_bounds__(256) void block8_token_kernel(const T* __restrict__
     if (l16 < N) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (o + e < O) narrow(fmaf(alpha, s[e], bias ? beta * bias[m * O + o + e] : 0.f), y[(m * N + l16) * O + o + e]);
+        if (o + e < O) narrow(fmaf(alpha, s[e], bias ? beta * bias[m * bstride + o + e] : 0.f), y[(m * N + l16) * O + o + e]);
     }
   }
 }
@@ -449,19 +449,19 @@ static int cdiv(int a, int b) { return (a + b - 1) / b; }
 
 template <class T, bool EXACT>
 static int linear_run(const void* x, const void* xs, long long xstride, long long xsstride, const void* w, const void* ws, int M,
-                      int N, int O, int nblk, const float* bias, float alpha, float beta, void* y, hipStream_t st) {
+                      int N, int O, int nblk, const float* bias, long long bstride, float alpha, float beta, void* y, hipStream_t st) {
   const int tn = cdiv(N, 128), to = cdiv(O, 128);
   block8_linear_kernel<T, EXACT, 128, 128, 2, 2><<<dim3((unsigned)(M * tn * to)), 256, 0, st>>>(
       (const unsigned char*)x, (const unsigned char*)xs, xstride, xsstride, (const unsigned char*)w, (const unsigned char*)ws, N, O,
-      nblk, bias, alpha, beta, (T*)y, tn, to);
+      nblk, bias, bstride, alpha, beta, (T*)y, tn, to);
   return check_launch("block8_linear");
 }
 
 template <class T>
 static int token_run(const void* x, long long xstride, int M, int N, int K, const void* w, const void* ws, int O,
-                     const float* bias, float alpha, float beta, void* y, hipStream_t st) {
+                     const float* bias, long long bstride, float alpha, float beta, void* y, hipStream_t st) {
   block8_token_kernel<T, 2><<<dim3(cdiv(O, 32), M), 256, 0, st>>>((const T*)x, xstride, N, K, (const unsigned char*)w,
-                                                               (const unsigned char*)ws, O, bias, alpha, beta, (T*)y);
+                                                               (const unsigned char*)ws, O, bias, bstride, alpha, beta, (T*)y);
   return check_launch("block8_token");
 }
 
@@ -511,7 +511,7 @@ using namespace hecka;
 extern "C" {
 
 int hecka_block8_linear(const void* x, const void* xscales, int x_members, const void* w, const void* wscales, int M, int N, int O,
-                        int I, const float* bias, float alpha, float beta, void* y, int dtype, void* stream) {
+                        int I, const float* bias, long long bstride, float alpha, float beta, void* y, int dtype, void* stream) {
   if (bad_type(dtype)) return fail(HECKA_EINVAL, "block8_linear: unknown dtype%s");
   if (bad_sizes(M, N, O, I)) return fail(HECKA_EINVAL, "%sblock8_linear: bad size (N = %lld, O = %lld)", "", N, O);
   if (x_members != M && x_members != 1) return fail(HECKA_EINVAL, "%sblock8_linear: codes of %lld members for %lld", "", x_members, M);
@@ -522,13 +522,13 @@ int hecka_block8_linear(const void* x, const void* xscales, int x_members, const
   const int nblk = row_blocks(I);
   const long long xst = x_members == 1 ? 0 : (long long)N * nblk * kBlock, sst = x_members == 1 ? 0 : (long long)N * scale_stride(I);
   hipStream_t st = (hipStream_t)stream;
-  return dtype == HECKA_DT_F32 ? linear_run<float, true>(x, xscales, xst, sst, w, wscales, M, N, O, nblk, bias, alpha, beta, y, st)
-         : dtype == HECKA_DT_BF16 ? linear_run<Bf16, false>(x, xscales, xst, sst, w, wscales, M, N, O, nblk, bias, alpha, beta, y, st)
-                                  : linear_run<F16, false>(x, xscales, xst, sst, w, wscales, M, N, O, nblk, bias, alpha, beta, y, st);
+  return dtype == HECKA_DT_F32 ? linear_run<float, true>(x, xscales, xst, sst, w, wscales, M, N, O, nblk, bias, bstride, alpha, beta, y, st)
+         : dtype == HECKA_DT_BF16 ? linear_run<Bf16, false>(x, xscales, xst, sst, w, wscales, M, N, O, nblk, bias, bstride, alpha, beta, y, st)
+                                  : linear_run<F16, false>(x, xscales, xst, sst, w, wscales, M, N, O, nblk, bias, bstride, alpha, beta, y, st);
 }
 
 int hecka_block8_linear_token(const void* x, int dtype, int x_members, const void* w, const void* wscales, int M, int N, int O, int I,
-                              const float* bias, float alpha, float beta, void* y, void* stream) {
+                              const float* bias, long long bstride, float alpha, float beta, void* y, void* stream) {
   if (bad_type(dtype)) return fail(HECKA_EINVAL, "block8_linear_token: unknown dtype%s");
   if (bad_sizes(M, N, O, I) || N > 16) return fail(HECKA_EINVAL, "%sblock8_linear_token: bad size (N = %lld, O = %lld)", "", N, O);
   if (x_members != M && x_members != 1) return fail(HECKA_EINVAL, "%sblock8_linear_token: rows of %lld members for %lld", "", x_members, M);
@@ -537,9 +537,9 @@ int hecka_block8_linear_token(const void* x, int dtype, int x_members, const voi
   clear_error();
   const long long xst = x_members == 1 ? 0 : (long long)N * I;
   hipStream_t st = (hipStream_t)stream;
-  return dtype == HECKA_DT_F32 ? token_run<float>(x, xst, M, N, I, w, wscales, O, bias, alpha, beta, y, st)
-         : dtype == HECKA_DT_BF16 ? token_run<Bf16>(x, xst, M, N, I, w, wscales, O, bias, alpha, beta, y, st)
-                                  : token_run<F16>(x, xst, M, N, I, w, wscales, O, bias, alpha, beta, y, st);
+  return dtype == HECKA_DT_F32 ? token_run<float>(x, xst, M, N, I, w, wscales, O, bias, bstride, alpha, beta, y, st)
+         : dtype == HECKA_DT_BF16 ? token_run<Bf16>(x, xst, M, N, I, w, wscales, O, bias, bstride, alpha, beta, y, st)
+                                  : token_run<F16>(x, xst, M, N, I, w, wscales, O, bias, bstride, alpha, beta, y, st);
 }
 
 size_t hecka_block8_wgrad_workspace_bytes(int M, int N, int O, int I) {

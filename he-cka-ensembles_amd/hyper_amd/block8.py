@@ -165,15 +165,17 @@ def quantize_weight(W, transposed=True):
     _check(W, 'block8.quantize_weight')
     if W.dim() != 3 or 0 in W.shape:
         raise ValueError('block8.quantize_weight: needs [members, outputs, inputs] without zero sizes, got %s' % (tuple(W.shape),))
-    W = W.detach().contiguous()
+    W = W.detach()
     M, O, I = W.shape
+    if W.stride()[1:] != (I, 1) or (M > 1 and W.stride(0) < O * I):      # a member's slice of a flat parameter row is read in place
+        W = W.contiguous()
     u8 = dict(device=W.device, dtype=torch.uint8)
     codes = torch.empty((M, O, row_blocks(I) * BLOCK), **u8)
     scales = torch.empty((M, row_blocks(O), scale_stride(I)), **u8)
     codes_t = torch.empty((M, I, row_blocks(O) * BLOCK), **u8) if transposed else None
     scales_t = torch.empty((M, row_blocks(I), scale_stride(O)), **u8) if transposed else None
     with torch.cuda.device(W.device):
-        _lib.check(_lib.lib().hecka_block8_weight(W.data_ptr(), DTYPES[W.dtype], M, O, I, codes.data_ptr(), scales.data_ptr(),
+        _lib.check(_lib.lib().hecka_block8_weight(W.data_ptr(), DTYPES[W.dtype], M, O, I, W.stride(0), codes.data_ptr(), scales.data_ptr(),
                                                   _ptr(codes_t), _ptr(scales_t), _st(W)), 'block8_weight')
     return Weight8(codes, scales, I, codes_t, scales_t)
 
@@ -187,6 +189,14 @@ def _members(q, M, what):
     return M
 
 
+def _bstride(b):
+    return b.stride(0) if b is not None else 0
+
+
+def _bias_rows(b):
+    return b if b is None or b.stride(1) == 1 else b.contiguous()
+
+
 def _product(q, codes, scales, M, O, I, bias, alpha, beta, dtype):
     xm = 1 if len(q.shape) == 2 else M
     N = q.shape[-2]
@@ -194,7 +204,7 @@ def _product(q, codes, scales, M, O, I, bias, alpha, beta, dtype):
     if y.numel():
         with torch.cuda.device(q.device):
             _lib.check(_lib.lib().hecka_block8_linear(q.codes.data_ptr(), q.scales.data_ptr(), xm, codes.data_ptr(), scales.data_ptr(),
-                                                      M, N, O, I, _ptr(bias), float(alpha), float(beta), y.data_ptr(),
+                                                      M, N, O, I, _ptr(bias), _bstride(bias), float(alpha), float(beta), y.data_ptr(),
                                                       DTYPES[dtype], _st(y)), 'block8_linear')
     return y
 
@@ -305,7 +315,7 @@ def linear(x, weight, bias=None, scale=1.0, bias_scale=1.0):
         _same_device(what, x, w, bias)
         N = x.shape[-2]
         _sizes(what, M, N, O, I)
-        b = bias.detach().contiguous() if bias is not None else None
+        b = _bias_rows(bias.detach() if bias is not None else None)
         if isinstance(x, Rows8) or N > 16:
             q = x if isinstance(x, Rows8) else _quantize(x)[0]
             return _product(q, w.codes, w.scales, M, O, I, b, scale, bias_scale, q.dtype)
@@ -314,7 +324,7 @@ def linear(x, weight, bias=None, scale=1.0, bias_scale=1.0):
         if N:
             with torch.cuda.device(x.device):
                 _lib.check(_lib.lib().hecka_block8_linear_token(x.data_ptr(), DTYPES[x.dtype], xm, w.codes.data_ptr(), w.scales.data_ptr(),
-                                                                M, N, O, I, _ptr(b), float(scale), float(bias_scale), y.data_ptr(),
+                                                                M, N, O, I, _ptr(b), _bstride(b), float(scale), float(bias_scale), y.data_ptr(),
                                                                 _st(x)), 'block8_linear_token')
         return y
     _check(x, what)
@@ -328,4 +338,4 @@ def linear(x, weight, bias=None, scale=1.0, bias_scale=1.0):
     _check_bias(what, bias, M, O)
     _same_device(what, x, weight, bias)
     _sizes(what, M, x.shape[-2], O, I)
-    return _Linear8.apply(x, weight, bias.contiguous() if bias is not None else None, float(scale), float(bias_scale))
+    return _Linear8.apply(x, weight, _bias_rows(bias), float(scale), float(bias_scale))

@@ -7,8 +7,9 @@ import math
 import torch
 import torch.nn.functional as F
 import torch.nn.init as init
+from torch.autograd.function import once_differentiable
 
-from .. import _lib, ops
+from .. import _lib, block8, ops
 from ..config import knobs
 from ..net import activation
 from .module import ParametersGroup, register_gen_module
@@ -96,9 +97,60 @@ class BatchedLinear(torch.autograd.Function):
         return dx, dW, db, None, None
 
 
+@ops.mode_aware
+class BatchedLinearCheckpoint(torch.autograd.Function):
+    """BatchedLinear whose saved input is an 8-bit checkpoint (block8: a byte per element instead of four): y and dx are BatchedLinear's,
+    dW = scale dy^T x8 and db come from hecka_block8_wgrad in one launch."""
+
+    @staticmethod
+    def forward(ctx, x, W, b, scale, bias_scale):
+        if not (x.is_cuda and W.is_cuda) or x.dtype != torch.float32 or W.dtype != torch.float32:
+            raise RuntimeError('hyper_amd Linear needs fp32 GPU tensors; there is no CPU path')
+        M, O, I = W.shape
+        shared = x.ndim == 2
+        x, W = x.contiguous(), W.contiguous()
+        N = x.shape[-2]
+        y = _bgemm(x, W, M, N, O, I, 0 if shared else N * I, O * I, False, scale, b.contiguous() if b is not None else None, bias_scale)
+        q = block8.quantize(x) if ctx.needs_input_grad[1] else None
+        ctx.save_for_backward(W if ctx.needs_input_grad[0] else None, *((q.codes, q.scales) if q is not None else (None, None)))
+        ctx.cfg = (scale, bias_scale, tuple(x.shape), tuple(W.shape), b is not None)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        W, codes, scales = ctx.saved_tensors
+        scale, bias_scale, xshape, (M, O, I), has_bias = ctx.cfg
+        dy = dy.contiguous()
+        N = xshape[-2]
+        dx = dW = db = None
+        if ctx.needs_input_grad[0]:
+            dx = _bgemm(dy, W, M, N, I, O, N * O, O * I, True, scale)
+            if len(xshape) == 2:
+                dx = dx.sum(0)
+        want_b = has_bias and ctx.needs_input_grad[2]
+        if ctx.needs_input_grad[1]:
+            dW, db = block8._weight_grad(dy, block8.Rows8(codes, scales, xshape, torch.float32), scale, bias_scale, want_b)
+        elif want_b:
+            db = bias_scale * dy.sum(1)
+        return dx, dW, db, None, None
+
+
 @register_gen_module('linear')
 class Linear(ParametersGroup):
-    def __init__(self, in_features, out_features, bias=True, act=None, gamma=1.0, param_scale='torch', track=True):
+    """checkpoint='e4m3' (not in the reference's signature): what the layer keeps for its backward pass - its input and, for the
+    activations that block8 knows, the activation's - is kept in 8-bit blocks; results are the same, gradients are taken at the
+    blocks' values.  compute='e4m3': the products themselves run on 8-bit blocks of x, W and the gradient (block8.linear; x fp32, bf16
+    or fp16), whose codes of x are the checkpoint."""
+
+    def __init__(self, in_features, out_features, bias=True, act=None, gamma=1.0, param_scale='torch', track=True, compute='fp32',
+                 checkpoint=None):
+        if compute not in ('fp32', 'e4m3'):
+            raise ValueError("compute is 'fp32' or 'e4m3', got %r" % (compute,))
+        if checkpoint not in (None, 'e4m3'):
+            raise ValueError("checkpoint is None or 'e4m3', got %r" % (checkpoint,))
+        self.compute, self.checkpoint = compute, checkpoint
+        self.act_name = act if isinstance(act, str) else None
         self.in_features, self.out_features = in_features, out_features
         self.param_scale, self.bias = param_scale, bias
         if param_scale == 'gamma':
@@ -144,11 +196,19 @@ class Linear(ParametersGroup):
                 'Input has wrong shape %s. Expecting (%d, B, %d)' % (tuple(x.shape), W.shape[0], self.in_features)
         else:
             raise ValueError('Bad x dimension. Got %d' % x.ndim)
-        y = BatchedLinear.apply(x, W, viewed['bias'] if self.bias else None, self.scale, self.bias_scale)
+        b = viewed['bias'] if self.bias else None
+        if self.compute == 'e4m3':
+            y = block8.linear(x, W, b, self.scale, self.bias_scale)
+        else:
+            y = (BatchedLinearCheckpoint if self.checkpoint else BatchedLinear).apply(x, W, b, self.scale, self.bias_scale)
+        if self.checkpoint and self.act_name in block8.ACTIVATIONS:
+            return activation.checkpointed(self.act_name, y)
         return y if self.act is None else self.act(y)
 
     def extra_repr(self):
-        return 'in_features=%d, out_features=%d, activation=%s' % (self.in_features, self.out_features, self.act)
+        return 'in_features=%d, out_features=%d, activation=%s%s%s' % (
+            self.in_features, self.out_features, self.act, ', compute=e4m3' if self.compute != 'fp32' else '',
+            ', checkpoint=e4m3' if self.checkpoint else '')
 
 
 @register_gen_module('final_linear')

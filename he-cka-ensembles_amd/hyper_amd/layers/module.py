@@ -3,6 +3,7 @@
 Activation :348-383, SequentialModule :386-450).  Every module maps (params, x) -> (tracked feature | None, y)
 with x = [members, samples, ...]."""
 import copy
+import functools
 from collections import OrderedDict
 
 import numpy as np
@@ -86,11 +87,19 @@ ACTIVATIONS = {
 
 @register_gen_module('activation')
 class Activation(GenModule):
-    def __init__(self, name, track=True):
+    """checkpoint='e4m3' (not in the reference's signature): the input is kept for the backward pass in 8-bit blocks (gelu, silu, tanh,
+    sigmoid and crater; _act.checkpointed)."""
+
+    def __init__(self, name, track=True, checkpoint=None):
         super().__init__(track=track)
         if isinstance(name, str) and name not in ACTIVATIONS:
             raise ValueError('invalid activation provided. please select from %s' % list(ACTIVATIONS))
         self._fn = ACTIVATIONS[name] if isinstance(name, str) else name
+        if checkpoint is not None:
+            from .. import block8
+            if checkpoint != 'e4m3' or name not in block8.ACTIVATIONS:
+                raise ValueError("checkpoint is None or, for one of %s, 'e4m3': got %r for %r" % (sorted(block8.ACTIVATIONS), checkpoint, name))
+            self._fn = functools.partial(_act.checkpointed, name)
         self._name = name if isinstance(name, str) else type(name).__name__
 
     def _forward(self, viewed, x):

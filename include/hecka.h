@@ -556,17 +556,17 @@ int hecka_block8_quantize(const void* x, int dtype, long long R, int K, long lon
 int hecka_block8_values(const void* codes, const void* scales, const void* dy, int dtype, long long R, int K, int act,
                         void* out, void* stream);
 /* codes of weights W [M, O, I]; codes_t / scales_t (both or neither): the same codes transposed, [M, I, Op] and
- * [M, ceil(I / 128), S(O)], for the product with W^T. */
-int hecka_block8_weight(const void* W, int dtype, int M, int O, int I, void* codes, void* scales, void* codes_t,
+ * [M, ceil(I / 128), S(O)], for the product with W^T.  Members of W are mstride elements apart. */
+int hecka_block8_weight(const void* W, int dtype, int M, int O, int I, long long mstride, void* codes, void* scales, void* codes_t,
                         void* scales_t, void* stream);
-/* y[m][n][o] = alpha sum_i x[m][n][i] w[m][o][i] + beta bias[m][o] (bias fp32, may be NULL) of rows in codes (x_members: M,
+/* y[m][n][o] = alpha sum_i x[m][n][i] w[m][o][i] + beta bias[m][o] (bias fp32, members bstride elements apart, may be NULL) of rows in codes (x_members: M,
  * or 1 for rows that all members share) and weights in codes; y in dtype.  HECKA_DT_F32: exact products, added in fp32;
  * 16-bit: fp8 matrix instructions (about 1.5e-5 of the result before its rounding).  Sizes up to 2^22. */
 int hecka_block8_linear(const void* x, const void* xscales, int x_members, const void* w, const void* wscales, int M, int N, int O,
-                        int I, const float* bias, float alpha, float beta, void* y, int dtype, void* stream);
+                        int I, const float* bias, long long bstride, float alpha, float beta, void* y, int dtype, void* stream);
 /* The same from rows x [x_members, N, I] (dtype) that are put into codes on the way, N <= 16: one launch. */
 int hecka_block8_linear_token(const void* x, int dtype, int x_members, const void* w, const void* wscales, int M, int N, int O, int I,
-                              const float* bias, float alpha, float beta, void* y, void* stream);
+                              const float* bias, long long bstride, float alpha, float beta, void* y, void* stream);
 /* dW [M, O, I] (fp32) = alpha dy^T x, db [M, O] (fp32, may be NULL) = beta sum_n dy; dy [M, N, O] (dtype), x in codes.  Exact
  * products, added in fp32, in a fixed order.  ws: hecka_block8_wgrad_workspace_bytes. */
 size_t hecka_block8_wgrad_workspace_bytes(int M, int N, int O, int I);

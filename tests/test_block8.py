@@ -453,12 +453,13 @@ def test_refusals_without_a_gpu():
     assert L.hecka_block8_quantize(p, 0, 1, 8, 8, 0, odd, p, None, None) == -1
     assert L.hecka_block8_values(p, p, None, 0, 1, 8, 1, p, None) == -1
     assert L.hecka_block8_values(p, p, None, 0, 0, 8, 0, p, None) == -1
-    assert L.hecka_block8_weight(p, 0, 1, 8, 8, p, p, p, None, None) == -1
-    assert L.hecka_block8_weight(p, 0, 0, 8, 8, p, p, None, None, None) == -1
-    assert L.hecka_block8_linear(p, p, 2, p, p, 3, 8, 8, 8, None, 1.0, 0.0, p, 0, None) == -1
-    assert L.hecka_block8_linear(p, p, 1, p, p, 1, 8, 8, (1 << 22) + 1, None, 1.0, 0.0, p, 0, None) == -1
-    assert L.hecka_block8_linear(odd, p, 1, p, p, 1, 8, 8, 8, None, 1.0, 0.0, p, 0, None) == -1
-    assert L.hecka_block8_linear_token(p, 0, 1, p, p, 1, 17, 8, 8, None, 1.0, 0.0, p, None) == -1
+    assert L.hecka_block8_weight(p, 0, 1, 8, 8, 64, p, p, p, None, None) == -1
+    assert L.hecka_block8_weight(p, 0, 2, 8, 8, 63, p, p, None, None, None) == -1
+    assert L.hecka_block8_weight(p, 0, 0, 8, 8, 64, p, p, None, None, None) == -1
+    assert L.hecka_block8_linear(p, p, 2, p, p, 3, 8, 8, 8, None, 0, 1.0, 0.0, p, 0, None) == -1
+    assert L.hecka_block8_linear(p, p, 1, p, p, 1, 8, 8, (1 << 22) + 1, None, 0, 1.0, 0.0, p, 0, None) == -1
+    assert L.hecka_block8_linear(odd, p, 1, p, p, 1, 8, 8, 8, None, 0, 1.0, 0.0, p, 0, None) == -1
+    assert L.hecka_block8_linear_token(p, 0, 1, p, p, 1, 17, 8, 8, None, 0, 1.0, 0.0, p, None) == -1
     assert L.hecka_block8_wgrad(p, 0, p, p, 1, 1, 5000, 8, 8, 1.0, 1.0, p, p, None, 0, None) == -3
     assert L.hecka_block8_wgrad_workspace_bytes(1, 0, 8, 8) == 0
 
