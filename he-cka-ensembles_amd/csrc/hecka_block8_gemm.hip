@@ -12,7 +12,6 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) void* lds_ptr;
 typedef __attribute__((address_space(3))) i16x4* lds_i16x4;
-typedef const __attribute__((address_space(1))) void* global_ptr;
 
 // eight codes as bf16 times their scale: exact, a code has four significant bits (and 2^-133, the smallest bf16, is below 2^-9 2^-124)
 __device__ __forceinline__ bf16x8 widen8(unsigned lo, unsigned hi, float s) {
@@ -20,6 +19,24 @@ __device__ __forceinline__ bf16x8 widen8(unsigned lo, unsigned hi, float s) {
   const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, true);
   bf16x8 r = {a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
   return r;
+}
+
+// Loads that go straight to LDS: lane l's 16 (4) bytes land at base + 16 l (4 l).  As asm, because the compiler, which cannot tell
+// the buffer that is being filled from the one that is being read, would wait for them before every LDS read; they write no
+// register, and whoever issues them waits for them (wait_loads) before the barrier behind which they are read.
+__device__ __forceinline__ unsigned lds_offset(const void* p) { return (unsigned)(uintptr_t)(lds_ptr)(const_cast<void*>(p)); }
+__device__ __forceinline__ void load_lds16(i32x4 rsrc, int voffset, int soffset, unsigned base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+               :: "s"(__builtin_amdgcn_readfirstlane(base)), "v"(voffset), "s"(rsrc), "s"(soffset) : "memory", "m0");
+}
+__device__ __forceinline__ void load_lds4(const void* p, unsigned base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
+               :: "s"(__builtin_amdgcn_readfirstlane(base)), "v"(p) : "memory", "m0");
+}
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ i32x4 buffer_of(const void* p) {      // raw buffer over the 2 GiB from p on
+  const unsigned long long a = (unsigned long long)p;
+  return i32x4{__builtin_amdgcn_readfirstlane((int)(unsigned)a), __builtin_amdgcn_readfirstlane((int)((a >> 32) & 0xffff)), 0x7fffffff, 0x00020000};
 }
 
 // Workgroup id -> tile.  Ids go round the eight XCDs; each XCD gets a contiguous run of tiles, walked in bands of up to eight
@@ -57,6 +74,7 @@ __global__ __launch_bounds__(64 * WO * WN) void block8_linear_kernel(
   constexpr int NWAVE = WO * WN, TO = BO / WO / 16, TN = BN / WN / 16;
   static_assert(BO / WO <= kBlock, "a wave's weight rows lie in one 128 x 128 block");
   __shared__ __attribute__((aligned(1024))) unsigned char sm[2][(BO + BN) * kBlock];
+  __shared__ unsigned sc[2][BO + BN];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wo = wave % WO, wn = wave / WO, l16 = lane & 15, g = lane >> 4;
   int m, tn, to;
@@ -68,44 +86,41 @@ __global__ __launch_bounds__(64 * WO * WN) void block8_linear_kernel(
   w += (long long)m * O * K;
   ws += (long long)m * ((O + kBlock - 1) / kBlock) * sstride;
 
-  // what this lane loads: row (i NWAVE + wave) 8 + lane / 8 of each operand's tile, rows behind the end repeat the last one
+  // what this lane loads: row (i NWAVE + wave) 8 + lane / 8 of each operand's tile, rows behind the end repeat the last one;
+  // offsets from the tile's first row stay below 2^30 (256 rows of at most 2^22), the step is the loads' scalar offset
   constexpr int LO = BO / 8 / NWAVE, LN = BN / 8 / NWAVE;
-  const unsigned char *pw[LO], *px[LN];
+  const i32x4 rw = buffer_of(w + (long long)o0 * K), rx = buffer_of(x + (long long)n0 * K);
+  int vw[LO], vx[LN];
   const int piece = ((lane & 7) ^ (lane >> 3)) * 16;
 #pragma unroll
   for (int i = 0; i < LO; ++i) {
-    const int o = o0 + (i * NWAVE + wave) * 8 + (lane >> 3);
-    pw[i] = w + (long long)(o < O ? o : O - 1) * K + piece;
+    const int r = (i * NWAVE + wave) * 8 + (lane >> 3);
+    vw[i] = (o0 + r < O ? r : O - 1 - o0) * (int)K + piece;
   }
 #pragma unroll
   for (int i = 0; i < LN; ++i) {
-    const int n = n0 + (i * NWAVE + wave) * 8 + (lane >> 3);
-    px[i] = x + (long long)(n < N ? n : N - 1) * K + piece;
+    const int r = (i * NWAVE + wave) * 8 + (lane >> 3);
+    vx[i] = (n0 + r < N ? r : N - 1 - n0) * (int)K + piece;
   }
-  auto fetch = [&](int buf) {
+  // scale bytes of four steps: a dword per row of both tiles, fetched with the first of the four
+  static_assert((BO + BN) == 64 * NWAVE, "one scale dword per thread");
+  const unsigned char* ps;
+  {
+    const int r = wave * 64 + lane;
+    const int o = o0 + r < O ? o0 + r : O - 1, n = n0 + r - BO < N ? n0 + r - BO : N - 1;
+    ps = r < BO ? ws + (long long)(o / kBlock) * sstride : xs + (long long)n * sstride;
+  }
+  const unsigned base = lds_offset(sm);
+  auto fetch = [&](int kb) {
+    const int buf = kb & 1, at = kb * kBlock;
 #pragma unroll
-    for (int i = 0; i < LO; ++i) {
-      __builtin_amdgcn_global_load_lds((global_ptr)pw[i], (lds_ptr)(sm[buf] + (i * NWAVE + wave) * 1024), 16, 0, 0);
-      pw[i] += kBlock;
-    }
+    for (int i = 0; i < LO; ++i)
+      load_lds16(rw, vw[i], at, base + buf * (BO + BN) * kBlock + (i * NWAVE + wave) * 1024);
 #pragma unroll
-    for (int i = 0; i < LN; ++i) {
-      __builtin_amdgcn_global_load_lds((global_ptr)px[i], (lds_ptr)(sm[buf] + BO * kBlock + (i * NWAVE + wave) * 1024), 16, 0, 0);
-      px[i] += kBlock;
-    }
+    for (int i = 0; i < LN; ++i)
+      load_lds16(rx, vx[i], at, base + (buf * (BO + BN) + BO) * kBlock + (i * NWAVE + wave) * 1024);
+    if ((kb & 3) == 0) load_lds4(ps + kb, lds_offset(sc) + ((kb >> 2) & 1) * (BO + BN) * 4 + wave * 256);
   };
-  // scales: four steps' bytes per dword, one dword per row tile and lane (x), one for the wave's weight block
-  const unsigned* pxs[TN];
-  unsigned sx[TN];
-#pragma unroll
-  for (int j = 0; j < TN; ++j) {
-    const int n = n0 + (wn * TN + j) * 16 + l16;
-    pxs[j] = reinterpret_cast<const unsigned*>(xs + (long long)(n < N ? n : N - 1) * sstride);
-  }
-  int ob = (o0 + wo * TO * 16) / kBlock;
-  if (ob * kBlock >= O) ob = (O - 1) / kBlock;
-  const unsigned* pws = reinterpret_cast<const unsigned*>(ws + (long long)ob * sstride);
-  unsigned sw = 0;
 
   f32x4v acc[TO][TN];
 #pragma unroll
@@ -114,19 +129,19 @@ __global__ __launch_bounds__(64 * WO * WN) void block8_linear_kernel(
     for (int j = 0; j < TN; ++j) acc[i][j] = f32x4v{0.f, 0.f, 0.f, 0.f};
 
   fetch(0);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  wait_loads();
   __syncthreads();
   for (int kb = 0; kb < nblk; ++kb) {
     const int buf = kb & 1, sh = (kb & 3) * 8;
-    if ((kb & 3) == 0) {
-#pragma unroll
-      for (int j = 0; j < TN; ++j) sx[j] = pxs[j][kb >> 2];
-      sw = pws[kb >> 2];
-    }
-    if (kb + 1 < nblk) fetch(buf ^ 1);
+    if (kb + 1 < nblk) fetch(kb + 1);
     const unsigned char* fo = sm[buf] + (wo * TO * 16 + l16) * kBlock + ((g ^ (l16 & 7)) * 16);
     const unsigned char* fn = sm[buf] + BO * kBlock + (wn * TN * 16 + l16) * kBlock + ((g ^ (l16 & 7)) * 16);
     const int flip = ((g ^ (l16 & 7)) & 4) ? -64 : 64;      // piece g + 4 of the same row
+    const unsigned* fs = sc[(kb >> 2) & 1];
+    const unsigned sw = fs[wo * TO * 16] >> sh;
+    unsigned sx[TN];
+#pragma unroll
+    for (int j = 0; j < TN; ++j) sx[j] = fs[BO + (wn * TN + j) * 16 + l16] >> sh;
     if constexpr (!EXACT) {
       i32x8 fx[TN];
 #pragma unroll
@@ -140,13 +155,13 @@ __global__ __launch_bounds__(64 * WO * WN) void block8_linear_kernel(
         const i32x8 fw = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
         for (int j = 0; j < TN; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw, fx[j], acc[i][j], 0, 0, 0, (int)(sw >> sh), 0, (int)(sx[j] >> sh));
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw, fx[j], acc[i][j], 0, 0, 0, (int)sw, 0, (int)sx[j]);
       }
     } else {
-      const float vw = scale_of((sw >> sh) & 255);
+      const float vw = scale_of(sw & 255);
       float vx[TN];
 #pragma unroll
-      for (int j = 0; j < TN; ++j) vx[j] = scale_of((sx[j] >> sh) & 255);
+      for (int j = 0; j < TN; ++j) vx[j] = scale_of(sx[j] & 255);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         i32x4 cx[TN];
@@ -167,7 +182,7 @@ __global__ __launch_bounds__(64 * WO * WN) void block8_linear_kernel(
         }
       }
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // the next step's codes are in LDS once every wave is here
+    wait_loads();      // the next step's codes are in LDS once every wave is here
     __syncthreads();
   }
 
@@ -450,10 +465,13 @@ static int cdiv(int a, int b) { return (a + b - 1) / b; }
 template <class T, bool EXACT>
 static int linear_run(const void* x, const void* xs, long long xstride, long long xsstride, const void* w, const void* ws, int M,
                       int N, int O, int nblk, const float* bias, long long bstride, float alpha, float beta, void* y, hipStream_t st) {
-  const int tn = cdiv(N, 128), to = cdiv(O, 128);
-  block8_linear_kernel<T, EXACT, 128, 128, 2, 2><<<dim3((unsigned)(M * tn * to)), 256, 0, st>>>(
-      (const unsigned char*)x, (const unsigned char*)xs, xstride, xsstride, (const unsigned char*)w, (const unsigned char*)ws, N, O,
-      nblk, bias, bstride, alpha, beta, (T*)y, tn, to);
+#define HECKA_LINEAR(B, WO, WN) \
+  block8_linear_kernel<T, EXACT, B, B, WO, WN><<<dim3((unsigned)(M * cdiv(N, B) * cdiv(O, B))), 64 * WO * WN, 0, st>>>( \
+      (const unsigned char*)x, (const unsigned char*)xs, xstride, xsstride, (const unsigned char*)w, (const unsigned char*)ws, N, O, \
+      nblk, bias, bstride, alpha, beta, (T*)y, cdiv(N, B), cdiv(O, B))
+  if ((long long)M * cdiv(N, 256) * cdiv(O, 256) >= 192) HECKA_LINEAR(256, 2, 4);
+  else HECKA_LINEAR(128, 2, 2);
+#undef HECKA_LINEAR
   return check_launch("block8_linear");
 }
 
