@@ -66,61 +66,92 @@ __device__ __forceinline__ void place(int id, int total, int tn, int to, int& m,
 // EXACT = true (fp32 results): the codes are widened to bf16 on their way out of LDS - exact - and the bf16 instruction
 //   adds their products in fp32 (1.4e-7 at K = 8192), at half the rate.
 // ------------------------------------------------------------------------------------------------------------------
-template <class T, bool EXACT, int BO, int BN, int WO, int WN>
-__global__ __launch_bounds__(64 * WO * WN) void block8_linear_kernel(
+template <bool EXACT> struct Raw { typedef i32x8 type; };
+template <> struct Raw<true> { typedef i32x4 type; };
+__device__ __forceinline__ i32x4 half4(i32x8 v, int h) {
+  return h ? __builtin_shufflevector(v, v, 4, 5, 6, 7) : __builtin_shufflevector(v, v, 0, 1, 2, 3);
+}
+// The products as asm: all 256 accumulation registers of a lane are sums here, and the compiler, left to itself, moves sums
+// about to place a result elsewhere than its addend, and the instructions to where they hide nothing.  What an instruction
+// needs then is up to this code: two idle cycles behind a vector instruction that wrote an operand (s_nop 1, free in the shadow
+// of the instruction before), and 18 behind the last product before a sum is read (mfma_settle).
+__device__ __forceinline__ void mfma_fp8(f32x4v& c, i32x8 a, i32x8 b, unsigned sa, unsigned sb) {
+  asm volatile("s_nop 1\n\tv_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0]" : "+a"(c) : "v"(a), "v"(b), "v"(sa), "v"(sb));
+}
+__device__ __forceinline__ void mfma_bf16(f32x4v& c, i32x4 a, i32x4 b) {
+  asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+}
+__device__ __forceinline__ void mfma_settle() { asm volatile("s_nop 15\n\ts_nop 15"); }
+
+template <class T, bool EXACT, int B>
+__global__ __launch_bounds__(256) void block8_linear_kernel(
     const unsigned char* __restrict__ x, const unsigned char* __restrict__ xs, long long xstride, long long xsstride,
     const unsigned char* __restrict__ w, const unsigned char* __restrict__ ws, int N, int O, int nblk,
     const float* __restrict__ bias, long long bstride, float alpha, float beta, T* __restrict__ y, int tiles_n, int tiles_o) {
-  constexpr int NWAVE = WO * WN, TO = BO / WO / 16, TN = BN / WN / 16;
-  static_assert(BO / WO <= kBlock, "a wave's weight rows lie in one 128 x 128 block");
-  __shared__ __attribute__((aligned(1024))) unsigned char sm[2][(BO + BN) * kBlock];
-  __shared__ unsigned sc[2][BO + BN];
+  constexpr int TO = B / 32, TN = B / 32, U = EXACT ? 2 : 1, SYNC = TO / 2, L = B / 32, STAGE = 2 * B * kBlock;
+  __shared__ __attribute__((aligned(1024))) unsigned char sm[2][STAGE];
+  __shared__ unsigned sc[2][2 * B];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wo = wave % WO, wn = wave / WO, l16 = lane & 15, g = lane >> 4;
+  const int wo = wave & 1, wn = wave >> 1, l16 = lane & 15, g = lane >> 4;
   int m, tn, to;
   place(blockIdx.x, gridDim.x, tiles_n, tiles_o, m, tn, to);
-  const int n0 = tn * BN, o0 = to * BO, sstride = (nblk + 3) & ~3;
+  const int n0 = tn * B, o0 = to * B, sstride = (nblk + 3) & ~3;
   const long long K = (long long)nblk * kBlock;
   x += m * xstride;
   xs += m * xsstride;
   w += (long long)m * O * K;
   ws += (long long)m * ((O + kBlock - 1) / kBlock) * sstride;
 
-  // what this lane loads: row (i NWAVE + wave) 8 + lane / 8 of each operand's tile, rows behind the end repeat the last one;
+  // what this lane loads: row (4 i + wave) 8 + lane / 8 of each operand's tile, rows behind the end repeat the last one;
   // offsets from the tile's first row stay below 2^30 (256 rows of at most 2^22), the step is the loads' scalar offset
-  constexpr int LO = BO / 8 / NWAVE, LN = BN / 8 / NWAVE;
   const i32x4 rw = buffer_of(w + (long long)o0 * K), rx = buffer_of(x + (long long)n0 * K);
-  int vw[LO], vx[LN];
+  int vw[L], vx[L];
   const int piece = ((lane & 7) ^ (lane >> 3)) * 16;
 #pragma unroll
-  for (int i = 0; i < LO; ++i) {
-    const int r = (i * NWAVE + wave) * 8 + (lane >> 3);
+  for (int i = 0; i < L; ++i) {
+    const int r = (i * 4 + wave) * 8 + (lane >> 3);
     vw[i] = (o0 + r < O ? r : O - 1 - o0) * (int)K + piece;
-  }
-#pragma unroll
-  for (int i = 0; i < LN; ++i) {
-    const int r = (i * NWAVE + wave) * 8 + (lane >> 3);
     vx[i] = (n0 + r < N ? r : N - 1 - n0) * (int)K + piece;
   }
-  // scale bytes of four steps: a dword per row of both tiles, fetched with the first of the four
-  static_assert((BO + BN) == 64 * NWAVE, "one scale dword per thread");
-  const unsigned char* ps;
+  // scale bytes: a dword holds four steps of a row, fetched with the first of them (a line per row: as dear as a row's codes)
+  constexpr bool SPLIT = B < 256;      // 256 threads, 2 B rows: waves 0, 1 the weights' and 2, 3 those of x, or each thread both
+  const unsigned char *psw, *psx;
   {
-    const int r = wave * 64 + lane;
-    const int o = o0 + r < O ? o0 + r : O - 1, n = n0 + r - BO < N ? n0 + r - BO : N - 1;
-    ps = r < BO ? ws + (long long)(o / kBlock) * sstride : xs + (long long)n * sstride;
+    const int r = threadIdx.x & (B - 1);
+    const int o = o0 + r < O ? o0 + r : O - 1, n = n0 + r < N ? n0 + r : N - 1;
+    psw = ws + (long long)(o / kBlock) * sstride;
+    psx = xs + (long long)n * sstride;
+    if (SPLIT && wave >= 2) psw = psx;
   }
-  const unsigned base = lds_offset(sm);
-  auto fetch = [&](int kb) {
-    const int buf = kb & 1, at = kb * kBlock;
-#pragma unroll
-    for (int i = 0; i < LO; ++i)
-      load_lds16(rw, vw[i], at, base + buf * (BO + BN) * kBlock + (i * NWAVE + wave) * 1024);
-#pragma unroll
-    for (int i = 0; i < LN; ++i)
-      load_lds16(rx, vx[i], at, base + (buf * (BO + BN) + BO) * kBlock + (i * NWAVE + wave) * 1024);
-    if ((kb & 3) == 0) load_lds4(ps + kb, lds_offset(sc) + ((kb >> 2) & 1) * (BO + BN) * 4 + wave * 256);
+  const unsigned base = lds_offset(sm), sbase = lds_offset(sc);
+  // load `part` of the LOADS with which a wave brings in its share of step kb
+  constexpr int LOADS = 2 * L + (SPLIT ? 1 : 2);
+  auto fetch = [&](int part, int kb, int into) {
+    const unsigned to_w = base + into * STAGE + wave * 1024, to_s = sbase + ((kb >> 2) & 1) * 2 * B * 4 + wave * 256;
+    if (part < L) load_lds16(rw, vw[part < L ? part : 0], kb * kBlock, to_w + part * 4096);
+    else if (part < 2 * L) load_lds16(rx, vx[part < 2 * L ? part - L : 0], kb * kBlock, to_w + B * kBlock + (part - L) * 4096);
+    else if (kb & 3) return;
+    else if (part == 2 * L) load_lds4(psw + kb, to_s);
+    else load_lds4(psx + kb, to_s + B * 4);
   };
+
+  // a lane's share of a fragment: pieces g and g + 4 of its row - 32 codes, one instruction's K (fp8), or 16 of them (EXACT: half
+  // a step, two instructions' K once widened)
+  typedef typename Raw<EXACT>::type raw_t;
+  const int swz = (g ^ (l16 & 7)) * 16, flip = (swz & 64) ? -64 : 64;
+  auto raw = [&](int kb, int u, int row) {
+    const unsigned char* at = sm[kb & 1] + (row + l16) * kBlock + swz;
+    if constexpr (EXACT) return *reinterpret_cast<const i32x4*>(at + u * flip);
+    else return __builtin_shufflevector(*reinterpret_cast<const i32x4*>(at), *reinterpret_cast<const i32x4*>(at + flip), 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  auto ready = [&](raw_t r, unsigned s) {      // what the instruction takes; s: the row's scale byte (EXACT)
+    if constexpr (EXACT) {
+      const float f = scale_of(s & 255);
+      return __builtin_shufflevector(__builtin_bit_cast(i32x4, widen8(r[0], r[1], f)), __builtin_bit_cast(i32x4, widen8(r[2], r[3], f)), 0, 1, 2, 3, 4, 5, 6, 7);
+    } else return r;
+  };
+  auto scale_w = [&](int kb) { return sc[(kb >> 2) & 1][wo * TO * 16] >> ((kb & 3) * 8); };
+  auto scale_x = [&](int kb, int j) { return sc[(kb >> 2) & 1][B + (wn * TN + j) * 16 + l16] >> ((kb & 3) * 8); };
 
   f32x4v acc[TO][TN];
 #pragma unroll
@@ -128,85 +159,121 @@ __global__ __launch_bounds__(64 * WO * WN) void block8_linear_kernel(
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = f32x4v{0.f, 0.f, 0.f, 0.f};
 
-  fetch(0);
-  wait_loads();
-  __syncthreads();
-  for (int kb = 0; kb < nblk; ++kb) {
-    const int buf = kb & 1, sh = (kb & 3) * 8;
-    if (kb + 1 < nblk) fetch(kb + 1);
-    const unsigned char* fo = sm[buf] + (wo * TO * 16 + l16) * kBlock + ((g ^ (l16 & 7)) * 16);
-    const unsigned char* fn = sm[buf] + BO * kBlock + (wn * TN * 16 + l16) * kBlock + ((g ^ (l16 & 7)) * 16);
-    const int flip = ((g ^ (l16 & 7)) & 4) ? -64 : 64;      // piece g + 4 of the same row
-    const unsigned* fs = sc[(kb >> 2) & 1];
-    const unsigned sw = fs[wo * TO * 16] >> sh;
-    unsigned sx[TN];
+  // What a unit (a step; EXACT: half a step) holds when it begins: the fragments of all its x rows and of the first row tile of w.
+  struct Unit { i32x8 fx[TN]; raw_t aw; unsigned sw, sx[TN]; };
+  const int rw0 = wo * TO * 16, rx0 = B + wn * TN * 16;
+  // One unit's products, and the next unit's fragments read meanwhile (the last steps' loads repeat what is there).
+  auto unit = [&](int kb, int u, const Unit& c, Unit& n) {
+    const bool turn = u == U - 1;      // the last reads of this step's codes
+    const int nkb = turn ? kb + 1 : kb, nu = turn ? 0 : u + 1;
+    const int far = kb + 2 < nblk ? kb + 2 : nblk - 1;
+    raw_t aw[TO], nx[TN];
+    aw[0] = c.aw;
 #pragma unroll
-    for (int j = 0; j < TN; ++j) sx[j] = fs[BO + (wn * TN + j) * 16 + l16] >> sh;
-    if constexpr (!EXACT) {
-      i32x8 fx[TN];
+    for (int i = 0; i < TO; ++i) {
+      // row tiles ahead of their use: one, and before the turn all that are left
+      if (i < SYNC - 1) aw[i + 1] = raw(kb, u, rw0 + (i + 1) * 16);
+      if (i == SYNC - 1) {
 #pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        const i32x4 a = *reinterpret_cast<const i32x4*>(fn + j * 2048), b = *reinterpret_cast<const i32x4*>(fn + flip + j * 2048);
-        fx[j] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        for (int k = SYNC; k < TO; ++k) aw[k] = raw(kb, u, rw0 + k * 16);
       }
-#pragma unroll
-      for (int i = 0; i < TO; ++i) {
-        const i32x4 a = *reinterpret_cast<const i32x4*>(fo + i * 2048), b = *reinterpret_cast<const i32x4*>(fo + flip + i * 2048);
-        const i32x8 fw = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-        for (int j = 0; j < TN; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw, fx[j], acc[i][j], 0, 0, 0, (int)sw, 0, (int)sx[j]);
+      if (i == SYNC && turn) {
+        wait_loads();      // step kb + 1, under way since the last turn
+        __syncthreads();   // and nobody reads step kb any more
       }
-    } else {
-      const float vw = scale_of(sw & 255);
-      float vx[TN];
+      if (i >= SYNC) {
+        constexpr int PER = TN / (TO - SYNC);
 #pragma unroll
-      for (int j = 0; j < TN; ++j) vx[j] = scale_of(sx[j] & 255);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        i32x4 cx[TN];
-#pragma unroll
-        for (int j = 0; j < TN; ++j) cx[j] = *reinterpret_cast<const i32x4*>(fn + h * flip + j * 2048);
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          bf16x8 bx[TN];
-#pragma unroll
-          for (int j = 0; j < TN; ++j) bx[j] = widen8(cx[j][2 * q], cx[j][2 * q + 1], vx[j]);
-#pragma unroll
-          for (int i = 0; i < TO; ++i) {
-            const uint2 c = *reinterpret_cast<const uint2*>(fo + h * flip + i * 2048 + q * 8);
-            const bf16x8 bw = widen8(c.x, c.y, vw);
-#pragma unroll
-            for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bw, bx[j], acc[i][j], 0, 0, 0);
-          }
+        for (int k = (i - SYNC) * PER; k < (i - SYNC + 1) * PER; ++k) {
+          nx[k] = raw(nkb, nu, rx0 + k * 16);
+          n.sx[k] = turn ? scale_x(nkb, k) : c.sx[k];
+        }
+        if (i == TO - 1) {
+          n.aw = raw(nkb, nu, rw0);
+          n.sw = turn ? scale_w(nkb) : c.sw;
         }
       }
+      __builtin_amdgcn_sched_barrier(0);
+      const i32x8 fw = ready(aw[i], c.sw);
+#pragma unroll
+      for (int e = 0; e < U * TN; ++e) {
+        const int j = e % TN;
+        if constexpr (EXACT) mfma_bf16(acc[i][j], half4(fw, e / TN), half4(c.fx[j], e / TN));
+        else mfma_fp8(acc[i][j], fw, c.fx[j], c.sw, c.sx[j]);
+        // step kb + 2 into the freed buffer: the loads one by one between the products, because a load that finds the queue full
+        // holds up its wave
+        if (turn && i >= SYNC) {
+          constexpr int SLOTS = (TO - SYNC) * U * TN;
+          const int slot = (i - SYNC) * U * TN + e;
+#pragma unroll
+          for (int part = slot * LOADS / SLOTS; part < (slot + 1) * LOADS / SLOTS; ++part) fetch(part, far, kb & 1);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
-    wait_loads();      // the next step's codes are in LDS once every wave is here
-    __syncthreads();
-  }
+#pragma unroll
+    for (int j = 0; j < TN; ++j) n.fx[j] = ready(nx[j], n.sx[j]);
+  };
 
 #pragma unroll
+  for (int part = 0; part < LOADS; ++part) fetch(part, 0, 0);
+#pragma unroll
+  for (int part = 0; part < LOADS; ++part) fetch(part, nblk > 1 ? 1 : 0, 1);
+  wait_loads();
+  __syncthreads();
+  Unit p, q;
+  p.sw = scale_w(0);
+  p.aw = raw(0, 0, rw0);
+#pragma unroll
+  for (int j = 0; j < TN; ++j) {
+    p.sx[j] = scale_x(0, j);
+    p.fx[j] = ready(raw(0, 0, rx0 + j * 16), p.sx[j]);
+  }
+  // two units a turn of the loop, so that what one leaves the other finds in place
+  int kb = 0;
+  for (; kb + 2 <= nblk * U; kb += 2) {
+    unit(EXACT ? kb >> 1 : kb, 0, p, q);
+    unit(EXACT ? kb >> 1 : kb + 1, U - 1, q, p);
+  }
+  if (kb < nblk * U) unit(kb, 0, p, q);
+  wait_loads();      // the last steps' repeated loads write LDS: not past the end of the workgroup
+  mfma_settle();
+#pragma unroll
+  for (int i = 0; i < TO; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) asm volatile("" : "+a"(acc[i][j]));
+
+  // The results, by way of LDS: a lane holds four neighbouring outputs of sixteen rows, a store of a wave should cover whole lines.
+  // Each wave has a quarter of the code buffers for its RP rows of RB bytes, whose 16-byte piece c lies at c ^ (row & MASK).
+  constexpr int RB = B / 2 * (int)sizeof(T), CH = RB / 16, MASK = CH < 16 ? CH - 1 : 15;
+  constexpr int RP = STAGE / 2 / RB < B / 2 ? STAGE / 2 / RB : B / 2;
+  Piece<float> bv[TO];
+#pragma unroll
   for (int i = 0; i < TO; ++i) {
-    const int o = o0 + (wo * TO + i) * 16 + 4 * g;
-    float bv[4];
+    if (bias) bv[i] = load_piece(bias + m * bstride, o0 + (wo * TO + i) * 16 + 4 * g, O);
+    else bv[i] = Piece<float>{};
+  }
+  __syncthreads();
+  unsigned char* mine = &sm[0][0] + wave * (STAGE / 2);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) bv[e] = bias && o + e < O ? beta * bias[m * bstride + o + e] : 0.f;
+  for (int pass = 0; pass < B / 2 / RP; ++pass) {
 #pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      const int n = n0 + (wn * TN + j) * 16 + l16;
-      if (n >= N || o >= O) continue;
-      T* yr = y + ((long long)m * N + n) * O + o;
-      struct { T e[4]; } out;
+    for (int j = 0; j < RP / 16; ++j) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) narrow(fmaf(alpha, acc[i][j][e], bv[e]), out.e[e]);
-      if (o + 4 <= O) {
-        __builtin_memcpy(yr, &out, sizeof(out));
-      } else {
+      for (int i = 0; i < TO; ++i) {
+        struct { T e[4]; } out;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (o + e < O) yr[e] = out.e[e];
+        for (int e = 0; e < 4; ++e) narrow(fmaf(alpha, acc[i][pass * (RP / 16) + j][e], beta * bv[i].e[e]), out.e[e]);
+        const int row = j * 16 + l16, col = (i * 16 + 4 * g) * (int)sizeof(T);
+        __builtin_memcpy(__builtin_assume_aligned(mine + row * RB + (((col >> 4) ^ (row & MASK)) << 4) + (col & 15), sizeof(out)), &out, sizeof(out));
       }
+    }
+#pragma unroll
+    for (int t = 0; t < RP * CH / 64; ++t) {
+      const int row = t * (64 / CH) + lane / CH, c = lane % CH;
+      const Piece<T> v = *reinterpret_cast<const Piece<T>*>(mine + row * RB + ((c ^ (row & MASK)) << 4));
+      const int n = n0 + wn * (B / 2) + pass * RP + row, o = o0 + wo * (B / 2) + c * Piece<T>::N;
+      if (n < N && o < O) store_piece(y + ((long long)m * N + n) * O, o, O, v);
     }
   }
 }
@@ -465,12 +532,12 @@ static int cdiv(int a, int b) { return (a + b - 1) / b; }
 template <class T, bool EXACT>
 static int linear_run(const void* x, const void* xs, long long xstride, long long xsstride, const void* w, const void* ws, int M,
                       int N, int O, int nblk, const float* bias, long long bstride, float alpha, float beta, void* y, hipStream_t st) {
-#define HECKA_LINEAR(B, WO, WN) \
-  block8_linear_kernel<T, EXACT, B, B, WO, WN><<<dim3((unsigned)(M * cdiv(N, B) * cdiv(O, B))), 64 * WO * WN, 0, st>>>( \
+#define HECKA_LINEAR(B) \
+  block8_linear_kernel<T, EXACT, B><<<dim3((unsigned)(M * cdiv(N, B) * cdiv(O, B))), 256, 0, st>>>( \
       (const unsigned char*)x, (const unsigned char*)xs, xstride, xsstride, (const unsigned char*)w, (const unsigned char*)ws, N, O, \
       nblk, bias, bstride, alpha, beta, (T*)y, cdiv(N, B), cdiv(O, B))
-  if ((long long)M * cdiv(N, 256) * cdiv(O, 256) >= 192) HECKA_LINEAR(256, 2, 4);
-  else HECKA_LINEAR(128, 2, 2);
+  if ((long long)M * cdiv(N, 256) * cdiv(O, 256) >= 192) HECKA_LINEAR(256);
+  else HECKA_LINEAR(128);
 #undef HECKA_LINEAR
   return check_launch("block8_linear");
 }
