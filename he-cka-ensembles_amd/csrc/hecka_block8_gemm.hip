@@ -53,6 +53,38 @@ __device__ __forceinline__ void place(int id, int total, int tn, int to, int& m,
   io = t / rows;
 }
 
+// The results of a wave's 16 S x 16 S outputs, by way of LDS: a lane holds four neighbouring columns (row tile i of the first
+// operand) of one row (column tile j), a store of a wave should cover whole lines.  `mine`: BYTES of LDS of this wave's own, for RP
+// rows of RB bytes whose 16-byte piece c lies at c ^ (row & MASK).  out[row][col] = alpha acc + beta bias[col], `rows` x `cols` of
+// them exist.
+template <class T, int S, int BYTES>
+__device__ __forceinline__ void store_tile(const f32x4v (&acc)[S][S], const Piece<float> (&bias)[S], float alpha, float beta,
+                                           unsigned char* mine, T* out, long long ld, int rows, int cols) {
+  constexpr int RB = 16 * S * (int)sizeof(T), CH = RB / 16, MASK = CH < 16 ? CH - 1 : 15, FIT = BYTES / RB;
+  constexpr int RP = FIT >= 16 * S ? 16 * S : FIT >= 64 ? 64 : 32;
+  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int pass = 0; pass < 16 * S / RP; ++pass) {
+#pragma unroll
+    for (int j = 0; j < RP / 16; ++j) {
+#pragma unroll
+      for (int i = 0; i < S; ++i) {
+        struct { T e[4]; } v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) narrow(fmaf(alpha, acc[i][pass * (RP / 16) + j][e], beta * bias[i].e[e]), v.e[e]);
+        const int row = j * 16 + l16, col = (i * 16 + 4 * g) * (int)sizeof(T);
+        __builtin_memcpy(__builtin_assume_aligned(mine + row * RB + (((col >> 4) ^ (row & MASK)) << 4) + (col & 15), sizeof(v)), &v, sizeof(v));
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < RP * CH / 64; ++t) {
+      const int row = t * (64 / CH) + lane / CH, c = lane % CH, r = pass * RP + row, o = c * Piece<T>::N;
+      const Piece<T> v = *reinterpret_cast<const Piece<T>*>(mine + row * RB + ((c ^ (row & MASK)) << 4));
+      if (r < rows && o < cols) store_piece(out + r * ld, o, cols, v);
+    }
+  }
+}
+
 // ------------------------------------------------------------------------------------------------------------------
 // y[m][n][o] = alpha sum_k x8[m][n][k] w8[m][o][k] + beta bias[m][o]
 //
@@ -80,6 +112,10 @@ __device__ __forceinline__ void mfma_fp8(f32x4v& c, i32x8 a, i32x8 b, unsigned s
 }
 __device__ __forceinline__ void mfma_bf16(f32x4v& c, i32x4 a, i32x4 b) {
   asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+}
+// sums in ordinary registers, which the compiler may copy about: done before anything behind it reads them
+__device__ __forceinline__ void mfma_bf16_now(f32x4v& c, i32x4 a, i32x4 b) {
+  asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %2, %0\n\ts_nop 15\n\ts_nop 3" : "+v"(c) : "v"(a), "v"(b));
 }
 __device__ __forceinline__ void mfma_settle() { asm volatile("s_nop 15\n\ts_nop 15"); }
 
@@ -243,10 +279,6 @@ __global__ __launch_bounds__(256) void block8_linear_kernel(
 #pragma unroll
     for (int j = 0; j < TN; ++j) asm volatile("" : "+a"(acc[i][j]));
 
-  // The results, by way of LDS: a lane holds four neighbouring outputs of sixteen rows, a store of a wave should cover whole lines.
-  // Each wave has a quarter of the code buffers for its RP rows of RB bytes, whose 16-byte piece c lies at c ^ (row & MASK).
-  constexpr int RB = B / 2 * (int)sizeof(T), CH = RB / 16, MASK = CH < 16 ? CH - 1 : 15;
-  constexpr int RP = STAGE / 2 / RB < B / 2 ? STAGE / 2 / RB : B / 2;
   Piece<float> bv[TO];
 #pragma unroll
   for (int i = 0; i < TO; ++i) {
@@ -254,28 +286,8 @@ __global__ __launch_bounds__(256) void block8_linear_kernel(
     else bv[i] = Piece<float>{};
   }
   __syncthreads();
-  unsigned char* mine = &sm[0][0] + wave * (STAGE / 2);
-#pragma unroll
-  for (int pass = 0; pass < B / 2 / RP; ++pass) {
-#pragma unroll
-    for (int j = 0; j < RP / 16; ++j) {
-#pragma unroll
-      for (int i = 0; i < TO; ++i) {
-        struct { T e[4]; } out;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) narrow(fmaf(alpha, acc[i][pass * (RP / 16) + j][e], beta * bv[i].e[e]), out.e[e]);
-        const int row = j * 16 + l16, col = (i * 16 + 4 * g) * (int)sizeof(T);
-        __builtin_memcpy(__builtin_assume_aligned(mine + row * RB + (((col >> 4) ^ (row & MASK)) << 4) + (col & 15), sizeof(out)), &out, sizeof(out));
-      }
-    }
-#pragma unroll
-    for (int t = 0; t < RP * CH / 64; ++t) {
-      const int row = t * (64 / CH) + lane / CH, c = lane % CH;
-      const Piece<T> v = *reinterpret_cast<const Piece<T>*>(mine + row * RB + ((c ^ (row & MASK)) << 4));
-      const int n = n0 + wn * (B / 2) + pass * RP + row, o = o0 + wo * (B / 2) + c * Piece<T>::N;
-      if (n < N && o < O) store_piece(y + ((long long)m * N + n) * O, o, O, v);
-    }
-  }
+  const int n1 = n0 + wn * (B / 2), o1 = o0 + wo * (B / 2);
+  store_tile<T, TO, STAGE / 2>(acc, bv, alpha, beta, &sm[0][0] + wave * (STAGE / 2), y + ((long long)m * N + n1) * O + o1, O, N - n1, O - o1);
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -364,8 +376,8 @@ __global__ __launch_bounds__(256) void block8_token_kernel(const T* __restrict__
 // dy is split exactly into TERMS bf16 terms by cutting (bf16 1, fp16 2, fp32 3 terms of eight significant bits), every term
 // multiplies x: the products are exact and added in fp32.  db: the sums of dy are one more product with a column of ones, made
 // by the waves that hold the first columns i.
-// LDS rows hold units of 16 columns (32 bytes); unit u of row n sits at u ^ (n & 3): a transposing read takes one unit of
-// four rows, which then lie on different banks.
+// LDS rows hold units of 16 columns (32 bytes); unit u of row n sits at u ^ (n & 7): a transposing read takes one unit of
+// sixteen rows, eight of which lie on different banks.
 // Few tiles (small O x I): the rows are cut into pieces by blockIdx.y, whose sums a second kernel adds up in order.
 // ------------------------------------------------------------------------------------------------------------------
 template <int TERMS>
@@ -382,140 +394,160 @@ __device__ __forceinline__ void cut(const float* v, unsigned (*out)[2]) {      /
   }
 }
 
-template <class T, int TERMS, int BO, int BI, int WO, int WI>
-__global__ __launch_bounds__(64 * WO * WI) void block8_wgrad_kernel(
+template <class T, int TERMS, int B, bool WHOLE>
+__global__ __launch_bounds__(256) void block8_wgrad_kernel(
     const T* __restrict__ dy, const unsigned char* __restrict__ x, const unsigned char* __restrict__ xs, long long xstride,
     long long xsstride, int N, int O, int I, float alpha, float beta, float* __restrict__ dW, float* __restrict__ db,
     int tiles_o, int tiles_i, int rows_per, long long slab, long long bslab) {
-  constexpr int NT = 64 * WO * WI, KS = 32, TO = BO / WO / 16, TI = BI / WI / 16;
-  constexpr int SZ = (TERMS * BO + BI) * KS * 2;
-  __shared__ __attribute__((aligned(16))) unsigned char sm[2][SZ];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), tid = threadIdx.x;
-  const int wi = wave % WI, wo = wave / WI, l16 = lane & 15, g = lane >> 4;
+  constexpr int KS = TERMS == 1 ? 64 : 32, S = KS / 32, TT = B / 32;      // rows a step, 32-row parts of it, tiles a wave and side
+  constexpr int TILE = KS * B * 2, STAGE = (TERMS + 1) * TILE;
+  __shared__ __attribute__((aligned(1024))) unsigned char sm[2][STAGE];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wi = wave & 1, wo = wave >> 1, l16 = lane & 15, g = lane >> 4;
   int m, to, ti;
   place(blockIdx.x, gridDim.x, tiles_o, tiles_i, m, to, ti);
-  const int o0 = to * BO, i0 = ti * BI, nblk = row_blocks(I), sstride = scale_stride(I);
-  const int first = blockIdx.y * rows_per, last = first + rows_per < N ? first + rows_per : N;
+  const int o0 = to * B, i0 = ti * B, nblk = row_blocks(I), sstride = scale_stride(I);
+  const int first = blockIdx.y * rows_per, last = first + rows_per < N ? first + rows_per : N, steps = (last - first + KS - 1) / KS;
   const long long Kp = (long long)nblk * kBlock;
-  dy += (long long)m * N * O;
-  x += m * xstride;
-  xs += m * xsstride;
-  dW += blockIdx.y * slab + (long long)m * O * I;
-  if (db) db += blockIdx.y * bslab + (long long)m * O;
-  const bool sums = db && ti == 0 && wi == 0;
+  dy += ((long long)m * N + first) * O;
+  x += m * xstride + first * Kp;
+  xs += m * xsstride + (long long)first * sstride;
 
-  // staging: dy in 16-byte pieces, codes sixteen at a time
-  constexpr int P = Piece<T>::N, DPR = BO / P, DL = KS * DPR / NT, XPR = BI / 16, XL = KS * XPR / NT;
+  // Staging: item 0 .. DL - 1 a 16-byte piece of dy, DL .. DL + XL - 1 sixteen codes; a thread holds one of each item for the step
+  // that is two ahead of the products.  WHOLE (dy's rows are whole aligned pieces): buffer loads, zero behind the last row;
+  // columns behind the end are the next row's - they only reach outputs that do not exist.
+  constexpr int P = Piece<T>::N, DPR = B / P, DL = KS * DPR / 256, XPR = B / 16, XL = KS * XPR / 256, ITEMS = DL + XL;
   Piece<T> rd[DL];
   i32x4 rx[XL];
   int rs[XL];
-  auto load = [&](int k0) {
-#pragma unroll
-    for (int j = 0; j < DL; ++j) {
-      const int t = j * NT + tid, n = first + k0 + t / DPR, o = o0 + (t % DPR) * P;
-      rd[j] = load_piece(dy + (long long)(n < last ? n : 0) * O, n < last ? o : O, O);
-    }
-#pragma unroll
-    for (int j = 0; j < XL; ++j) {
-      const int t = j * NT + tid, n = first + k0 + t / XPR, i = i0 + (t % XPR) * 16;
-      const bool in = n < last && i < Kp;
-      rx[j] = in ? *reinterpret_cast<const i32x4*>(x + n * Kp + i) : i32x4{0, 0, 0, 0};
-      rs[j] = in ? xs[(long long)n * sstride + (i >> 7)] : 127;
+  auto load = [&](int item, int step) {
+    const int k0 = step * KS, left = last - first - k0;      // rows from this step's first on (may be none)
+    if (item < DL) {
+      const int t = item * 256 + tid, n = t / DPR, c = (t % DPR) * P;
+      if constexpr (WHOLE) {
+        const long long bytes = (long long)left * O * (long long)sizeof(T) - (long long)o0 * (long long)sizeof(T);
+        const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(dy + (long long)k0 * O + o0), 0, left <= 0 ? 0 : bytes > 0x7fffffff ? 0x7fffffff : (int)bytes, 0x00020000);
+        rd[item] = __builtin_bit_cast(Piece<T>, __builtin_amdgcn_raw_buffer_load_b128(r, (n * O + c) * (int)sizeof(T), 0, 0));
+      } else {
+        rd[item] = load_piece(dy + (long long)(n < left ? k0 + n : 0) * O, n < left ? o0 + c : O, O);
+      }
+    } else {
+      const int j = item - DL, t = j * 256 + tid, n = t / XPR, c = (t % XPR) * 16;
+      const bool in = n < left && i0 + c < Kp;
+      const long long row = in ? k0 + n : 0;
+      const i32x4 v = *reinterpret_cast<const i32x4*>(x + row * Kp + (in ? i0 + c : 0));
+      rx[j] = in ? v : i32x4{0, 0, 0, 0};
+      rs[j] = xs[row * sstride + ((in ? i0 + c : 0) >> 7)];
     }
   };
-  auto stage = [&](int buf) {
-#pragma unroll
-    for (int j = 0; j < DL; ++j) {
-      const int t = j * NT + tid, n = t / DPR, o = (t % DPR) * P;
-      unsigned char* at = sm[buf] + n * BO * 2 + (((o >> 4) ^ (n & 3)) * 32) + (o & 15) * 2;
+  auto stage = [&](int item, int buf) {
+    if (item < DL) {
+      const int t = item * 256 + tid, n = t / DPR, o = (t % DPR) * P;
+      unsigned char* at = sm[buf] + n * B * 2 + (((o >> 4) ^ (n & 7)) * 32) + (o & 15) * 2;
       if constexpr (TERMS == 1) {
-        *reinterpret_cast<Piece<T>*>(at) = rd[j];
+        *reinterpret_cast<Piece<T>*>(at) = rd[item];
       } else {
 #pragma unroll
         for (int h = 0; h < P / 4; ++h) {
           float v[4];
           unsigned c[TERMS][2];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = widen(rd[j].e[h * 4 + e]);
+          for (int e = 0; e < 4; ++e) v[e] = widen(rd[item].e[h * 4 + e]);
           cut<TERMS>(v, c);
 #pragma unroll
-          for (int q = 0; q < TERMS; ++q) *reinterpret_cast<uint2*>(at + q * KS * BO * 2 + h * 8) = make_uint2(c[q][0], c[q][1]);
+          for (int q = 0; q < TERMS; ++q) *reinterpret_cast<uint2*>(at + q * TILE + h * 8) = make_uint2(c[q][0], c[q][1]);
         }
       }
-    }
-#pragma unroll
-    for (int j = 0; j < XL; ++j) {
-      const int t = j * NT + tid, n = t / XPR, u = t % XPR;
+    } else {
+      const int j = item - DL, t = j * 256 + tid, n = t / XPR, u = t % XPR;
       const float s = scale_of(rs[j]);
-      bf16x8* at = reinterpret_cast<bf16x8*>(sm[buf] + TERMS * KS * BO * 2 + n * BI * 2 + ((u ^ (n & 3)) * 32));
+      bf16x8* at = reinterpret_cast<bf16x8*>(sm[buf] + TERMS * TILE + n * B * 2 + ((u ^ (n & 7)) * 32));
       at[0] = widen8(rx[j][0], rx[j][1], s);
       at[1] = widen8(rx[j][2], rx[j][3], s);
     }
   };
 
-  f32x4v acc[TO][TI], accb[TO];
+  f32x4v acc[TT][TT], accb[TT];
 #pragma unroll
-  for (int i = 0; i < TO; ++i) {
+  for (int i = 0; i < TT; ++i) {
     accb[i] = f32x4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < TI; ++j) acc[i][j] = f32x4v{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < TT; ++j) acc[i][j] = f32x4v{0.f, 0.f, 0.f, 0.f};
   }
-  bf16x8 ones;
+  // the column sums: tile t of this workgroup's columns o belongs to one of the workgroups that share them, and there to one wave
+  unsigned sums = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) ones[i] = (__bf16)1.0f;
+  for (int j = 0; j < TT; ++j)
+    if (db && (wo * TT + j) % tiles_i == ti && (((wo * TT + j) / tiles_i) & 1) == wi) sums |= 1u << j;
+  const i32x4 ones = {0x3f803f80, 0x3f803f80, 0x3f803f80, 0x3f803f80};
 
-  // fragment of 16 columns (unit u) out of a tile whose rows are `width` columns: rows 4 g .. 4 g + 3 and 16 more down
-  const int fr = g * 4 + (l16 >> 2), sw = l16 >> 2;
-  auto frag = [&](const unsigned char* tile, int width, int u) {
-    const unsigned char* at = tile + fr * width * 2 + ((u ^ sw) * 32) + (l16 & 3) * 8;
+  // fragment of 16 columns (unit u) of a tile: rows 4 g .. 4 g + 3 and 16 more down
+  const int fr = (g * 4 + (l16 >> 2)) * B * 2 + (l16 & 3) * 8, sw = (g & 1) * 4 + (l16 >> 2);
+  auto frag = [&](const unsigned char* tile, int u) {
+    const unsigned char* at = tile + fr + ((u ^ sw) * 32);
     const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(at));
-    const i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(at + 16 * width * 2));
-    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+    const i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(at + 16 * B * 2));
+    return __builtin_bit_cast(i32x4, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
   };
 
-  const int steps = (last - first + KS - 1) / KS;
-  load(0);
-  stage(0);
+#pragma unroll
+  for (int item = 0; item < ITEMS; ++item) load(item, 0);
+#pragma unroll
+  for (int item = 0; item < ITEMS; ++item) { stage(item, 0); load(item, 1); }
   __syncthreads();
   for (int k = 0; k < steps; ++k) {
-    const int buf = k & 1;
-    if (k + 1 < steps) load((k + 1) * KS);
-    bf16x8 fx[TI];
+    const unsigned char* at = sm[k & 1];
+    i32x4 fx[S][TT], fd[2];
 #pragma unroll
-    for (int j = 0; j < TI; ++j) fx[j] = frag(sm[buf] + TERMS * KS * BO * 2, BI, wi * TI + j);
+    for (int i = 0; i < TT; ++i) fx[0][i] = frag(at + TERMS * TILE, wi * TT + i);
+    fd[0] = frag(at, wo * TT);
+    // groups of TT products: part s, tile j of columns o, term q; each reads the next one's fragment first
+    constexpr int GROUPS = S * TT * TERMS;
 #pragma unroll
-    for (int q = 0; q < TERMS; ++q) {
-#pragma unroll
-      for (int i = 0; i < TO; ++i) {
-        const bf16x8 fd = frag(sm[buf] + q * KS * BO * 2, BO, wo * TO + i);
-#pragma unroll
-        for (int j = 0; j < TI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fx[j], fd, acc[i][j], 0, 0, 0);
-        if (sums) accb[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, fd, accb[i], 0, 0, 0);
+    for (int e = 0; e < GROUPS; ++e) {
+      const int s = e / (TT * TERMS), j = e / TERMS % TT, q = e % TERMS;
+      if (e + 1 < GROUPS) {
+        const int s1 = (e + 1) / (TT * TERMS), j1 = (e + 1) / TERMS % TT, q1 = (e + 1) % TERMS;
+        fd[(e + 1) & 1] = frag(at + q1 * TILE + s1 * 32 * B * 2, wo * TT + j1);
       }
+      if (s + 1 < S && e % (TT * TERMS) < TT) fx[s + 1 < S ? s + 1 : 0][e % TT] = frag(at + TERMS * TILE + (s + 1) * 32 * B * 2, wi * TT + e % TT);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < TT / 2; ++i) mfma_bf16(acc[i][j], fx[s][i], fd[e & 1]);
+      __builtin_amdgcn_sched_barrier(0);
+      // the next step's items into the other buffer, and the loads of the step after it
+#pragma unroll
+      for (int item = e * ITEMS / GROUPS; item < (e + 1) * ITEMS / GROUPS; ++item) {
+        stage(item, (k + 1) & 1);
+        load(item, k + 2);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = TT / 2; i < TT; ++i) mfma_bf16(acc[i][j], fx[s][i], fd[e & 1]);
+      if (sums & (1u << j)) mfma_bf16_now(accb[j], ones, fd[e & 1]);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    if (k + 1 < steps) stage(buf ^ 1);
     __syncthreads();
   }
+  mfma_settle();
+#pragma unroll
+  for (int i = 0; i < TT; ++i) {
+#pragma unroll
+    for (int j = 0; j < TT; ++j) asm volatile("" : "+a"(acc[i][j]));
+  }
 
+  if (g == 0) {
+    float* to_db = db + blockIdx.y * bslab + (long long)m * O;
 #pragma unroll
-  for (int i = 0; i < TO; ++i) {
-    const int o = o0 + (wo * TO + i) * 16 + l16;
-    if (o >= O) continue;
-    if (sums && g == 0) db[o] = beta * accb[i][0];
-#pragma unroll
-    for (int j = 0; j < TI; ++j) {
-      const int c = i0 + (wi * TI + j) * 16 + 4 * g;
-      f32x4v v = acc[i][j] * alpha;
-      float* at = dW + (long long)o * I + c;
-      if (c + 4 <= I) {
-        __builtin_memcpy(at, &v, 16);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (c + e < I) at[e] = v[e];
-      }
+    for (int j = 0; j < TT; ++j) {
+      const int o = o0 + (wo * TT + j) * 16 + l16;
+      if ((sums & (1u << j)) && o < O) to_db[o] = beta * accb[j][0];
     }
   }
+  const Piece<float> none[TT] = {};
+  const int o1 = o0 + wo * (B / 2), i1 = i0 + wi * (B / 2);
+  store_tile<float, TT, STAGE / 2>(acc, none, alpha, 0.f, &sm[0][0] + wave * (STAGE / 2), dW + blockIdx.y * slab + ((long long)m * O + o1) * I + i1,
+                                   I, O - o1, I - i1);
 }
 
 // out[e] = sum over S slabs, in order
@@ -550,17 +582,22 @@ static int token_run(const void* x, long long xstride, int M, int N, int K, cons
   return check_launch("block8_token");
 }
 
-struct WgradPlan { int to, ti, splits, rows; };
-static WgradPlan wgrad_plan(int M, int N, int O, int I) {
+struct WgradPlan { int tile, to, ti, splits, rows; };
+static WgradPlan wgrad_plan(int M, int N, int O, int I, bool whole) {
   WgradPlan p;
-  p.to = cdiv(O, 128);
-  p.ti = cdiv(I, 128);
-  const long long tiles = (long long)M * p.to * p.ti;
-  // fewer tiles than two per CU: pieces of at least 256 rows until there are
-  long long s = tiles >= 512 ? 1 : 512 / tiles;
-  const int most = cdiv(N, 256);
-  p.splits = (int)(s < most ? s : most);
-  p.rows = cdiv(cdiv(N, p.splits), 32) * 32;
+  // 256 x 256 tiles, one workgroup per CU, where they - cut into pieces of at least 512 rows - fill three quarters of the
+  // chip; else, and where dy's rows are not whole 16-byte pieces (guarded loads, for which 256 x 256 leaves no registers),
+  // 128 x 128 tiles, two per CU, in pieces of at least 256 rows
+  for (p.tile = whole ? 256 : 128;; p.tile = 128) {
+    p.to = cdiv(O, p.tile);
+    p.ti = cdiv(I, p.tile);
+    const long long tiles = (long long)M * p.to * p.ti, fill = p.tile == 256 ? 256 : 512;
+    const int most = cdiv(N, 2 * p.tile);
+    const long long s = tiles >= fill ? 1 : fill / tiles;
+    p.splits = (int)(s < most ? s : most);
+    if (p.tile == 128 || (tiles * p.splits >= 192 && O > 128 && I > 128)) break;
+  }
+  p.rows = cdiv(cdiv(N, p.splits), 64) * 64;
   p.splits = cdiv(N, p.rows);
   return p;
 }
@@ -568,12 +605,18 @@ static WgradPlan wgrad_plan(int M, int N, int O, int I) {
 template <class T, int TERMS>
 static int wgrad_run(const void* dy, const void* x, const void* xs, long long xstride, long long xsstride, int M, int N, int O,
                      int I, float alpha, float beta, float* dW, float* db, float* ws, hipStream_t st) {
-  const WgradPlan p = wgrad_plan(M, N, O, I);
+  const bool whole = O % Piece<T>::N == 0 && aligned16(dy);
+  const WgradPlan p = wgrad_plan(M, N, O, I, whole);
   const long long nw = (long long)M * O * I, nb = (long long)M * O;
   const bool cut = p.splits > 1;
-  block8_wgrad_kernel<T, TERMS, 128, 128, 2, 2><<<dim3((unsigned)(M * p.to * p.ti), p.splits), 256, 0, st>>>(
-      (const T*)dy, (const unsigned char*)x, (const unsigned char*)xs, xstride, xsstride, N, O, I, alpha, beta, cut ? ws : dW,
-      db ? (cut ? ws + p.splits * nw : db) : nullptr, p.to, p.ti, p.rows, nw, nb);
+#define HECKA_WGRAD(B, WHOLE) \
+  block8_wgrad_kernel<T, TERMS, B, WHOLE><<<dim3((unsigned)(M * p.to * p.ti), p.splits), 256, 0, st>>>( \
+      (const T*)dy, (const unsigned char*)x, (const unsigned char*)xs, xstride, xsstride, N, O, I, alpha, beta, cut ? ws : dW, \
+      db ? (cut ? ws + p.splits * nw : db) : nullptr, p.to, p.ti, p.rows, nw, nb)
+  if (p.tile == 256) HECKA_WGRAD(256, true);
+  else if (whole) HECKA_WGRAD(128, true);
+  else HECKA_WGRAD(128, false);
+#undef HECKA_WGRAD
   if (cut) {
     block8_slabs_kernel<<<dim3((unsigned)((nw + 255) / 256 < 2048 ? (nw + 255) / 256 : 2048)), 256, 0, st>>>(ws, p.splits, nw, dW);
     if (db) block8_slabs_kernel<<<dim3((unsigned)((nb + 255) / 256 < 2048 ? (nb + 255) / 256 : 2048)), 256, 0, st>>>(ws + p.splits * nw, p.splits, nb, db);
@@ -629,8 +672,13 @@ int hecka_block8_linear_token(const void* x, int dtype, int x_members, const voi
 
 size_t hecka_block8_wgrad_workspace_bytes(int M, int N, int O, int I) {
   if (bad_sizes(M, N, O, I)) return 0;
-  const WgradPlan p = wgrad_plan(M, N, O, I);
-  return p.splits > 1 ? (size_t)p.splits * M * O * ((size_t)I + 1) * sizeof(float) : 0;
+  size_t most = 0;
+  for (bool whole : {false, true}) {
+    const WgradPlan p = wgrad_plan(M, N, O, I, whole);
+    const size_t need = p.splits > 1 ? (size_t)p.splits * M * O * ((size_t)I + 1) * sizeof(float) : 0;
+    most = need > most ? need : most;
+  }
+  return most;
 }
 
 int hecka_block8_wgrad(const void* dy, int dtype, const void* x, const void* xscales, int x_members, int M, int N, int O, int I,
