@@ -380,20 +380,6 @@ __global__ __launch_bounds__(256) void block8_token_kernel(const T* __restrict__
 // sixteen rows, eight of which lie on different banks.
 // Few tiles (small O x I): the rows are cut into pieces by blockIdx.y, whose sums a second kernel adds up in order.
 // ------------------------------------------------------------------------------------------------------------------
-template <int TERMS>
-__device__ __forceinline__ void cut(const float* v, unsigned (*out)[2]) {      // four floats -> TERMS x four bf16
-  float r[4] = {v[0], v[1], v[2], v[3]};
-#pragma unroll
-  for (int t = 0; t < TERMS; ++t) {
-    out[t][0] = __builtin_amdgcn_perm(__float_as_uint(r[1]), __float_as_uint(r[0]), 0x07060302);
-    out[t][1] = __builtin_amdgcn_perm(__float_as_uint(r[3]), __float_as_uint(r[2]), 0x07060302);
-    if (t + 1 < TERMS) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) r[i] -= __uint_as_float(__float_as_uint(r[i]) & 0xffff0000u);
-    }
-  }
-}
-
 template <class T, int TERMS, int B, bool WHOLE>
 __global__ __launch_bounds__(256) void block8_wgrad_kernel(
     const T* __restrict__ dy, const unsigned char* __restrict__ x, const unsigned char* __restrict__ xs, long long xstride,
@@ -413,57 +399,75 @@ __global__ __launch_bounds__(256) void block8_wgrad_kernel(
   x += m * xstride + first * Kp;
   xs += m * xsstride + (long long)first * sstride;
 
-  // Staging: item 0 .. DL - 1 a 16-byte piece of dy, DL .. DL + XL - 1 sixteen codes; a thread holds one of each item for the step
-  // that is two ahead of the products.  WHOLE (dy's rows are whole aligned pieces): buffer loads, zero behind the last row;
-  // columns behind the end are the next row's - they only reach outputs that do not exist.
-  constexpr int P = Piece<T>::N, DPR = B / P, DL = KS * DPR / 256, XPR = B / 16, XL = KS * XPR / 256, ITEMS = DL + XL;
+  // Staging: a thread's share of a step are DL items of dy (16-byte pieces) and XL items of x (sixteen codes).  The registers hold
+  // the step behind the one that is being written to LDS.  WHOLE (dy's rows are whole aligned pieces): buffer loads, zero behind
+  // the last row; columns behind the end are the next row's - they only reach outputs that do not exist.
+  constexpr int P = Piece<T>::N, DPR = B / P, DL = KS * DPR / 256, XPR = B / 16, XL = KS * XPR / 256;
+  constexpr int DROWS = 256 / DPR, XROWS = 256 / XPR;      // rows from one item to the next
   Piece<T> rd[DL];
   i32x4 rx[XL];
   int rs[XL];
-  auto load = [&](int item, int step) {
-    const int k0 = step * KS, left = last - first - k0;      // rows from this step's first on (may be none)
-    if (item < DL) {
-      const int t = item * 256 + tid, n = t / DPR, c = (t % DPR) * P;
-      if constexpr (WHOLE) {
-        const long long bytes = (long long)left * O * (long long)sizeof(T) - (long long)o0 * (long long)sizeof(T);
-        const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(dy + (long long)k0 * O + o0), 0, left <= 0 ? 0 : bytes > 0x7fffffff ? 0x7fffffff : (int)bytes, 0x00020000);
-        rd[item] = __builtin_bit_cast(Piece<T>, __builtin_amdgcn_raw_buffer_load_b128(r, (n * O + c) * (int)sizeof(T), 0, 0));
-      } else {
-        rd[item] = load_piece(dy + (long long)(n < left ? k0 + n : 0) * O, n < left ? o0 + c : O, O);
-      }
+  float r[4];
+  const int dn = tid / DPR, dc = (tid % DPR) * P, xn = tid / XPR, xc = (tid % XPR) * 16;
+  const int dv = (dn * O + dc) * (int)sizeof(T), xv = xn * (int)Kp + xc, sv = xn * sstride + ((i0 + xc) >> 7);
+  struct Source { __amdgpu_buffer_rsrc_t dy, x, xs; long long k0; int left; };
+  auto source = [&](int step) {
+    Source q;
+    q.k0 = (long long)step * KS;
+    const long long left = last - first - q.k0;
+    q.left = left < 0 ? 0 : (int)left;
+    auto buffer = [](const void* p, long long bytes) {
+      return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes < 0 ? 0 : bytes > 0x7fffffff ? 0x7fffffff : (int)bytes, 0x00020000);
+    };
+    q.dy = buffer(dy + q.k0 * O + o0, ((long long)q.left * O - o0) * (long long)sizeof(T));
+    q.x = buffer(x + q.k0 * Kp + i0, q.left * Kp - i0);
+    q.xs = buffer(xs + q.k0 * sstride, (long long)q.left * sstride);
+    return q;
+  };
+  auto load_dy = [&](const Source& q, int item) {
+    if constexpr (WHOLE) {
+      rd[item] = __builtin_bit_cast(Piece<T>, __builtin_amdgcn_raw_buffer_load_b128(q.dy, dv + item * DROWS * O * (int)sizeof(T), 0, 0));
     } else {
-      const int j = item - DL, t = j * 256 + tid, n = t / XPR, c = (t % XPR) * 16;
-      const bool in = n < left && i0 + c < Kp;
-      const long long row = in ? k0 + n : 0;
-      const i32x4 v = *reinterpret_cast<const i32x4*>(x + row * Kp + (in ? i0 + c : 0));
-      rx[j] = in ? v : i32x4{0, 0, 0, 0};
-      rs[j] = xs[row * sstride + ((in ? i0 + c : 0) >> 7)];
+      const int n = dn + item * DROWS;
+      rd[item] = load_piece(dy + (n < q.left ? q.k0 + n : 0) * O, n < q.left ? o0 + dc : O, O);
     }
   };
-  auto stage = [&](int item, int buf) {
-    if (item < DL) {
-      const int t = item * 256 + tid, n = t / DPR, o = (t % DPR) * P;
-      unsigned char* at = sm[buf] + n * B * 2 + (((o >> 4) ^ (n & 7)) * 32) + (o & 15) * 2;
+  auto load_x = [&](const Source& q, int item) {
+    rx[item] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(q.x, xv + item * XROWS * (int)Kp, 0, 0));
+    rs[item] = __builtin_amdgcn_raw_buffer_load_b8(q.xs, sv + item * XROWS * sstride, 0, 0);
+  };
+  // the work on one item in parts of three to six instructions, few enough to pass in the shadow of a product
+  constexpr int QUADS = P / 4, PERQ = TERMS == 1 ? 1 : (sizeof(T) == 2 ? 1 : 0) + 3 * (TERMS - 1) + 1;
+  constexpr int PERD = TERMS == 1 ? 1 : QUADS * PERQ, PARTS = DL * PERD + 2 * XL;
+  auto part = [&](int id, int buf, const Source& next) {
+    if (id < DL * PERD) {
+      const int item = id / PERD, n = dn + item * DROWS;
+      unsigned char* at = sm[buf] + n * B * 2 + (((dc >> 4) ^ (n & 7)) * 32) + (dc & 15) * 2;
       if constexpr (TERMS == 1) {
         *reinterpret_cast<Piece<T>*>(at) = rd[item];
       } else {
+        const int quad = id % PERD / PERQ;
+        int what = id % PERQ;
+        if constexpr (sizeof(T) == 2) --what;
+        if (what == -1 || (sizeof(T) == 4 && what == 0)) {
 #pragma unroll
-        for (int h = 0; h < P / 4; ++h) {
-          float v[4];
-          unsigned c[TERMS][2];
+          for (int e = 0; e < 4; ++e) r[e] = widen(rd[item].e[quad * 4 + e]);
+        }
+        if (what >= 0 && what % 3 == 0) {      // the next term of all four
+          const uint2 c = make_uint2(__builtin_amdgcn_perm(__float_as_uint(r[1]), __float_as_uint(r[0]), 0x07060302),
+                                     __builtin_amdgcn_perm(__float_as_uint(r[3]), __float_as_uint(r[2]), 0x07060302));
+          *reinterpret_cast<uint2*>(at + what / 3 * TILE + quad * 8) = c;
+        } else if (what > 0) {                 // what is left of two of them
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = widen(rd[item].e[h * 4 + e]);
-          cut<TERMS>(v, c);
-#pragma unroll
-          for (int q = 0; q < TERMS; ++q) *reinterpret_cast<uint2*>(at + q * TILE + h * 8) = make_uint2(c[q][0], c[q][1]);
+          for (int e = what % 3 * 2 - 2; e < what % 3 * 2; ++e) r[e] -= __uint_as_float(__float_as_uint(r[e]) & 0xffff0000u);
         }
       }
+      if (id % PERD == PERD - 1) load_dy(next, item);
     } else {
-      const int j = item - DL, t = j * 256 + tid, n = t / XPR, u = t % XPR;
-      const float s = scale_of(rs[j]);
-      bf16x8* at = reinterpret_cast<bf16x8*>(sm[buf] + TERMS * TILE + n * B * 2 + ((u ^ (n & 7)) * 32));
-      at[0] = widen8(rx[j][0], rx[j][1], s);
-      at[1] = widen8(rx[j][2], rx[j][3], s);
+      const int j = (id - DL * PERD) / 2, h = (id - DL * PERD) % 2, n = xn + j * XROWS;
+      bf16x8* at = reinterpret_cast<bf16x8*>(sm[buf] + TERMS * TILE + n * B * 2 + (((xc >> 4) ^ (n & 7)) * 32));
+      at[h] = widen8(rx[j][2 * h], rx[j][2 * h + 1], scale_of(rs[j]));
+      if (h == 1) load_x(next, j);
     }
   };
 
@@ -490,45 +494,73 @@ __global__ __launch_bounds__(256) void block8_wgrad_kernel(
     return __builtin_bit_cast(i32x4, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
   };
 
-#pragma unroll
-  for (int item = 0; item < ITEMS; ++item) load(item, 0);
-#pragma unroll
-  for (int item = 0; item < ITEMS; ++item) { stage(item, 0); load(item, 1); }
-  __syncthreads();
-  for (int k = 0; k < steps; ++k) {
-    const unsigned char* at = sm[k & 1];
-    i32x4 fx[S][TT], fd[2];
-#pragma unroll
-    for (int i = 0; i < TT; ++i) fx[0][i] = frag(at + TERMS * TILE, wi * TT + i);
-    fd[0] = frag(at, wo * TT);
-    // groups of TT products: part s, tile j of columns o, term q; each reads the next one's fragment first
-    constexpr int GROUPS = S * TT * TERMS;
+  // A step is GROUPS groups of TT products: part sub of its rows, tile j of columns o, term q.  At group TURN every fragment that
+  // is left of the step is in registers, the next step is in the other buffer, and the barrier there is the step's only one:
+  // behind it the next step's first fragments are read, and this step's buffer takes the step after that.
+  constexpr int GROUPS = S * TT * TERMS, TURN = GROUPS * 3 / 4, TAIL = GROUPS - TURN, SLOTS = GROUPS * TT;
+  i32x4 fx[2][TT], fd0;
+  Source next;
+  auto frag_d = [&](int e, int buf) {
+    const int sub = e / (TT * TERMS), j = e / TERMS % TT, q = e % TERMS;
+    return frag(sm[buf] + q * TILE + sub * 32 * B * 2, wo * TT + j);
+  };
+  auto frag_x = [&](int i, int sub, int buf) { return frag(sm[buf] + TERMS * TILE + sub * 32 * B * 2, wi * TT + i); };
+  auto step = [&](int k, int buf, int set) {      // set: which half of fx holds the step's first part
+    i32x4 fd[GROUPS];
+    fd[0] = fd0;
 #pragma unroll
     for (int e = 0; e < GROUPS; ++e) {
-      const int s = e / (TT * TERMS), j = e / TERMS % TT, q = e % TERMS;
-      if (e + 1 < GROUPS) {
-        const int s1 = (e + 1) / (TT * TERMS), j1 = (e + 1) / TERMS % TT, q1 = (e + 1) % TERMS;
-        fd[(e + 1) & 1] = frag(at + q1 * TILE + s1 * 32 * B * 2, wo * TT + j1);
+      const int sub = e / (TT * TERMS), j = e / TERMS % TT, hold = S == 2 ? sub : set;
+      if (e < TURN - 1) fd[e + 1] = frag_d(e + 1, buf);
+      if (e == TURN - 1) {
+#pragma unroll
+        for (int f = TURN; f < GROUPS; ++f) fd[f] = frag_d(f, buf);
       }
-      if (s + 1 < S && e % (TT * TERMS) < TT) fx[s + 1 < S ? s + 1 : 0][e % TT] = frag(at + TERMS * TILE + (s + 1) * 32 * B * 2, wi * TT + e % TT);
-      __builtin_amdgcn_sched_barrier(0);
+      if (S == 2 && e < TT) fx[1][e] = frag_x(e, 1, buf);
+      if (e == TURN) {
+        __syncthreads();
+        next = source(k + 3);
+      }
+      if (e >= TURN) {
 #pragma unroll
-      for (int i = 0; i < TT / 2; ++i) mfma_bf16(acc[i][j], fx[s][i], fd[e & 1]);
-      __builtin_amdgcn_sched_barrier(0);
-      // the next step's items into the other buffer, and the loads of the step after it
-#pragma unroll
-      for (int item = e * ITEMS / GROUPS; item < (e + 1) * ITEMS / GROUPS; ++item) {
-        stage(item, (k + 1) & 1);
-        load(item, k + 2);
+        for (int i = (e - TURN) * TT / TAIL; i < (e - TURN + 1) * TT / TAIL; ++i) fx[S == 2 ? 0 : set ^ 1][i] = frag_x(i, 0, buf ^ 1);
+        if (e == GROUPS - 1) fd0 = frag_d(0, buf ^ 1);
       }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int i = TT / 2; i < TT; ++i) mfma_bf16(acc[i][j], fx[s][i], fd[e & 1]);
-      if (sums & (1u << j)) mfma_bf16_now(accb[j], ones, fd[e & 1]);
-      __builtin_amdgcn_sched_barrier(0);
+      for (int i = 0; i < TT; ++i) {
+        mfma_bf16(acc[i][j], fx[hold][i], fd[e]);
+        // from turn to turn: the parts of the next step but one, evenly
+        const int slot = (e < TURN ? e + TAIL : e - TURN) * TT + i;
+#pragma unroll
+        for (int id = slot * PARTS / SLOTS; id < (slot + 1) * PARTS / SLOTS; ++id) part(id, e < TURN ? buf ^ 1 : buf, next);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (sums & (1u << j)) mfma_bf16_now(accb[j], ones, fd[e]);
     }
-    __syncthreads();
+  };
+
+  next = source(0);
+#pragma unroll
+  for (int i = 0; i < DL; ++i) load_dy(next, i);
+#pragma unroll
+  for (int i = 0; i < XL; ++i) load_x(next, i);
+  next = source(1);
+#pragma unroll
+  for (int id = 0; id < PARTS; ++id) part(id, 0, next);
+  next = source(2);
+#pragma unroll
+  for (int id = 0; id < TAIL * TT * PARTS / SLOTS; ++id) part(id, 1, next);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < TT; ++i) fx[0][i] = frag_x(i, 0, 0);
+  fd0 = frag_d(0, 0);
+  // two steps a turn of the loop, so that buffers and fragments have fixed places (a step behind the last one adds zeros)
+  for (int k = 0; k < steps; k += 2) {
+    step(k, 0, 0);
+    step(k + 1, 1, 1);
   }
+  __syncthreads();
   mfma_settle();
 #pragma unroll
   for (int i = 0; i < TT; ++i) {
