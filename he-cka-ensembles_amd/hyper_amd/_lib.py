@@ -140,3 +140,18 @@ def check(rc, what):
     if rc != 0:
         msg = lib().hecka_last_error()
         raise RuntimeError('libhecka %s failed (%d): %s' % (what, rc, msg.decode() if msg else '?'))
+
+
+def call(name, device, *args):
+    """Launch entry point `name` (its last argument is the stream) on `device`'s current stream, with `device` current; raises where
+    it fails.  A few microseconds less of host work than entering torch.cuda.device and building a Stream object per launch."""
+    import torch
+    index = device.index
+    fn = getattr(_lib if _lib is not None else lib(), name)
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc, name)

@@ -42,13 +42,8 @@ def _check(t, what):
 
 
 def _same_device(what, *ts):
-    devs = {t.device for t in ts if t is not None}
-    if len(devs) > 1:
-        raise RuntimeError('%s: tensors on different devices (%s)' % (what, ', '.join(sorted(map(str, devs)))))
-
-
-def _st(t):
-    return torch.cuda.current_stream(t.device).cuda_stream
+    if any(t is not None and t.device != ts[0].device for t in ts):
+        raise RuntimeError('%s: tensors on different devices (%s)' % (what, ', '.join(str(t.device) for t in ts if t is not None)))
 
 
 def _ptr(t):
@@ -101,6 +96,14 @@ class Weight8(object):
         self.codes, self.scales, self.codes_t, self.scales_t = codes, scales, codes_t, scales_t
         self.members, self.outputs, self.inputs = M, O, inputs
 
+    @classmethod
+    def _made(cls, codes, scales, inputs, codes_t, scales_t):
+        """Of tensors that quantize_weight laid out: nothing to check."""
+        w = cls.__new__(cls)
+        w.codes, w.scales, w.codes_t, w.scales_t = codes, scales, codes_t, scales_t
+        w.members, w.outputs, w.inputs = codes.shape[0], codes.shape[1], inputs
+        return w
+
     @property
     def device(self):
         return self.codes.device
@@ -131,18 +134,16 @@ def _quantize(x, act=0):
     codes = torch.empty((R, row_blocks(K) * BLOCK), device=x.device, dtype=torch.uint8)
     scales = torch.empty((R, scale_stride(K)), device=x.device, dtype=torch.uint8)
     if R:
-        with torch.cuda.device(x.device):
-            _lib.check(_lib.lib().hecka_block8_quantize(rows.data_ptr(), DTYPES[x.dtype], R, K, ld, act, codes.data_ptr(),
-                                                        scales.data_ptr(), _ptr(y), _st(x)), 'block8_quantize')
+        _lib.call('hecka_block8_quantize', x.device, rows.data_ptr(), DTYPES[x.dtype], R, K, ld, act, codes.data_ptr(),
+                  scales.data_ptr(), _ptr(y))
     return Rows8(codes, scales, x.shape, x.dtype), y
 
 
 def _values(q, dtype, act=0, dy=None):
     out = torch.empty(q.shape, device=q.device, dtype=dtype)
     if out.numel():
-        with torch.cuda.device(q.device):
-            _lib.check(_lib.lib().hecka_block8_values(q.codes.data_ptr(), q.scales.data_ptr(), _ptr(dy), DTYPES[dtype],
-                                                      q.codes.shape[0], q.shape[-1], act, out.data_ptr(), _st(out)), 'block8_values')
+        _lib.call('hecka_block8_values', q.device, q.codes.data_ptr(), q.scales.data_ptr(), _ptr(dy), DTYPES[dtype],
+                  q.codes.shape[0], q.shape[-1], act, out.data_ptr())
     return out
 
 
@@ -174,10 +175,9 @@ def quantize_weight(W, transposed=True):
     scales = torch.empty((M, row_blocks(O), scale_stride(I)), **u8)
     codes_t = torch.empty((M, I, row_blocks(O) * BLOCK), **u8) if transposed else None
     scales_t = torch.empty((M, row_blocks(I), scale_stride(O)), **u8) if transposed else None
-    with torch.cuda.device(W.device):
-        _lib.check(_lib.lib().hecka_block8_weight(W.data_ptr(), DTYPES[W.dtype], M, O, I, W.stride(0), codes.data_ptr(), scales.data_ptr(),
-                                                  _ptr(codes_t), _ptr(scales_t), _st(W)), 'block8_weight')
-    return Weight8(codes, scales, I, codes_t, scales_t)
+    _lib.call('hecka_block8_weight', W.device, W.data_ptr(), DTYPES[W.dtype], M, O, I, W.stride(0), codes.data_ptr(),
+              scales.data_ptr(), _ptr(codes_t), _ptr(scales_t))
+    return Weight8._made(codes, scales, I, codes_t, scales_t)
 
 
 def _members(q, M, what):
@@ -202,10 +202,8 @@ def _product(q, codes, scales, M, O, I, bias, alpha, beta, dtype):
     N = q.shape[-2]
     y = torch.empty((M, N, O), device=q.device, dtype=dtype)
     if y.numel():
-        with torch.cuda.device(q.device):
-            _lib.check(_lib.lib().hecka_block8_linear(q.codes.data_ptr(), q.scales.data_ptr(), xm, codes.data_ptr(), scales.data_ptr(),
-                                                      M, N, O, I, _ptr(bias), _bstride(bias), float(alpha), float(beta), y.data_ptr(),
-                                                      DTYPES[dtype], _st(y)), 'block8_linear')
+        _lib.call('hecka_block8_linear', q.device, q.codes.data_ptr(), q.scales.data_ptr(), xm, codes.data_ptr(), scales.data_ptr(),
+                  M, N, O, I, _ptr(bias), _bstride(bias), alpha, beta, y.data_ptr(), DTYPES[dtype])
     return y
 
 
@@ -217,13 +215,10 @@ def _weight_grad(dy, q, alpha, beta, want_bias=True):
     if N == 0:
         return dW.zero_(), db.zero_() if db is not None else None
     if dW.numel():
-        L = _lib.lib()
-        nbytes = L.hecka_block8_wgrad_workspace_bytes(M, N, O, I)
+        nbytes = _lib.lib().hecka_block8_wgrad_workspace_bytes(M, N, O, I)
         ws = torch.empty((nbytes // 4,), device=dy.device, dtype=torch.float32) if nbytes else None
-        with torch.cuda.device(dy.device):
-            _lib.check(L.hecka_block8_wgrad(dy.data_ptr(), DTYPES[dy.dtype], q.codes.data_ptr(), q.scales.data_ptr(),
-                                            1 if len(q.shape) == 2 else M, M, N, O, I, float(alpha), float(beta), dW.data_ptr(),
-                                            _ptr(db), _ptr(ws), nbytes, _st(dy)), 'block8_wgrad')
+        _lib.call('hecka_block8_wgrad', dy.device, dy.data_ptr(), DTYPES[dy.dtype], q.codes.data_ptr(), q.scales.data_ptr(),
+                  1 if len(q.shape) == 2 else M, M, N, O, I, alpha, beta, dW.data_ptr(), _ptr(db), _ptr(ws), nbytes)
     return dW, db
 
 
@@ -322,10 +317,8 @@ def linear(x, weight, bias=None, scale=1.0, bias_scale=1.0):
         x = x.detach().contiguous()
         y = torch.empty((M, N, O), device=x.device, dtype=x.dtype)
         if N:
-            with torch.cuda.device(x.device):
-                _lib.check(_lib.lib().hecka_block8_linear_token(x.data_ptr(), DTYPES[x.dtype], xm, w.codes.data_ptr(), w.scales.data_ptr(),
-                                                                M, N, O, I, _ptr(b), _bstride(b), float(scale), float(bias_scale), y.data_ptr(),
-                                                                _st(x)), 'block8_linear_token')
+            _lib.call('hecka_block8_linear_token', x.device, x.data_ptr(), DTYPES[x.dtype], xm, w.codes.data_ptr(), w.scales.data_ptr(),
+                      M, N, O, I, _ptr(b), _bstride(b), scale, bias_scale, y.data_ptr())
         return y
     _check(x, what)
     _check(weight, what)

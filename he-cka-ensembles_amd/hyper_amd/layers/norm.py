@@ -248,55 +248,55 @@ class _BatchNorm(_NormBase):
 _NORM_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
+def _ptr(t):
+    return t.data_ptr() if t is not None else None
+
+
 class _LayerNorm(torch.autograd.Function):
-    """Layer norm of x [G, R, D] (libhecka hecka_layernorm_*).  weight / bias [G, D] fp32; packed: `weight` is the flat
-    parameter row [G, 2 D] (weight | bias), read in place, its gradient returned as one tensor."""
+    """Layer norm of x [..., D] as G groups of rows (libhecka hecka_layernorm_*).  weight / bias fp32 [G, D], [D] where G = 1;
+    packed: `weight` is the flat parameter row [G, 2 D] (weight | bias), read in place, its gradient returned as one tensor.
+    Reshapes happen in here: outside they would be nodes of the graph."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, eps, packed):
-        G, R, D = x.shape
+    def forward(ctx, x, weight, bias, eps, packed, G):
+        x = x.contiguous()
+        D = x.shape[-1]
+        R = x.numel() // (G * D) if G else 0
         y = torch.empty_like(x)
-        want = any(ctx.needs_input_grad[:3])
-        mean = torch.empty((G, R), device=x.device, dtype=torch.float32) if want else None
-        rstd = torch.empty_like(mean) if want else None
-        w_ptr = weight.data_ptr() if weight is not None else None
-        b_ptr = w_ptr + 4 * D if packed else bias.data_ptr() if bias is not None else None
-        ptr = lambda t: t.data_ptr() if t is not None else None   # noqa: E731
-        if x.numel():
-            with torch.cuda.device(x.device):
-                _lib.check(_lib.lib().hecka_layernorm_fwd(
-                    x.data_ptr(), _NORM_DTYPES[x.dtype], G, R, D, w_ptr, b_ptr, 2 * D if packed else D, float(eps), y.data_ptr(),
-                    ptr(mean), ptr(rstd), torch.cuda.current_stream(x.device).cuda_stream), 'layernorm_fwd')
-        ctx.save_for_backward(x, mean, rstd, weight)
-        ctx.cfg = (packed, bias is not None)
+        w = weight.contiguous() if weight is not None else None
+        b = bias.contiguous() if bias is not None else None
+        mean = rstd = None
+        if any(ctx.needs_input_grad):
+            mean, rstd = torch.empty((2, G, R), device=x.device, dtype=torch.float32).unbind(0)
+        if R:
+            w_ptr = _ptr(w)
+            _lib.call('hecka_layernorm_fwd', x.device, x.data_ptr(), _NORM_DTYPES[x.dtype], G, R, D, w_ptr,
+                      w_ptr + 4 * D if packed else _ptr(b), 2 * D if packed else D, eps, y.data_ptr(), _ptr(mean), _ptr(rstd))
+        ctx.save_for_backward(x, mean, rstd, w)
+        ctx.cfg = (packed, bias is not None, G, R)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, mean, rstd, weight = ctx.saved_tensors
-        packed, has_bias = ctx.cfg
-        G, R, D = x.shape
-        dy = dy.contiguous()
-        f32 = dict(device=x.device, dtype=torch.float32)
-        dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
-        dw = db = None
-        if weight is not None and ctx.needs_input_grad[1]:
-            dw = torch.empty((G, 2 * D if packed else D), **f32)
-        if has_bias and ctx.needs_input_grad[2]:
-            db = torch.empty((G, D), **f32)
-        if x.numel() == 0:
-            return dx, dw.zero_() if dw is not None else None, db.zero_() if db is not None else None, None, None
-        ptr = lambda t: t.data_ptr() if t is not None else None   # noqa: E731
-        L = _lib.lib()
-        nbytes = L.hecka_layernorm_bwd_workspace_bytes(G, R, D) if dw is not None or db is not None else 0
-        ws = torch.empty((nbytes // 4,), **f32) if nbytes else None
-        with torch.cuda.device(x.device):
-            _lib.check(L.hecka_layernorm_bwd(
-                dy.data_ptr(), x.data_ptr(), _NORM_DTYPES[x.dtype], mean.data_ptr(), rstd.data_ptr(), G, R, D, ptr(weight),
-                2 * D if packed else D, ptr(dx), ptr(dw), dw.data_ptr() + 4 * D if packed and dw is not None else ptr(db),
-                2 * D if packed else D, ptr(ws), nbytes, torch.cuda.current_stream(x.device).cuda_stream), 'layernorm_bwd')
-        return dx, dw, db, None, None
+        x, mean, rstd, w = ctx.saved_tensors
+        packed, has_bias, G, R = ctx.cfg
+        D = x.shape[-1]
+        need = ctx.needs_input_grad
+        dx = torch.empty_like(x) if need[0] else None
+        dw = torch.empty_like(w) if w is not None and need[1] else None
+        db = torch.empty(w.shape, device=x.device, dtype=torch.float32) if has_bias and need[2] else None
+        if R == 0:
+            return dx, dw.zero_() if dw is not None else None, db.zero_() if db is not None else None, None, None, None
+        nbytes, ws = 0, None
+        if dw is not None or db is not None:
+            nbytes = _lib.lib().hecka_layernorm_bwd_workspace_bytes(G, R, D)
+            ws = torch.empty((nbytes // 4,), device=x.device, dtype=torch.float32) if nbytes else None
+        dy = dy.contiguous()      # (kept: a copy has to live until the launch)
+        _lib.call('hecka_layernorm_bwd', x.device, dy.data_ptr(), x.data_ptr(), _NORM_DTYPES[x.dtype], mean.data_ptr(),
+                  rstd.data_ptr(), G, R, D, _ptr(w), 2 * D if packed else D, _ptr(dx), _ptr(dw),
+                  dw.data_ptr() + 4 * D if packed and dw is not None else _ptr(db), 2 * D if packed else D, _ptr(ws), nbytes)
+        return dx, dw, db, None, None, None
 
 
 def _check_layer_norm(x, affine):
@@ -335,9 +335,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
         raise ValueError('layer norm: weight has to be (%d,) or (members, %d), got %s' % (D, D, tuple(weight.shape)))
     if G > 65535:
         raise ValueError('layer norm: at most 65535 members, got %d' % G)
-    row = lambda t: t.reshape(G, D).contiguous() if t is not None else None   # noqa: E731
-    rows = x.numel() // (G * D) if G else 0
-    return _LayerNorm.apply(x.contiguous().view(G, rows, D), row(weight), row(bias), eps, False).view(x.shape)
+    return _LayerNorm.apply(x, weight, bias, float(eps), False, G)
 
 
 @register_gen_module('layer_norm')
@@ -365,9 +363,7 @@ class LayerNorm(GenModule):
             raise ValueError('expected (members, ..., %d) input (got %s)' % (self.num_features, tuple(input.shape)))
         if flat is not None and tuple(flat.shape) != (input.shape[0], 2 * self.num_features):
             raise ValueError('expected parameters (%d, %d) (got %s)' % (input.shape[0], 2 * self.num_features, tuple(flat.shape)))
-        M = input.shape[0]
-        x = input.contiguous().view(M, input.numel() // max(M * self.num_features, 1), self.num_features)
-        y = _LayerNorm.apply(x, flat.contiguous() if flat is not None else None, None, self.eps, flat is not None).view(input.shape)
+        y = _LayerNorm.apply(input, flat, None, float(self.eps), flat is not None, input.shape[0])
         return self.track_feature(y), y
 
     def extra_repr(self):
