@@ -27,11 +27,6 @@ __device__ __forceinline__ void store8(T* row, int col, int K, const float* v) {
     if (col + j * Piece<T>::N < K) store_piece(row, col + j * Piece<T>::N, K, p);
   }
 }
-__device__ __forceinline__ float max16(float a) {      // over the sixteen lanes of a block
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor(a, o));
-  return a;
-}
 __device__ __forceinline__ float max8(const float* v) {
   float a = 0.f;
 #pragma unroll

@@ -6,93 +6,106 @@
 // HBM bound: the forward reads x and writes y once, the backward reads x and dy and writes dx once.  A row therefore stays in
 // the registers of TPR threads (16 elements each at most) between its loads and its stores, so that the variance is the
 // two-pass one (mean first, then squared distances) at no extra traffic; all statistics are fp32.  A row of up to 1024
-// elements belongs to one wave (its sums are shuffles, no barrier), a longer one to 256 / 512 / 1024 threads.
+// elements belongs to 16, 32 or 64 lanes of a wave (its sums need no barrier), a longer one to 256 / 512 / 1024 threads; the
+// next row's loads are under way while a row is summed.
 // The backward keeps every thread's columns of dw and db in registers over all rows of its workgroup and writes them once:
 // [workgroups per member, 2, D] partial sums, added up in a fixed order by a second kernel - no atomics, the same bits on
-// every run.  About 512 workgroups (two per CU) hold the partial sums to a few per cent of the traffic.
+// every run.
 #include "hecka_host.hpp"
 #include "hecka_vec.hpp"
 
 namespace hecka {
 
-// Sums of two values over the TPR threads of a row.  `red` is one of two LDS buffers used in turn: a wave that is past the
+// Sum of a value over the TPR threads of a row.  `red` is one of two LDS buffers used in turn: a wave that is past the
 // barrier of one sum writes the other buffer next, so one barrier per sum suffices.
-template <int TPR, int NW>
-__device__ __forceinline__ void row_sum(float& a, float& b, float (*red)[2]) {
-  a = wave_sum(a);
-  b = wave_sum(b);
+template <int TPR>
+__device__ __forceinline__ float row_sum(float a, float* red) {
+  constexpr int NW = TPR / 64;
+  a = lanes_sum<TPR < 64 ? TPR : 64>(a);
   if constexpr (NW > 1) {
-    const int wave = threadIdx.x >> 6;
-    if ((threadIdx.x & 63) == 0) { red[wave][0] = a; red[wave][1] = b; }
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
     __syncthreads();
-    a = red[0][0];
-    b = red[0][1];
+    a = red[0];
 #pragma unroll
-    for (int i = 1; i < NW; ++i) { a += red[i][0]; b += red[i][1]; }
-  }
-}
-template <int TPR, int NW>
-__device__ __forceinline__ float row_sum(float a, float (*red)[2]) {
-  a = wave_sum(a);
-  if constexpr (NW > 1) {
-    const int wave = threadIdx.x >> 6;
-    if ((threadIdx.x & 63) == 0) red[wave][0] = a;
-    __syncthreads();
-    a = red[0][0];
-#pragma unroll
-    for (int i = 1; i < NW; ++i) a += red[i][0];
+    for (int i = 1; i < NW; ++i) a += red[i];
   }
   return a;
+}
+// of two values at once
+template <int TPR>
+__device__ __forceinline__ void row_sum2(float& a, float& b, float* red) {
+  constexpr int NW = TPR / 64;
+  a = lanes_sum<TPR < 64 ? TPR : 64>(a);
+  b = lanes_sum<TPR < 64 ? TPR : 64>(b);
+  if constexpr (NW > 1) {
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) { red[wave] = a; red[NW + wave] = b; }
+    __syncthreads();
+    a = red[0];
+    b = red[NW];
+#pragma unroll
+    for (int i = 1; i < NW; ++i) { a += red[i]; b += red[NW + i]; }
+  }
+}
+
+// a thread's pieces of row r of a member's rows (those of the last row again where r is behind it)
+template <class T, int TPR, int NV>
+__device__ __forceinline__ void load_row(Piece<T> (&p)[NV], const T* x, long long r, long long R, int D, int lane) {
+  const T* row = x + (r < R ? r : R - 1) * D;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) p[j] = load_piece(row, (j * TPR + lane) * Piece<T>::N, D);
+}
+template <class T, int TPR, int NV>
+__device__ __forceinline__ void load_params(float (&v)[NV * Piece<T>::N], const float* w, int D, int lane, float none) {
+  constexpr int N = Piece<T>::N;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+#pragma unroll
+    for (int h = 0; h < N / 4; ++h) {
+      const int c = (j * TPR + lane) * N + 4 * h;
+      const Piece<float> p = w ? load_piece(w, c, D) : Piece<float>{none, none, none, none};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[j * N + 4 * h + i] = p.e[i];
+    }
+  }
 }
 
 template <class T, int TPR, int NV>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layernorm_fwd_kernel(
     const T* __restrict__ x, long long R, int D, int chunks, const float* __restrict__ w, const float* __restrict__ b,
     long long wstride, float eps, T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd) {
-  constexpr int N = Piece<T>::N, NW = TPR / 64, RPB = TPR < 256 ? 256 / TPR : 1;
-  __shared__ float red[2][NW][2];
-  const long long m = blockIdx.x / chunks;
+  constexpr int N = Piece<T>::N, RPB = TPR < 256 ? 256 / TPR : 1;
+  __shared__ float red[2][TPR < 64 ? 1 : TPR / 64];
+  const long long m = blockIdx.x / chunks, step = (long long)chunks * RPB;
   const int chunk = blockIdx.x % chunks, sub = threadIdx.x / TPR, lane = threadIdx.x % TPR;
   float wr[NV * N], br[NV * N];
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = (j * TPR + lane) * N + i;
-      wr[j * N + i] = w && c < D ? w[m * wstride + c] : 1.f;
-      br[j * N + i] = b && c < D ? b[m * wstride + c] : 0.f;
-    }
-  }
-  const float inv = 1.0f / (float)D;
-  for (long long r = (long long)chunk * RPB + sub; r < R; r += (long long)chunks * RPB) {
-    const T* xr = x + (m * R + r) * D;
+  Piece<T> p[NV];
+  long long r = (long long)chunk * RPB + sub;
+  x += m * R * D;
+  y += m * R * D;
+  load_row<T, TPR, NV>(p, x, r, R, D, lane);
+  load_params<T, TPR, NV>(wr, w ? w + m * wstride : nullptr, D, lane, 1.f);
+  load_params<T, TPR, NV>(br, b ? b + m * wstride : nullptr, D, lane, 0.f);
+  for (; r < R; r += step) {
     float v[NV * N], s = 0.f;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (j * TPR + lane) * N;
-      const Piece<T> p = load_piece(xr, c, D);
-#pragma unroll
-      for (int i = 0; i < N; ++i) { v[j * N + i] = widen(p.e[i]); s += v[j * N + i]; }
-    }
-    const float mu = row_sum<TPR, NW>(s, red[0]) / (float)D;      // a division: a constant row of exact sum has this mean
+    for (int k = 0; k < NV * N; ++k) { v[k] = widen(p[k / N].e[k % N]); s += v[k]; }
+    load_row<T, TPR, NV>(p, x, r + step, R, D, lane);
+    const float mu = row_sum<TPR>(s, red[0]) / (float)D;      // a division: a constant row of exact sum has this mean
     float q = 0.f;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        v[j * N + i] -= mu;
-        if ((j * TPR + lane) * N + i < D) q = fmaf(v[j * N + i], v[j * N + i], q);
-      }
+    for (int k = 0; k < NV * N; ++k) {
+      v[k] -= mu;
+      if ((k / N * TPR + lane) * N + k % N < D) q = fmaf(v[k], v[k], q);
     }
-    const float rs = 1.0f / sqrtf(row_sum<TPR, NW>(q, red[1]) * inv + eps);
+    const float rs = 1.0f / sqrtf(row_sum<TPR>(q, red[1]) / (float)D + eps);
     if (mean && lane == 0) { mean[m * R + r] = mu; rstd[m * R + r] = rs; }
-    T* yr = y + (m * R + r) * D;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      Piece<T> p;
+      Piece<T> o;
 #pragma unroll
-      for (int i = 0; i < N; ++i) narrow(fmaf(v[j * N + i] * rs, wr[j * N + i], br[j * N + i]), p.e[i]);
-      store_piece(yr, (j * TPR + lane) * N, D, p);
+      for (int i = 0; i < N; ++i) narrow(fmaf(v[j * N + i] * rs, wr[j * N + i], br[j * N + i]), o.e[i]);
+      store_piece(y + r * D, (j * TPR + lane) * N, D, o);
     }
   }
 }
@@ -102,65 +115,65 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layernorm_bwd_kernel(
     const T* __restrict__ dy, const T* __restrict__ x, const float* __restrict__ mean, const float* __restrict__ rstd,
     long long R, int D, int chunks, const float* __restrict__ w, long long wstride, T* __restrict__ dx,
     float* __restrict__ dw, float* __restrict__ db, long long gstride, long long pstride) {
-  constexpr int N = Piece<T>::N, NW = TPR / 64, RPB = TPR < 256 ? 256 / TPR : 1;
-  __shared__ float red[2][NW][2];
+  constexpr int N = Piece<T>::N, RPB = TPR < 256 ? 256 / TPR : 1;
+  __shared__ float red[2][TPR < 64 ? 1 : TPR / 32];
   __shared__ float fold[RPB > 1 ? RPB - 1 : 1][RPB > 1 ? TPR : 1][RPB > 1 ? 2 * NV * N + 1 : 1];
-  const long long m = blockIdx.x / chunks;
+  const long long m = blockIdx.x / chunks, step = (long long)chunks * RPB;
   const int chunk = blockIdx.x % chunks, sub = threadIdx.x / TPR, lane = threadIdx.x % TPR;
   float wr[NV * N], aw[NV * N], ab[NV * N];
+  Piece<T> px[NV], pd[NV];
+  long long r = (long long)chunk * RPB + sub;
+  x += m * R * D;
+  dy += m * R * D;
+  mean += m * R;
+  rstd += m * R;
+  load_row<T, TPR, NV>(px, x, r, R, D, lane);
+  load_row<T, TPR, NV>(pd, dy, r, R, D, lane);
+  float mu = mean[r < R ? r : R - 1], rs = rstd[r < R ? r : R - 1];
+  load_params<T, TPR, NV>(wr, w ? w + m * wstride : nullptr, D, lane, 1.f);
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = (j * TPR + lane) * N + i;
-      wr[j * N + i] = w && c < D ? w[m * wstride + c] : 1.f;
-      aw[j * N + i] = ab[j * N + i] = 0.f;
-    }
-  }
+  for (int k = 0; k < NV * N; ++k) aw[k] = ab[k] = 0.f;
   const float inv = 1.0f / (float)D;
   int turn = 0;
-  for (long long r = (long long)chunk * RPB + sub; r < R; r += (long long)chunks * RPB, turn ^= 1) {
-    const long long row = m * R + r;
-    const float mu = mean[row], rs = rstd[row];
+  for (; r < R; r += step, turn ^= 1) {
     float g[NV * N], h[NV * N], s1 = 0.f, s2 = 0.f;
+    const float rt = rs;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (j * TPR + lane) * N;
-      const Piece<T> p = load_piece(x + row * D, c, D), q = load_piece(dy + row * D, c, D);
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int k = j * N + i;
-        const float d = widen(q.e[i]);      // zero behind the row's end, as g then is: nothing of it enters the sums
-        h[k] = (widen(p.e[i]) - mu) * rs;
-        aw[k] = fmaf(d, h[k], aw[k]);
-        ab[k] += d;
-        g[k] = d * wr[k];
-        s1 += g[k];
-        s2 = fmaf(g[k], h[k], s2);
-      }
+    for (int k = 0; k < NV * N; ++k) {
+      const float d = widen(pd[k / N].e[k % N]);      // zero behind the row's end, as g then is: nothing of it enters the sums
+      h[k] = (widen(px[k / N].e[k % N]) - mu) * rt;
+      aw[k] = fmaf(d, h[k], aw[k]);
+      ab[k] += d;
+      g[k] = d * wr[k];
+      s1 += g[k];
+      s2 = fmaf(g[k], h[k], s2);
     }
+    load_row<T, TPR, NV>(px, x, r + step, R, D, lane);
+    load_row<T, TPR, NV>(pd, dy, r + step, R, D, lane);
+    mu = mean[r + step < R ? r + step : R - 1];
+    rs = rstd[r + step < R ? r + step : R - 1];
     if (dx) {
-      row_sum<TPR, NW>(s1, s2, red[turn]);
+      row_sum2<TPR>(s1, s2, red[turn]);
       s1 *= inv;
       s2 *= inv;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        Piece<T> p;
+        Piece<T> o;
 #pragma unroll
-        for (int i = 0; i < N; ++i) narrow(rs * (g[j * N + i] - s1 - h[j * N + i] * s2), p.e[i]);
-        store_piece(dx + row * D, (j * TPR + lane) * N, D, p);
+        for (int i = 0; i < N; ++i) narrow(rt * (g[j * N + i] - s1 - h[j * N + i] * s2), o.e[i]);
+        store_piece(dx + (m * R + r) * D, (j * TPR + lane) * N, D, o);
       }
     }
   }
   if (!dw && !db) return;
-  if constexpr (RPB > 1) {     // the waves' sums of the same columns, added in the order of the waves
+  if constexpr (RPB > 1) {     // the sums of the same columns of different rows, added in order
     if (sub > 0) {
 #pragma unroll
       for (int k = 0; k < NV * N; ++k) { fold[sub - 1][lane][2 * k] = aw[k]; fold[sub - 1][lane][2 * k + 1] = ab[k]; }
     }
     __syncthreads();
     if (sub > 0) return;
-#pragma unroll
+#pragma unroll 1
     for (int o = 0; o < RPB - 1; ++o) {
 #pragma unroll
       for (int k = 0; k < NV * N; ++k) { aw[k] += fold[o][lane][2 * k]; ab[k] += fold[o][lane][2 * k + 1]; }
@@ -169,11 +182,11 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layernorm_bwd_kernel(
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = (j * TPR + lane) * N + i;
+    for (int h = 0; h < N / 4; ++h) {
+      const int c = (j * TPR + lane) * N + 4 * h, k = j * N + 4 * h;
       if (c < D) {
-        if (dw) dw[m * gstride + chunk * pstride + c] = aw[j * N + i];
-        if (db) db[m * gstride + chunk * pstride + c] = ab[j * N + i];
+        if (dw) store_piece(dw + m * gstride + chunk * pstride, c, D, Piece<float>{aw[k], aw[k + 1], aw[k + 2], aw[k + 3]});
+        if (db) store_piece(db + m * gstride + chunk * pstride, c, D, Piece<float>{ab[k], ab[k + 1], ab[k + 2], ab[k + 3]});
       }
     }
   }
@@ -205,27 +218,35 @@ __global__ __launch_bounds__(1024) void layernorm_fold_kernel(const float* __res
 
 static const int kMaxNormWidth = 16384;
 
-static int norm_threads(int D) { return D <= 1024 ? 64 : D <= 4096 ? 256 : D <= 8192 ? 512 : 1024; }
+// threads of a row: few enough that most have work (a piece is 4 or 8 elements), enough that none has more than 16 elements
+static int norm_threads(int D, int piece) {
+  return D <= 16 * piece ? 16 : D <= 32 * piece ? 32 : D <= 1024 ? 64 : D <= 4096 ? 256 : D <= 8192 ? 512 : 1024;
+}
 
-// workgroups per member: every row its own share up to `most` workgroups in all
-static int norm_chunks(long long G, long long R, int D, long long most) {
-  const int rpb = norm_threads(D) == 64 ? 4 : 1;
+// Workgroups per member: every row its own share, up to `most` in all.  Forward: eight per CU, but for long rows (whose weight
+// and bias, 8 bytes an element, a workgroup reads once) two.  Backward: enough to fill the chip once, so that the partial sums
+// stay a few per cent of the traffic.
+static int norm_chunks(long long G, long long R, int threads, bool forward) {
+  const int rpb = threads < 256 ? 256 / threads : 1;
+  const long long most = threads >= 1024 ? 512 : threads == 512 ? (forward ? 1024 : 512) : forward ? 2048 : 1024;
   const long long want = (R + rpb - 1) / rpb, share = most / G < 1 ? 1 : most / G;
   return (int)(want < share ? want : share);
 }
-static const long long kFwdBlocks = 2048, kBwdBlocks = 512;
 
 template <class T, class F>
 static int norm_dispatch(int D, const F& f) {
   constexpr int N = Piece<T>::N;
-  const int t = norm_threads(D), need = (D + t * N - 1) / (t * N);      // pieces per thread: 1, 2 or (fp32) 4
+  const int t = norm_threads(D, N), need = (D + t * N - 1) / (t * N);      // pieces per thread: 1, 2 or (fp32) 4
 #define HECKA_NORM(TPR) \
   case TPR: return need <= 1 ? f.template run<T, TPR, 1>() : need <= 2 ? f.template run<T, TPR, 2>() : f.template run<T, TPR, 16 / N>();
   switch (t) {
+    case 16: return f.template run<T, 16, 1>();
+    case 32: return f.template run<T, 32, 1>();
     HECKA_NORM(64)
     HECKA_NORM(256)
     HECKA_NORM(512)
-    default: return need <= 1 ? f.template run<T, 1024, 1>() : need <= 2 ? f.template run<T, 1024, 2>() : f.template run<T, 1024, 16 / N>();
+    HECKA_NORM(1024)
+    default: return HECKA_EINVAL;
   }
 #undef HECKA_NORM
 }
@@ -233,15 +254,16 @@ static int norm_dispatch(int D, const F& f) {
 struct NormFwd {
   const void* x; long long G, R; int D; const float *w, *b; long long wstride; float eps; void* y; float *mean, *rstd; hipStream_t st;
   template <class T, int TPR, int NV> int run() const {
-    const int chunks = norm_chunks(G, R, D, kFwdBlocks);
+    const int chunks = norm_chunks(G, R, TPR, true);
     layernorm_fwd_kernel<T, TPR, NV><<<dim3((unsigned)(G * chunks)), TPR < 256 ? 256 : TPR, 0, st>>>(
         (const T*)x, R, D, chunks, w, b, wstride, eps, (T*)y, mean, rstd);
     return check_launch("layernorm_fwd");
   }
 };
 struct NormBwd {
-  const void *dy, *x; const float *mean, *rstd; long long G, R; int D; const float* w; long long wstride; void* dx; float *dw, *db; long long gstride; float* ws; int chunks; hipStream_t st;
+  const void *dy, *x; const float *mean, *rstd; long long G, R; int D; const float* w; long long wstride; void* dx; float *dw, *db; long long gstride; float* ws; hipStream_t st;
   template <class T, int TPR, int NV> int run() const {
+    const int chunks = norm_chunks(G, R, TPR, false);
     const bool part = chunks > 1 && (dw || db);
     layernorm_bwd_kernel<T, TPR, NV><<<dim3((unsigned)(G * chunks)), TPR < 256 ? 256 : TPR, 0, st>>>(
         (const T*)dy, (const T*)x, mean, rstd, R, D, chunks, w, wstride, (T*)dx, part ? ws : dw, part ? ws + D : db,
@@ -280,7 +302,8 @@ int hecka_layernorm_fwd(const void* x, int dtype, int G, long long R, int D, con
 
 size_t hecka_layernorm_bwd_workspace_bytes(int G, long long R, int D) {
   if (G <= 0 || R <= 0 || D <= 0 || G > 65535 || D > kMaxNormWidth) return 0;
-  const int chunks = norm_chunks(G, R, D, kBwdBlocks);
+  const int fp32 = norm_chunks(G, R, norm_threads(D, 4), false), other = norm_chunks(G, R, norm_threads(D, 8), false);
+  const int chunks = fp32 > other ? fp32 : other;
   return chunks > 1 ? (size_t)G * chunks * 2 * D * sizeof(float) : 0;
 }
 
@@ -294,7 +317,7 @@ int hecka_layernorm_bwd(const void* dy, const void* x, int dtype, const float* m
     return fail(HECKA_EWORKSPACE, "%slayernorm_bwd: workspace too small (%lld bytes given)", "", (long long)ws_bytes);
   clear_error();
   return norm_type(dtype, D, NormBwd{dy, x, mean, rstd, G, R, D, weight, wstride, dx, dweight, dbias, gstride, (float*)ws,
-                                     norm_chunks(G, R, D, kBwdBlocks), (hipStream_t)stream});
+                                     (hipStream_t)stream});
 }
 
 }  // extern "C"

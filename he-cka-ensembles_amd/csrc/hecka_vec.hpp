@@ -49,10 +49,35 @@ __device__ __forceinline__ void store_piece(T* row, int col, int D, const Piece<
   }
 }
 
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-  return v;
+// v of another lane of the same sixteen: ctrl 0xB1 / 0x4E exchange neighbours / pairs in a quad, 0x141 / 0x140 mirror eight /
+// sixteen lanes.  Applied in this order every lane ends up with the sum (maximum) of its sixteen, in vector instructions alone.
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float sum16(float v) {
+  v += dpp<0xB1>(v);
+  v += dpp<0x4E>(v);
+  v += dpp<0x141>(v);
+  return v + dpp<0x140>(v);
+}
+__device__ __forceinline__ float max16(float v) {
+  v = fmaxf(v, dpp<0xB1>(v));
+  v = fmaxf(v, dpp<0x4E>(v));
+  v = fmaxf(v, dpp<0x141>(v));
+  return fmaxf(v, dpp<0x140>(v));
+}
+__device__ __forceinline__ float lane_value(float v, int lane) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
+}
+// sum over the LANES (16, 32, 64) lanes that a row has of this wave
+template <int LANES>
+__device__ __forceinline__ float lanes_sum(float v) {
+  v = sum16(v);
+  if constexpr (LANES == 16) return v;
+  const float a = lane_value(v, 0) + lane_value(v, 16), b = lane_value(v, 32) + lane_value(v, 48);
+  if constexpr (LANES == 32) return (threadIdx.x & 32) ? b : a;
+  return a + b;
 }
 
 }  // namespace hecka
