@@ -34,95 +34,164 @@ __device__ __forceinline__ float max8(const float* v) {
   return a;
 }
 
-// codes and scale byte of the block that the sixteen lanes hold
-__device__ __forceinline__ void write_block(float* v, unsigned char* codes, unsigned char* scales, long long row, int blk,
-                                            int nblk, int lane16) {
-  const int byte = scale_byte(max16(max8(v)));
-  const float inv = inverse_scale(byte);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = encodable(v[i]);
-  uint2 c;
-  c.x = encode4(v[0], v[1], v[2], v[3], inv);
-  c.y = encode4(v[4], v[5], v[6], v[7], inv);
-  *reinterpret_cast<uint2*>(codes + (row * nblk + blk) * kBlock + lane16 * 8) = c;
-  if (lane16 == 0) {
-    unsigned char* s = scales + row * ((nblk + 3) & ~3);
-    s[blk] = (unsigned char)byte;
-    if (blk == nblk - 1)
-      for (int i = nblk; i < ((nblk + 3) & ~3); ++i) s[i] = 127;
-  }
-}
-
 enum { kActNone = 0, kActGelu = 1, kActSilu = 2, kActTanh = 3, kActSigmoid = 4, kActCrater = 5 };
 static constexpr float kHalfRoot = 0.70710678118654752f, kCrater = 0.70710678118654752f + 0.008274364699f;
 
+// e^x, x <= 0, from the hardware's 2^x: the exponent's rounding error, |x| 2^-25, is worked out and put back, so the result is good
+// to about 2 units in the last place (the hardware's own included); 0 from -104 down, where no float is left.
+__device__ __forceinline__ float exp_near(float x) {
+  x = fmaxf(x, -104.f);
+  const float t = x * 1.44269504f;
+  const float r = fmaf(x, 1.44269504f, -t) + x * 1.92596299e-8f;      // 1.44269504f + 1.92596299e-8f = log2 e
+  const float p = __builtin_amdgcn_exp2f(t);
+  return fmaf(p, r * 0.69314718f, p);
+}
+// sigmoid(x) and 1 - sigmoid(x), both without cancellation: q = e^-|x| <= 1
+__device__ __forceinline__ void sigmoid_pair(float x, float& p, float& n) {
+  const float q = exp_near(-fabsf(x)), s = __builtin_amdgcn_rcpf(1.0f + q), qs = q * s;
+  p = x >= 0.f ? s : qs;
+  n = x >= 0.f ? qs : s;
+  if (x != x) p = n = x;
+}
+// normal distribution below x: 0.5 erfc(-x / sqrt 2).  erfc(z) for z >= 0 as a polynomial in 1 / (1 + p z) times e^-z^2
+// (Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26; absolute error below 1.5e-7), no cancellation on either side.
+__device__ __forceinline__ float normal_below(float x, float& bell) {
+  const float z = fabsf(x) * kHalfRoot, t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, z, 1.0f));
+  bell = exp_near(-0.5f * x * x);
+  float c = fmaf(1.061405429f, t, -1.453152027f);
+  c = fmaf(c, t, 1.421413741f);
+  c = fmaf(c, t, -0.284496736f);
+  c = fmaf(c, t, 0.254829592f);
+  const float half = 0.5f * c * t * bell;
+  return x >= 0.f ? 1.0f - half : half;
+}
+
 template <int ACT>
 __device__ __forceinline__ float act_value(float x) {
-  if (ACT == kActGelu) return 0.5f * x * erfcf(-kHalfRoot * x);      // erfc: no cancellation where gelu is close to zero
-  if (ACT == kActSilu) return x / (1.0f + expf(-x));
+  float p, n;
+  if (ACT == kActGelu) return x * normal_below(x, n);
   if (ACT == kActTanh) return tanhf(x);
-  if (ACT == kActSigmoid) return 1.0f / (1.0f + expf(-x));
-  return kCrater * x * (1.0f + tanhf(kHalfRoot * (x + 1.0f)));
+  sigmoid_pair(ACT == kActCrater ? 2.0f * kHalfRoot * (x + 1.0f) : x, p, n);      // 1 + tanh z = 2 sigmoid(2 z)
+  return ACT == kActSilu ? x * p : ACT == kActSigmoid ? p : 2.0f * kCrater * (x * p);
 }
 template <int ACT>
 __device__ __forceinline__ float act_slope(float x) {
-  if (ACT == kActGelu) return fmaf(x * 0.39894228040143268f, expf(-0.5f * x * x), 0.5f * erfcf(-kHalfRoot * x));
-  if (ACT == kActTanh) { const float t = tanhf(x); return 1.0f - t * t; }
-  if (ACT == kActSilu || ACT == kActSigmoid) {
-    const float p = 1.0f / (1.0f + expf(-x));
-    return ACT == kActSilu ? p * (1.0f + x * (1.0f - p)) : p * (1.0f - p);
+  float p, n;
+  if (ACT == kActGelu) {
+    p = normal_below(x, n);
+    return fmaf(x * 0.39894228f, n, p);
   }
-  const float t = tanhf(kHalfRoot * (x + 1.0f));
-  return kCrater * (1.0f + t + kHalfRoot * x * (1.0f - t * t));
+  sigmoid_pair(ACT == kActTanh ? 2.0f * x : ACT == kActCrater ? 2.0f * kHalfRoot * (x + 1.0f) : x, p, n);
+  if (ACT == kActTanh) return 4.0f * p * n;
+  if (ACT == kActSigmoid) return p * n;
+  if (ACT == kActSilu) return fmaf(x * p, n, p);
+  return 2.0f * kCrater * fmaf(2.0f * kHalfRoot, x * (p * n), p);
+}
+
+// Which blocks a group of sixteen lanes works on, and where they lie.  FLAT (whole blocks, rows without gaps, their number a
+// multiple of four so that the scale bytes have none either): everything is one long row.  UNROLL blocks at a time are loaded before
+// the first is worked on: one block per lane group in flight (128 bytes of codes) leaves the memory idle - decoding bf16 reached
+// 2.75 TB/s that way.
+template <bool FLAT>
+struct Place { long long row; int blk, col; };
+template <bool FLAT>
+__device__ __forceinline__ Place<FLAT> place_block(long long b, long long total, int nblk, int lane16) {
+  if constexpr (FLAT) return {0, 0, 0};
+  const long long row = total <= 0xffffffffLL ? (long long)((unsigned)b / (unsigned)nblk) : b / nblk;
+  const int blk = (int)(b - row * nblk);
+  return {row, blk, blk * kBlock + lane16 * 8};
 }
 
 // rows of K elements, `ld` apart; ACT != 0: y (rows of K, contiguous) = act(x) beside the codes of x
-template <class T, int ACT>
+template <class T, int ACT, bool FLAT>
 __global__ __launch_bounds__(256) void block8_rows_kernel(const T* __restrict__ x, long long R, int K, long long ld,
                                                           unsigned char* __restrict__ codes, unsigned char* __restrict__ scales,
                                                           T* __restrict__ y) {
-  const int nblk = row_blocks(K), lane16 = threadIdx.x & 15;
+  constexpr int UNROLL = 16 / sizeof(T) / 2;      // 4 (16-bit) or 2 blocks: 64 bytes per lane
+  const int nblk = row_blocks(K), lane16 = threadIdx.x & 15, group = threadIdx.x >> 4;
   const long long total = R * nblk;
-  for (long long b = (long long)blockIdx.x * 16 + (threadIdx.x >> 4); b < total; b += (long long)gridDim.x * 16) {
-    const long long row = total <= 0xffffffffLL ? (long long)((unsigned)b / (unsigned)nblk) : b / nblk;
-    const int blk = (int)(b - row * nblk), col = blk * kBlock + lane16 * 8;
-    float v[8];
-    load8(x + row * ld, col, K, v);
-    if (ACT != kActNone) {
-      float a[8];
+  for (long long b0 = (long long)blockIdx.x * (16 * UNROLL) + group; b0 < total; b0 += (long long)gridDim.x * (16 * UNROLL)) {
+    float v[UNROLL][8];
+    Place<FLAT> at[UNROLL];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) a[i] = act_value<ACT>(v[i]);
-      store8(y + row * K, col, K, a);
+    for (int u = 0; u < UNROLL; ++u) {
+      const long long b = b0 + u * 16 < total ? b0 + u * 16 : total - 1;
+      at[u] = place_block<FLAT>(b, total, nblk, lane16);
+      if constexpr (FLAT) load8(x + b * kBlock, lane16 * 8, kBlock, v[u]);
+      else load8(x + at[u].row * ld, at[u].col, K, v[u]);
     }
-    write_block(v, codes, scales, row, blk, nblk, lane16);
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const long long b = b0 + u * 16;
+      if (b >= total) break;
+      if (ACT != kActNone) {
+        float a[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a[i] = act_value<ACT>(v[u][i]);
+        if constexpr (FLAT) store8(y + b * kBlock, lane16 * 8, kBlock, a);
+        else store8(y + at[u].row * K, at[u].col, K, a);
+      }
+      const int byte = scale_byte(max16(max8(v[u])));
+      const float inv = inverse_scale(byte);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[u][i] = encodable(v[u][i]);
+      *reinterpret_cast<uint2*>(codes + b * kBlock + lane16 * 8) =
+          make_uint2(encode4(v[u][0], v[u][1], v[u][2], v[u][3], inv), encode4(v[u][4], v[u][5], v[u][6], v[u][7], inv));
+      if (lane16 == 0) {
+        if constexpr (FLAT) {
+          scales[b] = (unsigned char)byte;
+        } else {
+          unsigned char* s = scales + at[u].row * ((nblk + 3) & ~3);
+          s[at[u].blk] = (unsigned char)byte;
+          if (at[u].blk == nblk - 1)
+            for (int i = nblk; i < ((nblk + 3) & ~3); ++i) s[i] = 127;
+        }
+      }
+    }
   }
 }
 
 // ACT = 0: out = the values of the codes; else out = dy * act'(values)
-template <class T, int ACT>
+template <class T, int ACT, bool FLAT>
 __global__ __launch_bounds__(256) void block8_values_kernel(const unsigned char* __restrict__ codes,
                                                             const unsigned char* __restrict__ scales, const T* __restrict__ dy,
                                                             long long R, int K, T* __restrict__ out) {
-  const int nblk = row_blocks(K), lane16 = threadIdx.x & 15;
+  constexpr int UNROLL = ACT == kActNone ? 4 : 16 / sizeof(T) / 2;
+  const int nblk = row_blocks(K), lane16 = threadIdx.x & 15, group = threadIdx.x >> 4;
   const long long total = R * nblk;
-  for (long long b = (long long)blockIdx.x * 16 + (threadIdx.x >> 4); b < total; b += (long long)gridDim.x * 16) {
-    const long long row = total <= 0xffffffffLL ? (long long)((unsigned)b / (unsigned)nblk) : b / nblk;
-    const int blk = (int)(b - row * nblk), col = blk * kBlock + lane16 * 8;
-    const uint2 c = *reinterpret_cast<const uint2*>(codes + b * kBlock + lane16 * 8);
-    const float s = scale_of(scales[row * ((nblk + 3) & ~3) + blk]);
-    float v[8];
-    decode4(c.x, s, v);
-    decode4(c.y, s, v + 4);
-    if (ACT != kActNone) {
-      float d[8];
-      load8(dy + row * K, col, K, d);
+  for (long long b0 = (long long)blockIdx.x * (16 * UNROLL) + group; b0 < total; b0 += (long long)gridDim.x * (16 * UNROLL)) {
+    uint2 c[UNROLL];
+    int byte[UNROLL];
+    float d[UNROLL][8];
+    Place<FLAT> at[UNROLL];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = d[i] * act_slope<ACT>(v[i]);
-    } else if constexpr (__is_same(T, F16)) {      // fp16's largest, 65504, is kept as 65536: back to what fp16 holds
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = fabsf(v[i]) == 65536.f ? copysignf(65504.f, v[i]) : v[i];
+    for (int u = 0; u < UNROLL; ++u) {
+      const long long b = b0 + u * 16 < total ? b0 + u * 16 : total - 1;
+      at[u] = place_block<FLAT>(b, total, nblk, lane16);
+      c[u] = *reinterpret_cast<const uint2*>(codes + b * kBlock + lane16 * 8);
+      byte[u] = FLAT ? scales[b] : scales[at[u].row * ((nblk + 3) & ~3) + at[u].blk];
+      if (ACT != kActNone) {
+        if constexpr (FLAT) load8(dy + b * kBlock, lane16 * 8, kBlock, d[u]);
+        else load8(dy + at[u].row * K, at[u].col, K, d[u]);
+      }
     }
-    store8(out + row * K, col, K, v);
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const long long b = b0 + u * 16;
+      if (b >= total) break;
+      float v[8];
+      decode4(c[u].x, scale_of(byte[u]), v);
+      decode4(c[u].y, scale_of(byte[u]), v + 4);
+      if (ACT != kActNone) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = d[u][i] * act_slope<ACT>(v[i]);
+      } else if constexpr (__is_same(T, F16)) {      // fp16's largest, 65504, is kept as 65536: back to what fp16 holds
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = fabsf(v[i]) == 65536.f ? copysignf(65504.f, v[i]) : v[i];
+      }
+      if constexpr (FLAT) store8(out + b * kBlock, lane16 * 8, kBlock, v);
+      else store8(out + at[u].row * K, at[u].col, K, v);
+    }
   }
 }
 
@@ -201,26 +270,34 @@ __global__ __launch_bounds__(256) void block8_weight_kernel(const T* __restrict_
   }
 }
 
-// workgroups of a streaming launch: 16 blocks each, at most eight per CU
-static unsigned stream_grid(long long blocks) {
-  const long long want = (blocks + 15) / 16;
+// workgroups of a streaming launch: 16 `unroll` blocks each a turn, at most eight per CU
+static unsigned stream_grid(long long blocks, int unroll) {
+  const long long want = (blocks + 16 * unroll - 1) / (16 * unroll);
   return (unsigned)(want < 2048 ? want : 2048);
 }
 
 template <class T>
 static int rows_run(const void* x, long long R, int K, long long ld, void* codes, void* scales, int act, void* y, hipStream_t st) {
-  const unsigned grid = stream_grid(R * row_blocks(K));
+  const unsigned grid = stream_grid(R * row_blocks(K), 8 / sizeof(T));
+  const bool flat = K % (4 * kBlock) == 0 && ld == K;
 #define HECKA_ROWS(A) \
-  case A: block8_rows_kernel<T, A><<<grid, 256, 0, st>>>((const T*)x, R, K, ld, (unsigned char*)codes, (unsigned char*)scales, (T*)y); break;
+  case A: \
+    if (flat) block8_rows_kernel<T, A, true><<<grid, 256, 0, st>>>((const T*)x, R, K, ld, (unsigned char*)codes, (unsigned char*)scales, (T*)y); \
+    else block8_rows_kernel<T, A, false><<<grid, 256, 0, st>>>((const T*)x, R, K, ld, (unsigned char*)codes, (unsigned char*)scales, (T*)y); \
+    break;
   switch (act) { HECKA_ROWS(kActNone) HECKA_ROWS(kActGelu) HECKA_ROWS(kActSilu) HECKA_ROWS(kActTanh) HECKA_ROWS(kActSigmoid) HECKA_ROWS(kActCrater) }
 #undef HECKA_ROWS
   return check_launch("block8_rows");
 }
 template <class T>
 static int values_run(const void* codes, const void* scales, const void* dy, long long R, int K, int act, void* out, hipStream_t st) {
-  const unsigned grid = stream_grid(R * row_blocks(K));
+  const unsigned grid = stream_grid(R * row_blocks(K), act == kActNone ? 4 : 8 / sizeof(T));
+  const bool flat = K % (4 * kBlock) == 0;
 #define HECKA_VALUES(A) \
-  case A: block8_values_kernel<T, A><<<grid, 256, 0, st>>>((const unsigned char*)codes, (const unsigned char*)scales, (const T*)dy, R, K, (T*)out); break;
+  case A: \
+    if (flat) block8_values_kernel<T, A, true><<<grid, 256, 0, st>>>((const unsigned char*)codes, (const unsigned char*)scales, (const T*)dy, R, K, (T*)out); \
+    else block8_values_kernel<T, A, false><<<grid, 256, 0, st>>>((const unsigned char*)codes, (const unsigned char*)scales, (const T*)dy, R, K, (T*)out); \
+    break;
   switch (act) { HECKA_VALUES(kActNone) HECKA_VALUES(kActGelu) HECKA_VALUES(kActSilu) HECKA_VALUES(kActTanh) HECKA_VALUES(kActSigmoid) HECKA_VALUES(kActCrater) }
 #undef HECKA_VALUES
   return check_launch("block8_values");

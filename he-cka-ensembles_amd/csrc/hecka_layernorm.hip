@@ -71,10 +71,10 @@ __device__ __forceinline__ void load_params(float (&v)[NV * Piece<T>::N], const 
 }
 
 template <class T, int TPR, int NV>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layernorm_fwd_kernel(
+__global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void layernorm_fwd_kernel(
     const T* __restrict__ x, long long R, int D, int chunks, const float* __restrict__ w, const float* __restrict__ b,
     long long wstride, float eps, T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd) {
-  constexpr int N = Piece<T>::N, RPB = TPR < 256 ? 256 / TPR : 1;
+  constexpr int N = Piece<T>::N, RPB = TPR <= 64 ? 256 / TPR : 1;
   __shared__ float red[2][TPR < 64 ? 1 : TPR / 64];
   const long long m = blockIdx.x / chunks, step = (long long)chunks * RPB;
   const int chunk = blockIdx.x % chunks, sub = threadIdx.x / TPR, lane = threadIdx.x % TPR;
@@ -110,48 +110,55 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layernorm_fwd_kernel(
   }
 }
 
-template <class T, int TPR, int NV>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layernorm_bwd_kernel(
+// AHEAD: the next row's pieces are loaded while a row is summed (up to 8 elements per thread).  Otherwise (16 elements) the
+// registers hold one row, and what a row's sums took from its pieces is worked out again for dx.
+template <class T, int TPR, int NV, bool AHEAD>
+__global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void layernorm_bwd_kernel(
     const T* __restrict__ dy, const T* __restrict__ x, const float* __restrict__ mean, const float* __restrict__ rstd,
     long long R, int D, int chunks, const float* __restrict__ w, long long wstride, T* __restrict__ dx,
     float* __restrict__ dw, float* __restrict__ db, long long gstride, long long pstride) {
-  constexpr int N = Piece<T>::N, RPB = TPR < 256 ? 256 / TPR : 1;
+  constexpr int N = Piece<T>::N, E = NV * N, RPB = TPR <= 64 ? 256 / TPR : 1;
   __shared__ float red[2][TPR < 64 ? 1 : TPR / 32];
-  __shared__ float fold[RPB > 1 ? RPB - 1 : 1][RPB > 1 ? TPR : 1][RPB > 1 ? 2 * NV * N + 1 : 1];
+  __shared__ float fold[RPB > 1 ? RPB - 1 : 1][RPB > 1 ? TPR : 1][RPB > 1 ? 2 * E + 1 : 1];
   const long long m = blockIdx.x / chunks, step = (long long)chunks * RPB;
   const int chunk = blockIdx.x % chunks, sub = threadIdx.x / TPR, lane = threadIdx.x % TPR;
-  float wr[NV * N], aw[NV * N], ab[NV * N];
+  float wr[E], aw[E], ab[E];
   Piece<T> px[NV], pd[NV];
   long long r = (long long)chunk * RPB + sub;
   x += m * R * D;
   dy += m * R * D;
   mean += m * R;
   rstd += m * R;
-  load_row<T, TPR, NV>(px, x, r, R, D, lane);
-  load_row<T, TPR, NV>(pd, dy, r, R, D, lane);
-  float mu = mean[r < R ? r : R - 1], rs = rstd[r < R ? r : R - 1];
+  if (AHEAD) {
+    load_row<T, TPR, NV>(px, x, r, R, D, lane);
+    load_row<T, TPR, NV>(pd, dy, r, R, D, lane);
+  }
   load_params<T, TPR, NV>(wr, w ? w + m * wstride : nullptr, D, lane, 1.f);
 #pragma unroll
-  for (int k = 0; k < NV * N; ++k) aw[k] = ab[k] = 0.f;
+  for (int k = 0; k < E; ++k) aw[k] = ab[k] = 0.f;
   const float inv = 1.0f / (float)D;
   int turn = 0;
   for (; r < R; r += step, turn ^= 1) {
-    float g[NV * N], h[NV * N], s1 = 0.f, s2 = 0.f;
-    const float rt = rs;
-#pragma unroll
-    for (int k = 0; k < NV * N; ++k) {
-      const float d = widen(pd[k / N].e[k % N]);      // zero behind the row's end, as g then is: nothing of it enters the sums
-      h[k] = (widen(px[k / N].e[k % N]) - mu) * rt;
-      aw[k] = fmaf(d, h[k], aw[k]);
-      ab[k] += d;
-      g[k] = d * wr[k];
-      s1 += g[k];
-      s2 = fmaf(g[k], h[k], s2);
+    const float mu = mean[r], rs = rstd[r];
+    if (!AHEAD) {
+      load_row<T, TPR, NV>(px, x, r, R, D, lane);
+      load_row<T, TPR, NV>(pd, dy, r, R, D, lane);
     }
-    load_row<T, TPR, NV>(px, x, r + step, R, D, lane);
-    load_row<T, TPR, NV>(pd, dy, r + step, R, D, lane);
-    mu = mean[r + step < R ? r + step : R - 1];
-    rs = rstd[r + step < R ? r + step : R - 1];
+    float g[AHEAD ? E : 1], h[AHEAD ? E : 1], s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+      const float d = widen(pd[k / N].e[k % N]);      // zero behind the row's end, as d w then is: nothing of it enters the sums
+      const float xh = (widen(px[k / N].e[k % N]) - mu) * rs, dw_ = d * wr[k];
+      aw[k] = fmaf(d, xh, aw[k]);
+      ab[k] += d;
+      s1 += dw_;
+      s2 = fmaf(dw_, xh, s2);
+      if (AHEAD) { g[k] = dw_; h[k] = xh; }
+    }
+    if (AHEAD) {
+      load_row<T, TPR, NV>(px, x, r + step, R, D, lane);
+      load_row<T, TPR, NV>(pd, dy, r + step, R, D, lane);
+    }
     if (dx) {
       row_sum2<TPR>(s1, s2, red[turn]);
       s1 *= inv;
@@ -160,7 +167,12 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layernorm_bwd_kernel(
       for (int j = 0; j < NV; ++j) {
         Piece<T> o;
 #pragma unroll
-        for (int i = 0; i < N; ++i) narrow(rt * (g[j * N + i] - s1 - h[j * N + i] * s2), o.e[i]);
+        for (int i = 0; i < N; ++i) {
+          const int k = j * N + i;
+          const float gk = AHEAD ? g[AHEAD ? k : 0] : widen(pd[j].e[i]) * wr[k];
+          const float hk = AHEAD ? h[AHEAD ? k : 0] : (widen(px[j].e[i]) - mu) * rs;
+          narrow(rs * (gk - s1 - hk * s2), o.e[i]);
+        }
         store_piece(dx + (m * R + r) * D, (j * TPR + lane) * N, D, o);
       }
     }
@@ -218,31 +230,38 @@ __global__ __launch_bounds__(1024) void layernorm_fold_kernel(const float* __res
 
 static const int kMaxNormWidth = 16384;
 
-// threads of a row: few enough that most have work (a piece is 4 or 8 elements), enough that none has more than 16 elements
-static int norm_threads(int D, int piece) {
-  return D <= 16 * piece ? 16 : D <= 32 * piece ? 32 : D <= 1024 ? 64 : D <= 4096 ? 256 : D <= 8192 ? 512 : 1024;
+// Threads of a row: few enough that most have work (a piece is 4 or 8 elements), enough that none has more than 16 elements
+// (forward) or 8 (backward, which holds five values for each and would leave too few waves: bf16 rows of 8192 350 us with 8
+// elements in 1024 threads, 475 us with 16 in 512).  Beyond 8192 the backward has 16 as well and loads nothing ahead.
+static int norm_threads(int D, int piece, bool forward) {
+  if (D <= 16 * piece) return 16;
+  if (D <= 32 * piece) return 32;
+  const int share = forward || D > 8192 ? 16 : 8;
+  if (forward ? D <= 1024 : D <= 512) return 64;
+  return D <= 128 * share ? 128 : D <= 256 * share ? 256 : D <= 512 * share ? 512 : 1024;
 }
 
 // Workgroups per member: every row its own share, up to `most` in all.  Forward: eight per CU, but for long rows (whose weight
-// and bias, 8 bytes an element, a workgroup reads once) two.  Backward: enough to fill the chip once, so that the partial sums
-// stay a few per cent of the traffic.
+// and bias, 8 bytes an element, a workgroup reads once) two.  Backward: enough to fill the chip once with sixteen waves per CU,
+// so that the partial sums stay a few per cent of the traffic.
 static int norm_chunks(long long G, long long R, int threads, bool forward) {
-  const int rpb = threads < 256 ? 256 / threads : 1;
-  const long long most = threads >= 1024 ? 512 : threads == 512 ? (forward ? 1024 : 512) : forward ? 2048 : 1024;
+  const int rpb = threads <= 64 ? 256 / threads : 1;
+  const long long most = forward ? (threads >= 1024 ? 512 : threads == 512 ? 1024 : 2048) : threads <= 256 ? (threads == 128 ? 2048 : 1024) : threads == 512 ? 512 : 256;
   const long long want = (R + rpb - 1) / rpb, share = most / G < 1 ? 1 : most / G;
   return (int)(want < share ? want : share);
 }
 
 template <class T, class F>
-static int norm_dispatch(int D, const F& f) {
+static int norm_dispatch(int D, bool forward, const F& f) {
   constexpr int N = Piece<T>::N;
-  const int t = norm_threads(D, N), need = (D + t * N - 1) / (t * N);      // pieces per thread: 1, 2 or (fp32) 4
+  const int t = norm_threads(D, N, forward), need = (D + t * N - 1) / (t * N);      // pieces per thread: 1, 2 or (fp32) 4
 #define HECKA_NORM(TPR) \
   case TPR: return need <= 1 ? f.template run<T, TPR, 1>() : need <= 2 ? f.template run<T, TPR, 2>() : f.template run<T, TPR, 16 / N>();
   switch (t) {
     case 16: return f.template run<T, 16, 1>();
     case 32: return f.template run<T, 32, 1>();
     HECKA_NORM(64)
+    HECKA_NORM(128)
     HECKA_NORM(256)
     HECKA_NORM(512)
     HECKA_NORM(1024)
@@ -255,7 +274,7 @@ struct NormFwd {
   const void* x; long long G, R; int D; const float *w, *b; long long wstride; float eps; void* y; float *mean, *rstd; hipStream_t st;
   template <class T, int TPR, int NV> int run() const {
     const int chunks = norm_chunks(G, R, TPR, true);
-    layernorm_fwd_kernel<T, TPR, NV><<<dim3((unsigned)(G * chunks)), TPR < 256 ? 256 : TPR, 0, st>>>(
+    layernorm_fwd_kernel<T, TPR, NV><<<dim3((unsigned)(G * chunks)), TPR <= 64 ? 256 : TPR, 0, st>>>(
         (const T*)x, R, D, chunks, w, b, wstride, eps, (T*)y, mean, rstd);
     return check_launch("layernorm_fwd");
   }
@@ -263,9 +282,10 @@ struct NormFwd {
 struct NormBwd {
   const void *dy, *x; const float *mean, *rstd; long long G, R; int D; const float* w; long long wstride; void* dx; float *dw, *db; long long gstride; float* ws; hipStream_t st;
   template <class T, int TPR, int NV> int run() const {
+    constexpr bool AHEAD = NV * Piece<T>::N <= 8;
     const int chunks = norm_chunks(G, R, TPR, false);
     const bool part = chunks > 1 && (dw || db);
-    layernorm_bwd_kernel<T, TPR, NV><<<dim3((unsigned)(G * chunks)), TPR < 256 ? 256 : TPR, 0, st>>>(
+    layernorm_bwd_kernel<T, TPR, NV, AHEAD><<<dim3((unsigned)(G * chunks)), TPR <= 64 ? 256 : TPR, 0, st>>>(
         (const T*)dy, (const T*)x, mean, rstd, R, D, chunks, w, wstride, (T*)dx, part ? ws : dw, part ? ws + D : db,
         part ? (long long)chunks * 2 * D : gstride, part ? 2LL * D : 0);
     if (part)
@@ -275,8 +295,9 @@ struct NormBwd {
 };
 
 template <class F>
-static int norm_type(int dtype, int D, const F& f) {
-  return dtype == HECKA_DT_F32 ? norm_dispatch<float>(D, f) : dtype == HECKA_DT_BF16 ? norm_dispatch<Bf16>(D, f) : norm_dispatch<F16>(D, f);
+static int norm_type(int dtype, int D, bool forward, const F& f) {
+  return dtype == HECKA_DT_F32 ? norm_dispatch<float>(D, forward, f)
+         : dtype == HECKA_DT_BF16 ? norm_dispatch<Bf16>(D, forward, f) : norm_dispatch<F16>(D, forward, f);
 }
 
 static int norm_check(const char* what, int dtype, int G, long long R, int D) {
@@ -297,12 +318,12 @@ int hecka_layernorm_fwd(const void* x, int dtype, int G, long long R, int D, con
   if (int rc = norm_check("layernorm_fwd", dtype, G, R, D)) return rc;
   if (!x || !y || !mean != !rstd) return fail(HECKA_EINVAL, "layernorm_fwd: null pointer%s");
   clear_error();
-  return norm_type(dtype, D, NormFwd{x, G, R, D, weight, bias, wstride, eps, y, mean, rstd, (hipStream_t)stream});
+  return norm_type(dtype, D, true, NormFwd{x, G, R, D, weight, bias, wstride, eps, y, mean, rstd, (hipStream_t)stream});
 }
 
 size_t hecka_layernorm_bwd_workspace_bytes(int G, long long R, int D) {
   if (G <= 0 || R <= 0 || D <= 0 || G > 65535 || D > kMaxNormWidth) return 0;
-  const int fp32 = norm_chunks(G, R, norm_threads(D, 4), false), other = norm_chunks(G, R, norm_threads(D, 8), false);
+  const int fp32 = norm_chunks(G, R, norm_threads(D, 4, false), false), other = norm_chunks(G, R, norm_threads(D, 8, false), false);
   const int chunks = fp32 > other ? fp32 : other;
   return chunks > 1 ? (size_t)G * chunks * 2 * D * sizeof(float) : 0;
 }
@@ -316,7 +337,7 @@ int hecka_layernorm_bwd(const void* dy, const void* x, int dtype, const float* m
   if ((dweight || dbias) && (ws ? ws_bytes : 0) < hecka_layernorm_bwd_workspace_bytes(G, R, D))
     return fail(HECKA_EWORKSPACE, "%slayernorm_bwd: workspace too small (%lld bytes given)", "", (long long)ws_bytes);
   clear_error();
-  return norm_type(dtype, D, NormBwd{dy, x, mean, rstd, G, R, D, weight, wstride, dx, dweight, dbias, gstride, (float*)ws,
+  return norm_type(dtype, D, false, NormBwd{dy, x, mean, rstd, G, R, D, weight, wstride, dx, dweight, dbias, gstride, (float*)ws,
                                      (hipStream_t)stream});
 }
 
