@@ -40,6 +40,81 @@ __device__ __forceinline__ float encodable(float x) {
   return a <= top ? x : a <= 3.402823466e38f ? copysignf(top, x) : __uint_as_float(0x7fc00000u);
 }
 
+// A lane's 32 elements of a block (Piece<T>s), the block's other elements in the lanes 16, 32 and 48 further on: codes as eight
+// dwords, and the scale byte.  Magnitudes are compared as integers (two 16-bit ones at a time), which finds NaN and infinities on
+// the way; without any, and below 240 2^120, the conversion takes the elements as they are and divides by the scale itself.
+template <class T> struct Magnitude { static constexpr unsigned kLast = 0x7f70; };      // of bf16: 240 2^120
+template <> struct Magnitude<float> { static constexpr unsigned kLast = 0x7f700000; };
+template <> struct Magnitude<F16> { static constexpr unsigned kLast = 0x7bff; };
+typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+typedef short i16x2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+
+template <class T>
+__device__ __forceinline__ int encode32(const Piece<T> (&p)[32 / Piece<T>::N], unsigned (&codes)[8]) {
+  constexpr int D = sizeof(T) == 4 ? 32 : 16;      // dwords
+  const unsigned* raw = reinterpret_cast<const unsigned*>(&p[0]);
+  unsigned big = 0;
+#pragma unroll
+  for (int i = 0; i < D; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      const unsigned a = raw[i] & 0x7fffffffu;
+      big = a > big ? a : big;
+    } else {
+      const u16x2_t a = __builtin_bit_cast(u16x2_t, raw[i] & 0x7fff7fffu);
+      big = __builtin_bit_cast(unsigned, __builtin_elementwise_max(a, __builtin_bit_cast(u16x2_t, big)));
+    }
+  }
+  if constexpr (sizeof(T) == 2) {
+    const unsigned hi = big >> 16, lo = big & 0xffffu;
+    big = hi > lo ? hi : lo;
+  }
+  unsigned o = (unsigned)__shfl_xor((int)big, 16);
+  big = o > big ? o : big;
+  o = (unsigned)__shfl_xor((int)big, 32);
+  big = o > big ? o : big;
+  if (__any(big > Magnitude<T>::kLast)) {
+    float v[32], a = 0.f;
+#pragma unroll
+    for (int k = 0; k < 32; ++k) {
+      v[k] = widen(p[k / Piece<T>::N].e[k % Piece<T>::N]);
+      a = fmaxf(a, finite_abs(v[k]));
+      v[k] = encodable(v[k]);
+    }
+    a = fmaxf(a, __shfl_xor(a, 16));
+    a = fmaxf(a, __shfl_xor(a, 32));
+    const int byte = scale_byte(a);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) codes[i] = encode4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], inverse_scale(byte));
+    return byte;
+  }
+  T top;
+  if constexpr (sizeof(T) == 4) top = __uint_as_float(big);
+  else top = __builtin_bit_cast(T, (unsigned short)big);
+  const int byte = scale_byte(widen(top));
+  const float s = scale_of(byte);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    i16x2_t c = {0, 0};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if constexpr (sizeof(T) == 4) {
+        const float a = __uint_as_float(raw[4 * i + 2 * h]), b = __uint_as_float(raw[4 * i + 2 * h + 1]);
+        c = h ? __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c, a, b, s, true) : __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c, a, b, s, false);
+      } else if constexpr (__is_same(T, Bf16)) {
+        const bf16x2_t a = __builtin_bit_cast(bf16x2_t, raw[2 * i + h]);
+        c = h ? __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(c, a, s, true) : __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(c, a, s, false);
+      } else {
+        const f16x2_t a = __builtin_bit_cast(f16x2_t, raw[2 * i + h]);
+        c = h ? __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(c, a, s, true) : __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(c, a, s, false);
+      }
+    }
+    codes[i] = __builtin_bit_cast(unsigned, c);
+  }
+  return byte;
+}
+
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void decode4(unsigned c, float s, float* v) {
   const f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);

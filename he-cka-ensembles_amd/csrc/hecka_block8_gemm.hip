@@ -292,17 +292,17 @@ __global__ __launch_bounds__(256) void block8_linear_kernel(
 
 // ------------------------------------------------------------------------------------------------------------------
 // The same product for up to sixteen rows x (fp32 / bf16 / fp16) that are not in codes yet: one launch.  It reads every weight
-// code once, which is what bounds it, so nothing is staged: a wave takes 16 NT weight rows, its four-way share of the blocks
-// of K, and reads 32 codes per lane and row; each wave makes the codes of x for its blocks by itself (the same codes as
+// code once, which is what bounds it, so nothing is staged: a wave takes 16 NT weight rows, its W-th share of the blocks of K,
+// reads 32 codes per lane and row, a block ahead, and makes the codes of x for its blocks by itself (the same codes as
 // hecka_block8_quantize: 32 elements per lane, the maximum over the four lanes of a row).  All products in bf16, exact.
-// The four waves' sums are added in order.
+// The W waves' sums are added in order.
 // ------------------------------------------------------------------------------------------------------------------
-template <class T, int NT>
-__global__ __launch_bounds__(256) void block8_token_kernel(const T* __restrict__ x, long long xstride, int N, int K,
-                                                           const unsigned char* __restrict__ w, const unsigned char* __restrict__ ws,
-                                                           int O, const float* __restrict__ bias, long long bstride, float alpha, float beta,
-                                                           T* __restrict__ y) {
-  __shared__ f32x4v red[4][NT][64];
+template <class T, int NT, int W>
+__global__ __launch_bounds__(64 * W) void block8_token_kernel(const T* __restrict__ x, long long xstride, int N, int K,
+                                                              const unsigned char* __restrict__ w, const unsigned char* __restrict__ ws,
+                                                              int O, const float* __restrict__ bias, long long bstride, float alpha, float beta,
+                                                              T* __restrict__ y) {
+  __shared__ f32x4v red[W][NT][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g = lane >> 4;
   const int nblk = row_blocks(K), sstride = scale_stride(K), o0 = blockIdx.x * 16 * NT;
   const long long m = blockIdx.y, Kp = (long long)nblk * kBlock;
@@ -315,39 +315,38 @@ __global__ __launch_bounds__(256) void block8_token_kernel(const T* __restrict__
     pw[i] = w + (long long)(o < O ? o : O - 1) * Kp + g * 32;
   }
   ws += (m * ((O + kBlock - 1) / kBlock) + o0 / kBlock) * sstride;      // 16 NT <= 128 rows of one block
-  f32x4v acc[NT];
-#pragma unroll
-  for (int i = 0; i < NT; ++i) acc[i] = f32x4v{0.f, 0.f, 0.f, 0.f};
-  for (int kb = wave; kb < nblk; kb += 4) {
-    i32x4 c[NT][2];
+  constexpr int PX = 32 / Piece<T>::N;
+  i32x4 c[NT][2];
+  Piece<T> px[PX];
+  int sb = 127;
+  auto load = [&](int kb) {
+    kb = kb < nblk ? kb : nblk - 1;
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       c[i][0] = *reinterpret_cast<const i32x4*>(pw[i] + (long long)kb * kBlock);
       c[i][1] = *reinterpret_cast<const i32x4*>(pw[i] + (long long)kb * kBlock + 16);
     }
-    float v[32], a = 0.f;
 #pragma unroll
-    for (int j = 0; j < 32 / Piece<T>::N; ++j) {
-      const Piece<T> p = load_piece(x, kb * kBlock + g * 32 + j * Piece<T>::N, K);
+    for (int j = 0; j < PX; ++j) px[j] = load_piece(x, kb * kBlock + g * 32 + j * Piece<T>::N, K);
+    sb = ws[kb];
+  };
+  f32x4v acc[NT];
 #pragma unroll
-      for (int i = 0; i < Piece<T>::N; ++i) {
-        v[j * Piece<T>::N + i] = widen(p.e[i]);
-        a = fmaxf(a, finite_abs(v[j * Piece<T>::N + i]));
-      }
-    }
-    a = fmaxf(a, __shfl_xor(a, 16));
-    a = fmaxf(a, __shfl_xor(a, 32));
-    const int byte = scale_byte(a);
-    const float inv = inverse_scale(byte), sx = scale_of(byte), sw = scale_of(ws[kb]);
+  for (int i = 0; i < NT; ++i) acc[i] = f32x4v{0.f, 0.f, 0.f, 0.f};
+  if (wave < nblk) load(wave);
+  for (int kb = wave; kb < nblk; kb += W) {
+    i32x4 d[NT][2];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) { d[i][0] = c[i][0]; d[i][1] = c[i][1]; }
+    unsigned cx[8];
+    const float sx = scale_of(encode32(px, cx)), sw = scale_of(sb);
+    load(kb + W);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[q * 8 + i] = encodable(v[q * 8 + i]);
-      const bf16x8 bx = widen8(encode4(v[q * 8], v[q * 8 + 1], v[q * 8 + 2], v[q * 8 + 3], inv),
-                               encode4(v[q * 8 + 4], v[q * 8 + 5], v[q * 8 + 6], v[q * 8 + 7], inv), sx);
+      const bf16x8 bx = widen8(cx[2 * q], cx[2 * q + 1], sx);
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
-        const bf16x8 bw = widen8(c[i][q >> 1][(q & 1) * 2], c[i][q >> 1][(q & 1) * 2 + 1], sw);
+        const bf16x8 bw = widen8(d[i][q >> 1][(q & 1) * 2], d[i][q >> 1][(q & 1) * 2 + 1], sw);
         acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bw, bx, acc[i], 0, 0, 0);
       }
     }
@@ -355,10 +354,10 @@ __global__ __launch_bounds__(256) void block8_token_kernel(const T* __restrict__
 #pragma unroll
   for (int i = 0; i < NT; ++i) red[wave][i][lane] = acc[i];
   __syncthreads();
-  for (int i = wave; i < NT; i += 4) {
+  for (int i = wave; i < NT; i += W) {
     f32x4v s = red[0][i][lane];
 #pragma unroll
-    for (int k = 1; k < 4; ++k) s += red[k][i][lane];
+    for (int k = 1; k < W; ++k) s += red[k][i][lane];
     const int o = o0 + i * 16 + 4 * g;
     if (l16 < N) {
 #pragma unroll
@@ -609,8 +608,29 @@ static int linear_run(const void* x, const void* xs, long long xstride, long lon
 template <class T>
 static int token_run(const void* x, long long xstride, int M, int N, int K, const void* w, const void* ws, int O,
                      const float* bias, long long bstride, float alpha, float beta, void* y, hipStream_t st) {
-  block8_token_kernel<T, 2><<<dim3(cdiv(O, 32), M), 256, 0, st>>>((const T*)x, xstride, N, K, (const unsigned char*)w,
-                                                               (const unsigned char*)ws, O, bias, bstride, alpha, beta, (T*)y);
+#define HECKA_TOKEN(NT, W) \
+  block8_token_kernel<T, NT, W><<<dim3(cdiv(O, 16 * NT), M), 64 * W, 0, st>>>((const T*)x, xstride, N, K, (const unsigned char*)w, \
+                                                                           (const unsigned char*)ws, O, bias, bstride, alpha, beta, (T*)y)
+  // Sixteen weight rows a wave where that makes few waves, 32 otherwise (a workgroup reads all of x, and makes its codes); K is
+  // shared out to as many waves as fill the chip, two blocks each at least where there are many.  Measured (bf16, weights from HBM):
+  // 8 x 4096 x 4096, one row, 40 us with 32 rows x 4 waves, 55 us with 16 x 4; 1 x 4096 x 4096 11 us with 16 x 8, 17 us with 32 x 4;
+  // 1 x 8192 x 8192, sixteen rows, 29 us with 32 x 8, 35 us with 16 x 8; 1 x 1000 x 8192 12 us with 16 x 16, 23 us with 16 x 4.
+  const long long rows16 = (long long)M * cdiv(O, 16);
+  const int nblk = row_blocks(K);
+  if (rows16 >= 512) {
+    if (rows16 >= 1024 || nblk < 16) HECKA_TOKEN(2, 4);
+    else HECKA_TOKEN(2, 8);
+  } else if (rows16 >= 128) {
+    if (nblk < 16) HECKA_TOKEN(1, 4);
+    else HECKA_TOKEN(1, 8);
+  } else if (nblk <= 4) {
+    HECKA_TOKEN(1, 4);
+  } else if (nblk < 32) {
+    HECKA_TOKEN(1, 8);
+  } else {
+    HECKA_TOKEN(1, 16);
+  }
+#undef HECKA_TOKEN
   return check_launch("block8_token");
 }
 
