@@ -105,18 +105,20 @@ __device__ __forceinline__ i32x4 half4(i32x8 v, int h) {
 }
 // The products as asm: all 256 accumulation registers of a lane are sums here, and the compiler, left to itself, moves sums
 // about to place a result elsewhere than its addend, and the instructions to where they hide nothing.  What an instruction
-// needs then is up to this code: two idle cycles behind a vector instruction that wrote an operand (s_nop 1, free in the shadow
-// of the instruction before), and 18 behind the last product before a sum is read (mfma_settle).
+// needs then is up to this code: two idle issue slots behind a vector instruction that wrote an operand (mfma_ready, once before a
+// group of products whose operands are all there - most come from LDS and need none; an idle pair before every product cost 8 % of
+// the bf16 rate), and 18 behind the last product before a sum is read (mfma_settle).
 __device__ __forceinline__ void mfma_fp8(f32x4v& c, i32x8 a, i32x8 b, unsigned sa, unsigned sb) {
-  asm volatile("s_nop 1\n\tv_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0]" : "+a"(c) : "v"(a), "v"(b), "v"(sa), "v"(sb));
+  asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0]" : "+a"(c) : "v"(a), "v"(b), "v"(sa), "v"(sb));
 }
 __device__ __forceinline__ void mfma_bf16(f32x4v& c, i32x4 a, i32x4 b) {
-  asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+  asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }
 // sums in ordinary registers, which the compiler may copy about: done before anything behind it reads them
 __device__ __forceinline__ void mfma_bf16_now(f32x4v& c, i32x4 a, i32x4 b) {
   asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %2, %0\n\ts_nop 15\n\ts_nop 3" : "+v"(c) : "v"(a), "v"(b));
 }
+__device__ __forceinline__ void mfma_ready() { asm volatile("s_nop 1"); }
 __device__ __forceinline__ void mfma_settle() { asm volatile("s_nop 15\n\ts_nop 15"); }
 
 template <class T, bool EXACT, int B>
@@ -231,6 +233,8 @@ __global__ __launch_bounds__(256) void block8_linear_kernel(
       }
       __builtin_amdgcn_sched_barrier(0);
       const i32x8 fw = ready(aw[i], c.sw);
+      __builtin_amdgcn_sched_barrier(0);
+      mfma_ready();
 #pragma unroll
       for (int e = 0; e < U * TN; ++e) {
         const int j = e % TN;
@@ -497,7 +501,8 @@ __global__ __launch_bounds__(256) void block8_wgrad_kernel(
   // is left of the step is in registers, the next step is in the other buffer, and the barrier there is the step's only one:
   // behind it the next step's first fragments are read, and this step's buffer takes the step after that.
   constexpr int GROUPS = S * TT * TERMS, TURN = GROUPS * 3 / 4, TAIL = GROUPS - TURN, SLOTS = GROUPS * TT;
-  i32x4 fx[2][TT], fd0;
+  constexpr int LEAD = 1;      // groups between a fragment's read and its use
+  i32x4 fx[2][TT], fd0[LEAD];
   Source next;
   auto frag_d = [&](int e, int buf) {
     const int sub = e / (TT * TERMS), j = e / TERMS % TT, q = e % TERMS;
@@ -506,12 +511,13 @@ __global__ __launch_bounds__(256) void block8_wgrad_kernel(
   auto frag_x = [&](int i, int sub, int buf) { return frag(sm[buf] + TERMS * TILE + sub * 32 * B * 2, wi * TT + i); };
   auto step = [&](int k, int buf, int set) {      // set: which half of fx holds the step's first part
     i32x4 fd[GROUPS];
-    fd[0] = fd0;
+#pragma unroll
+    for (int e = 0; e < LEAD; ++e) fd[e] = fd0[e];
 #pragma unroll
     for (int e = 0; e < GROUPS; ++e) {
       const int sub = e / (TT * TERMS), j = e / TERMS % TT, hold = S == 2 ? sub : set;
-      if (e < TURN - 1) fd[e + 1] = frag_d(e + 1, buf);
-      if (e == TURN - 1) {
+      if (e + LEAD < TURN) fd[e + LEAD] = frag_d(e + LEAD, buf);
+      if (e == TURN - LEAD) {
 #pragma unroll
         for (int f = TURN; f < GROUPS; ++f) fd[f] = frag_d(f, buf);
       }
@@ -523,9 +529,10 @@ __global__ __launch_bounds__(256) void block8_wgrad_kernel(
       if (e >= TURN) {
 #pragma unroll
         for (int i = (e - TURN) * TT / TAIL; i < (e - TURN + 1) * TT / TAIL; ++i) fx[S == 2 ? 0 : set ^ 1][i] = frag_x(i, 0, buf ^ 1);
-        if (e == GROUPS - 1) fd0 = frag_d(0, buf ^ 1);
+        if (e >= GROUPS - LEAD) fd0[e - (GROUPS - LEAD)] = frag_d(e - (GROUPS - LEAD), buf ^ 1);
       }
       __builtin_amdgcn_sched_barrier(0);
+      mfma_ready();
 #pragma unroll
       for (int i = 0; i < TT; ++i) {
         mfma_bf16(acc[i][j], fx[hold][i], fd[e]);
@@ -553,7 +560,8 @@ __global__ __launch_bounds__(256) void block8_wgrad_kernel(
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < TT; ++i) fx[0][i] = frag_x(i, 0, 0);
-  fd0 = frag_d(0, 0);
+#pragma unroll
+  for (int e = 0; e < LEAD; ++e) fd0[e] = frag_d(e, 0);
   // two steps a turn of the loop, so that buffers and fragments have fixed places (a step behind the last one adds zeros)
   for (int k = 0; k < steps; k += 2) {
     step(k, 0, 0);
