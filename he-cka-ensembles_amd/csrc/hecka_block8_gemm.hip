@@ -103,7 +103,7 @@ template <> struct Raw<true> { typedef i32x4 type; };
 __device__ __forceinline__ i32x4 half4(i32x8 v, int h) {
   return h ? __builtin_shufflevector(v, v, 4, 5, 6, 7) : __builtin_shufflevector(v, v, 0, 1, 2, 3);
 }
-// The products as asm: all 256 accumulation registers of a lane are sums here, and the compiler, left to itself, moves sums
+// The products of the 256 x 256 tiles as asm: all 256 accumulation registers of a lane are sums here, and the compiler, left to itself, moves sums
 // about to place a result elsewhere than its addend, and the instructions to where they hide nothing.  What an instruction
 // needs then is up to this code: two idle issue slots behind a vector instruction that wrote an operand (mfma_ready, once before a
 // group of products whose operands are all there - most come from LDS and need none; an idle pair before every product cost 8 % of
@@ -114,9 +114,20 @@ __device__ __forceinline__ void mfma_fp8(f32x4v& c, i32x8 a, i32x8 b, unsigned s
 __device__ __forceinline__ void mfma_bf16(f32x4v& c, i32x4 a, i32x4 b) {
   asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }
-// sums in ordinary registers, which the compiler may copy about: done before anything behind it reads them
-__device__ __forceinline__ void mfma_bf16_now(f32x4v& c, i32x4 a, i32x4 b) {
-  asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %2, %0\n\ts_nop 15\n\ts_nop 3" : "+v"(c) : "v"(a), "v"(b));
+// A sum in ordinary registers: settled (mfma_settle) before the compiler can touch it.
+__device__ __forceinline__ void add_columns(f32x4v& c, i32x4 a, i32x4 b) {
+  asm volatile("s_nop 3\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
+}
+// The same by the compiler's own means, which waits for what needs it: for the smaller tiles, whose sums leave it registers.
+template <bool OWN>
+__device__ __forceinline__ void mul_fp8(f32x4v& c, i32x8 a, i32x8 b, unsigned sa, unsigned sb) {
+  if constexpr (OWN) mfma_fp8(c, a, b, sa, sb);
+  else c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, (int)sa, 0, (int)sb);
+}
+template <bool OWN>
+__device__ __forceinline__ void mul_bf16(f32x4v& c, i32x4 a, i32x4 b) {
+  if constexpr (OWN) mfma_bf16(c, a, b);
+  else c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 __device__ __forceinline__ void mfma_ready() { asm volatile("s_nop 1"); }
 __device__ __forceinline__ void mfma_settle() { asm volatile("s_nop 15\n\ts_nop 15"); }
@@ -234,12 +245,12 @@ __global__ __launch_bounds__(256) void block8_linear_kernel(
       __builtin_amdgcn_sched_barrier(0);
       const i32x8 fw = ready(aw[i], c.sw);
       __builtin_amdgcn_sched_barrier(0);
-      mfma_ready();
+      if (B == 256) mfma_ready();
 #pragma unroll
       for (int e = 0; e < U * TN; ++e) {
         const int j = e % TN;
-        if constexpr (EXACT) mfma_bf16(acc[i][j], half4(fw, e / TN), half4(c.fx[j], e / TN));
-        else mfma_fp8(acc[i][j], fw, c.fx[j], c.sw, c.sx[j]);
+        if constexpr (EXACT) mul_bf16<B == 256>(acc[i][j], half4(fw, e / TN), half4(c.fx[j], e / TN));
+        else mul_fp8<B == 256>(acc[i][j], fw, c.fx[j], c.sw, c.sx[j]);
         // step kb + 2 into the freed buffer: the loads one by one between the products, because a load that finds the queue full
         // holds up its wave
         if (turn && i >= SYNC) {
@@ -277,11 +288,13 @@ __global__ __launch_bounds__(256) void block8_linear_kernel(
   }
   if (kb < nblk * U) unit(kb, 0, p, q);
   wait_loads();      // the last steps' repeated loads write LDS: not past the end of the workgroup
-  mfma_settle();
+  if constexpr (B == 256) {
+    mfma_settle();
 #pragma unroll
-  for (int i = 0; i < TO; ++i)
+    for (int i = 0; i < TO; ++i)
 #pragma unroll
-    for (int j = 0; j < TN; ++j) asm volatile("" : "+a"(acc[i][j]));
+      for (int j = 0; j < TN; ++j) asm volatile("" : "+a"(acc[i][j]));
+  }
 
   Piece<float> bv[TO];
 #pragma unroll
@@ -413,41 +426,42 @@ __global__ __launch_bounds__(256) void block8_wgrad_kernel(
   float r[4];
   const int dn = tid / DPR, dc = (tid % DPR) * P, xn = tid / XPR, xc = (tid % XPR) * 16;
   const int dv = (dn * O + dc) * (int)sizeof(T), xv = xn * (int)Kp + xc, sv = xn * sstride + ((i0 + xc) >> 7);
-  struct Source { __amdgpu_buffer_rsrc_t dy, x, xs; long long k0; int left; };
-  auto source = [&](int step) {
-    Source q;
-    q.k0 = (long long)step * KS;
-    const long long left = last - first - q.k0;
-    q.left = left < 0 ? 0 : (int)left;
-    auto buffer = [](const void* p, long long bytes) {
-      return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes < 0 ? 0 : bytes > 0x7fffffff ? 0x7fffffff : (int)bytes, 0x00020000);
-    };
-    q.dy = buffer(dy + q.k0 * O + o0, ((long long)q.left * O - o0) * (long long)sizeof(T));
-    q.x = buffer(x + q.k0 * Kp + i0, q.left * Kp - i0);
-    q.xs = buffer(xs + q.k0 * sstride, (long long)q.left * sstride);
-    return q;
+  // where the loads' step begins, and what is left of each operand from there on; one step further with a few scalar instructions
+  struct Source { const T* dy; const unsigned char *x, *xs; long long dy_bytes, x_bytes; int left; };
+  const long long dy_step = (long long)KS * O, x_step = KS * Kp;
+  Source at = {dy + o0, x + i0, xs, ((long long)(last - first) * O - o0) * (long long)sizeof(T), (last - first) * Kp - i0, last - first};
+  auto advance = [&]() {
+    at.dy += dy_step;
+    at.x += x_step;
+    at.xs += KS * sstride;
+    at.dy_bytes -= dy_step * (long long)sizeof(T);
+    at.x_bytes -= x_step;
+    at.left -= KS;
   };
-  auto load_dy = [&](const Source& q, int item) {
+  auto buffer = [](const void* p, long long bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes < 0 ? 0 : bytes > 0x7fffffff ? 0x7fffffff : (int)bytes, 0x00020000);
+  };
+  auto load_dy = [&](int item) {
     if constexpr (WHOLE) {
-      rd[item] = __builtin_bit_cast(Piece<T>, __builtin_amdgcn_raw_buffer_load_b128(q.dy, dv + item * DROWS * O * (int)sizeof(T), 0, 0));
+      rd[item] = __builtin_bit_cast(Piece<T>, __builtin_amdgcn_raw_buffer_load_b128(buffer(at.dy, at.dy_bytes), dv + item * DROWS * O * (int)sizeof(T), 0, 0));
     } else {
       const int n = dn + item * DROWS;
-      rd[item] = load_piece(dy + (n < q.left ? q.k0 + n : 0) * O, n < q.left ? o0 + dc : O, O);
+      rd[item] = load_piece(n < at.left ? at.dy - o0 + (long long)n * O : dy, n < at.left ? o0 + dc : O, O);
     }
   };
-  auto load_x = [&](const Source& q, int item) {
-    rx[item] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(q.x, xv + item * XROWS * (int)Kp, 0, 0));
-    rs[item] = __builtin_amdgcn_raw_buffer_load_b8(q.xs, sv + item * XROWS * sstride, 0, 0);
+  auto load_x = [&](int item) {
+    rx[item] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(buffer(at.x, at.x_bytes), xv + item * XROWS * (int)Kp, 0, 0));
+    rs[item] = __builtin_amdgcn_raw_buffer_load_b8(buffer(at.xs, at.left < 0 ? 0 : (long long)at.left * sstride), sv + item * XROWS * sstride, 0, 0);
   };
   // the work on one item in parts of three to six instructions, few enough to pass in the shadow of a product
   constexpr int QUADS = P / 4, PERQ = TERMS == 1 ? 1 : (sizeof(T) == 2 ? 1 : 0) + 3 * (TERMS - 1) + 1;
   constexpr int PERD = TERMS == 1 ? 1 : QUADS * PERQ, PARTS = DL * PERD + 2 * XL;
-  auto part = [&](int id, int buf, const Source& next) {
+  auto part = [&](int id, int buf) {
     if (id < DL * PERD) {
       const int item = id / PERD, n = dn + item * DROWS;
-      unsigned char* at = sm[buf] + n * B * 2 + (((dc >> 4) ^ (n & 7)) * 32) + (dc & 15) * 2;
+      unsigned char* to = sm[buf] + n * B * 2 + (((dc >> 4) ^ (n & 7)) * 32) + (dc & 15) * 2;
       if constexpr (TERMS == 1) {
-        *reinterpret_cast<Piece<T>*>(at) = rd[item];
+        *reinterpret_cast<Piece<T>*>(to) = rd[item];
       } else {
         const int quad = id % PERD / PERQ;
         int what = id % PERQ;
@@ -459,41 +473,41 @@ __global__ __launch_bounds__(256) void block8_wgrad_kernel(
         if (what >= 0 && what % 3 == 0) {      // the next term of all four
           const uint2 c = make_uint2(__builtin_amdgcn_perm(__float_as_uint(r[1]), __float_as_uint(r[0]), 0x07060302),
                                      __builtin_amdgcn_perm(__float_as_uint(r[3]), __float_as_uint(r[2]), 0x07060302));
-          *reinterpret_cast<uint2*>(at + what / 3 * TILE + quad * 8) = c;
+          *reinterpret_cast<uint2*>(to + what / 3 * TILE + quad * 8) = c;
         } else if (what > 0) {                 // what is left of two of them
 #pragma unroll
           for (int e = what % 3 * 2 - 2; e < what % 3 * 2; ++e) r[e] -= __uint_as_float(__float_as_uint(r[e]) & 0xffff0000u);
         }
       }
-      if (id % PERD == PERD - 1) load_dy(next, item);
+      if (id % PERD == PERD - 1) load_dy(item);
     } else {
       const int j = (id - DL * PERD) / 2, h = (id - DL * PERD) % 2, n = xn + j * XROWS;
-      bf16x8* at = reinterpret_cast<bf16x8*>(sm[buf] + TERMS * TILE + n * B * 2 + (((xc >> 4) ^ (n & 7)) * 32));
-      at[h] = widen8(rx[j][2 * h], rx[j][2 * h + 1], scale_of(rs[j]));
-      if (h == 1) load_x(next, j);
+      bf16x8* to = reinterpret_cast<bf16x8*>(sm[buf] + TERMS * TILE + n * B * 2 + (((xc >> 4) ^ (n & 7)) * 32));
+      to[h] = widen8(rx[j][2 * h], rx[j][2 * h + 1], scale_of(rs[j]));
+      if (h == 1) load_x(j);
     }
   };
 
-  f32x4v acc[TT][TT], accb[TT];
+  f32x4v acc[TT][TT];
 #pragma unroll
-  for (int i = 0; i < TT; ++i) {
-    accb[i] = f32x4v{0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < TT; ++i)
 #pragma unroll
     for (int j = 0; j < TT; ++j) acc[i][j] = f32x4v{0.f, 0.f, 0.f, 0.f};
-  }
-  // the column sums: tile t of this workgroup's columns o belongs to one of the workgroups that share them, and there to one wave
-  unsigned sums = 0;
+  // The column sums: the TT tiles of a half of this workgroup's columns o are shared out to the 2 tiles_i waves that hold them; this
+  // wave has tiles mine, mine + 2 tiles_i, ... - with many tiles_i one at most.
+  constexpr int OWN = TT / 2;
+  const int mine = db ? ti * 2 + wi : TT;
+  f32x4v accb[OWN];
 #pragma unroll
-  for (int j = 0; j < TT; ++j)
-    if (db && (wo * TT + j) % tiles_i == ti && (((wo * TT + j) / tiles_i) & 1) == wi) sums |= 1u << j;
+  for (int n = 0; n < OWN; ++n) accb[n] = f32x4v{0.f, 0.f, 0.f, 0.f};
   const i32x4 ones = {0x3f803f80, 0x3f803f80, 0x3f803f80, 0x3f803f80};
 
   // fragment of 16 columns (unit u) of a tile: rows 4 g .. 4 g + 3 and 16 more down
   const int fr = (g * 4 + (l16 >> 2)) * B * 2 + (l16 & 3) * 8, sw = (g & 1) * 4 + (l16 >> 2);
   auto frag = [&](const unsigned char* tile, int u) {
-    const unsigned char* at = tile + fr + ((u ^ sw) * 32);
-    const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(at));
-    const i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(at + 16 * B * 2));
+    const unsigned char* from = tile + fr + ((u ^ sw) * 32);
+    const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(from));
+    const i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(from + 16 * B * 2));
     return __builtin_bit_cast(i32x4, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
   };
 
@@ -503,19 +517,23 @@ __global__ __launch_bounds__(256) void block8_wgrad_kernel(
   constexpr int GROUPS = S * TT * TERMS, TURN = GROUPS * 3 / 4, TAIL = GROUPS - TURN, SLOTS = GROUPS * TT;
   constexpr int LEAD = 1;      // groups between a fragment's read and its use
   i32x4 fx[2][TT], fd0[LEAD];
-  Source next;
   auto frag_d = [&](int e, int buf) {
     const int sub = e / (TT * TERMS), j = e / TERMS % TT, q = e % TERMS;
     return frag(sm[buf] + q * TILE + sub * 32 * B * 2, wo * TT + j);
   };
+  auto frag_s = [&](int j, int f, int buf) { return frag(sm[buf] + f % TERMS * TILE + f / TERMS * 32 * B * 2, wo * TT + j); };
   auto frag_x = [&](int i, int sub, int buf) { return frag(sm[buf] + TERMS * TILE + sub * 32 * B * 2, wi * TT + i); };
-  auto step = [&](int k, int buf, int set) {      // set: which half of fx holds the step's first part
-    i32x4 fd[GROUPS];
+  auto step = [&](int buf, int set) {      // set: which half of fx holds the step's first part
+    i32x4 fd[GROUPS], fs[S * TERMS];
 #pragma unroll
     for (int e = 0; e < LEAD; ++e) fd[e] = fd0[e];
 #pragma unroll
     for (int e = 0; e < GROUPS; ++e) {
       const int sub = e / (TT * TERMS), j = e / TERMS % TT, hold = S == 2 ? sub : set;
+      if (e == TURN - 2) {
+#pragma unroll
+        for (int f = 0; f < S * TERMS; ++f) fs[f] = frag_s(mine < TT ? mine : 0, f, buf);
+      }
       if (e + LEAD < TURN) fd[e + LEAD] = frag_d(e + LEAD, buf);
       if (e == TURN - LEAD) {
 #pragma unroll
@@ -523,8 +541,19 @@ __global__ __launch_bounds__(256) void block8_wgrad_kernel(
       }
       if (S == 2 && e < TT) fx[1][e] = frag_x(e, 1, buf);
       if (e == TURN) {
+        if (mine < TT) {      // before the step's buffer is given up
+#pragma unroll
+          for (int f = 0; f < S * TERMS; ++f) add_columns(accb[0], ones, fs[f]);
+#pragma unroll
+          for (int n = 1; n < OWN; ++n) {
+            if (mine + n * 2 * tiles_i < TT) {
+#pragma unroll
+              for (int f = 0; f < S * TERMS; ++f) add_columns(accb[n], ones, frag_s(mine + n * 2 * tiles_i, f, buf));
+            }
+          }
+          mfma_settle();
+        }
         __syncthreads();
-        next = source(k + 3);
       }
       if (e >= TURN) {
 #pragma unroll
@@ -532,31 +561,32 @@ __global__ __launch_bounds__(256) void block8_wgrad_kernel(
         if (e >= GROUPS - LEAD) fd0[e - (GROUPS - LEAD)] = frag_d(e - (GROUPS - LEAD), buf ^ 1);
       }
       __builtin_amdgcn_sched_barrier(0);
-      mfma_ready();
+      if (B == 256) mfma_ready();
 #pragma unroll
       for (int i = 0; i < TT; ++i) {
-        mfma_bf16(acc[i][j], fx[hold][i], fd[e]);
+        mul_bf16<B == 256>(acc[i][j], fx[hold][i], fd[e]);
         // from turn to turn: the parts of the next step but one, evenly
         const int slot = (e < TURN ? e + TAIL : e - TURN) * TT + i;
 #pragma unroll
-        for (int id = slot * PARTS / SLOTS; id < (slot + 1) * PARTS / SLOTS; ++id) part(id, e < TURN ? buf ^ 1 : buf, next);
+        for (int id = slot * PARTS / SLOTS; id < (slot + 1) * PARTS / SLOTS; ++id) {
+          if (id == 0) advance();
+          part(id, e < TURN ? buf ^ 1 : buf);
+        }
         __builtin_amdgcn_sched_barrier(0);
       }
-      if (sums & (1u << j)) mfma_bf16_now(accb[j], ones, fd[e]);
     }
   };
 
-  next = source(0);
 #pragma unroll
-  for (int i = 0; i < DL; ++i) load_dy(next, i);
+  for (int i = 0; i < DL; ++i) load_dy(i);
 #pragma unroll
-  for (int i = 0; i < XL; ++i) load_x(next, i);
-  next = source(1);
+  for (int i = 0; i < XL; ++i) load_x(i);
+  advance();
 #pragma unroll
-  for (int id = 0; id < PARTS; ++id) part(id, 0, next);
-  next = source(2);
+  for (int id = 0; id < PARTS; ++id) part(id, 0);
+  advance();
 #pragma unroll
-  for (int id = 0; id < TAIL * TT * PARTS / SLOTS; ++id) part(id, 1, next);
+  for (int id = 0; id < TAIL * TT * PARTS / SLOTS; ++id) part(id, 1);
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < TT; ++i) fx[0][i] = frag_x(i, 0, 0);
@@ -564,23 +594,24 @@ __global__ __launch_bounds__(256) void block8_wgrad_kernel(
   for (int e = 0; e < LEAD; ++e) fd0[e] = frag_d(e, 0);
   // two steps a turn of the loop, so that buffers and fragments have fixed places (a step behind the last one adds zeros)
   for (int k = 0; k < steps; k += 2) {
-    step(k, 0, 0);
-    step(k + 1, 1, 1);
+    step(0, 0);
+    step(1, 1);
   }
   __syncthreads();
-  mfma_settle();
+  if constexpr (B == 256) {
+    mfma_settle();
 #pragma unroll
-  for (int i = 0; i < TT; ++i) {
+    for (int i = 0; i < TT; ++i)
 #pragma unroll
-    for (int j = 0; j < TT; ++j) asm volatile("" : "+a"(acc[i][j]));
+      for (int j = 0; j < TT; ++j) asm volatile("" : "+a"(acc[i][j]));
   }
 
   if (g == 0) {
     float* to_db = db + blockIdx.y * bslab + (long long)m * O;
 #pragma unroll
-    for (int j = 0; j < TT; ++j) {
-      const int o = o0 + (wo * TT + j) * 16 + l16;
-      if ((sums & (1u << j)) && o < O) to_db[o] = beta * accb[j][0];
+    for (int n = 0; n < OWN; ++n) {
+      const int t = mine + n * 2 * tiles_i, o = o0 + (wo * TT + t) * 16 + l16;
+      if (t < TT && o < O) to_db[o] = beta * accb[n][0];
     }
   }
   const Piece<float> none[TT] = {};
