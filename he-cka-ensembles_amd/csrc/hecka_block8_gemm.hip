@@ -39,16 +39,16 @@ __device__ __forceinline__ i32x4 buffer_of(const void* p) {      // raw buffer o
   return i32x4{__builtin_amdgcn_readfirstlane((int)(unsigned)a), __builtin_amdgcn_readfirstlane((int)((a >> 32) & 0xffff)), 0x7fffffff, 0x00020000};
 }
 
-// Workgroup id -> tile.  Ids go round the eight XCDs; each XCD gets a contiguous run of tiles, walked in bands of up to eight
-// row tiles, so that the operands which the tiles in flight on one XCD share stay in that XCD's L2.
+// Workgroup id -> tile.  Ids go round the eight XCDs; each XCD gets a contiguous run of tiles, walked in bands of up to four
+// row tiles (eight or sixteen: 4 to 9 % slower), so that the operands which the tiles in flight on one XCD share stay in that XCD's L2.
 __device__ __forceinline__ void place(int id, int total, int tn, int to, int& m, int& in, int& io) {
   const int q = total >> 3, r = total & 7, xcd = id & 7, at = id >> 3;
   int t = xcd < r ? xcd * (q + 1) + at : r * (q + 1) + (xcd - r) * q + at;
   const int per = tn * to;
   m = t / per;
   t -= m * per;
-  const int band = t / (8 * to), first = band * 8, rows = tn - first < 8 ? tn - first : 8;
-  t -= band * 8 * to;
+  const int band = t / (4 * to), first = band * 4, rows = tn - first < 4 ? tn - first : 4;
+  t -= band * 4 * to;
   in = first + t % rows;
   io = t / rows;
 }
@@ -403,7 +403,10 @@ __global__ __launch_bounds__(256) void block8_wgrad_kernel(
     int tiles_o, int tiles_i, int rows_per, long long slab, long long bslab) {
   constexpr int KS = TERMS == 1 ? 64 : 32, S = KS / 32, TT = B / 32;      // rows a step, 32-row parts of it, tiles a wave and side
   constexpr int TILE = KS * B * 2, STAGE = (TERMS + 1) * TILE;
-  __shared__ __attribute__((aligned(1024))) unsigned char sm[2][STAGE];
+  // both buffers of dy, then both of x: whichever buffer, an LDS instruction's 16-bit offset reaches it from one address register
+  __shared__ __attribute__((aligned(1024))) unsigned char sm[2 * STAGE];
+  auto dy_tile = [&](int buf, int q) { return sm + (buf * TERMS + q) * TILE; };
+  auto x_tile = [&](int buf) { return sm + (2 * TERMS + buf) * TILE; };
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wi = wave & 1, wo = wave >> 1, l16 = lane & 15, g = lane >> 4;
   int m, to, ti;
@@ -416,42 +419,59 @@ __global__ __launch_bounds__(256) void block8_wgrad_kernel(
   xs += m * xsstride + (long long)first * sstride;
 
   // Staging: a thread's share of a step are DL items of dy (16-byte pieces) and XL items of x (sixteen codes).  The registers hold
-  // the step behind the one that is being written to LDS.  WHOLE (dy's rows are whole aligned pieces): buffer loads, zero behind
+  // two steps: while one is written to LDS the next is in, and the one after it takes the place of what was written.  WHOLE (dy's rows are whole aligned pieces): buffer loads, zero behind
   // the last row; columns behind the end are the next row's - they only reach outputs that do not exist.
   constexpr int P = Piece<T>::N, DPR = B / P, DL = KS * DPR / 256, XPR = B / 16, XL = KS * XPR / 256;
   constexpr int DROWS = 256 / DPR, XROWS = 256 / XPR;      // rows from one item to the next
-  Piece<T> rd[DL];
-  i32x4 rx[XL];
-  int rs[XL];
+  Piece<T> rd[2][DL];
+  i32x4 rx[2][XL];
+  int rs[2][XL];
   float r[4];
   const int dn = tid / DPR, dc = (tid % DPR) * P, xn = tid / XPR, xc = (tid % XPR) * 16;
   const int dv = (dn * O + dc) * (int)sizeof(T), xv = xn * (int)Kp + xc, sv = xn * sstride + ((i0 + xc) >> 7);
-  // where the loads' step begins, and what is left of each operand from there on; one step further with a few scalar instructions
-  struct Source { const T* dy; const unsigned char *x, *xs; long long dy_bytes, x_bytes; int left; };
-  const long long dy_step = (long long)KS * O, x_step = KS * Kp;
-  Source at = {dy + o0, x + i0, xs, ((long long)(last - first) * O - o0) * (long long)sizeof(T), (last - first) * Kp - i0, last - first};
+  // Where the loads' step begins, and the bytes that each operand has from there on (what of them a buffer descriptor can say).
+  // Worked out once a step and by halves of 32 bits, for which there are scalar instructions: 64-bit comparisons go through the
+  // vector unit, and a descriptor made at every load cost a fifth of the time.
+  struct Source { const T* dy; const unsigned char *x, *xs; long long dy_left, x_left; int left, dy_bytes, x_bytes, xs_bytes; };
+  const long long dy_step = (long long)KS * O * (int)sizeof(T), x_step = KS * Kp;
+  Source at;
+  auto said = [](long long bytes) {
+    const int hi = (int)(bytes >> 32), lo = (int)bytes;
+    return __builtin_amdgcn_readfirstlane(hi < 0 ? 0 : hi > 0 || lo < 0 ? 0x7fffffff : lo);
+  };
+  auto say = [&]() {
+    at.dy_bytes = said(at.dy_left);
+    at.x_bytes = said(at.x_left);
+    at.xs_bytes = said(at.left * (long long)sstride);
+  };
   auto advance = [&]() {
-    at.dy += dy_step;
+    at.dy += KS * (long long)O;
     at.x += x_step;
     at.xs += KS * sstride;
-    at.dy_bytes -= dy_step * (long long)sizeof(T);
-    at.x_bytes -= x_step;
+    at.dy_left -= dy_step;
+    at.x_left -= x_step;
     at.left -= KS;
+    say();
   };
-  auto buffer = [](const void* p, long long bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes < 0 ? 0 : bytes > 0x7fffffff ? 0x7fffffff : (int)bytes, 0x00020000);
-  };
-  auto load_dy = [&](int item) {
+  at.dy = dy + o0;
+  at.x = x + i0;
+  at.xs = xs;
+  at.left = last - first;
+  at.dy_left = ((long long)at.left * O - o0) * (long long)sizeof(T);
+  at.x_left = at.left * Kp - i0;
+  say();
+  auto buffer = [](const void* p, int bytes) { return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00020000); };
+  auto load_dy = [&](int set, int item) {
     if constexpr (WHOLE) {
-      rd[item] = __builtin_bit_cast(Piece<T>, __builtin_amdgcn_raw_buffer_load_b128(buffer(at.dy, at.dy_bytes), dv + item * DROWS * O * (int)sizeof(T), 0, 0));
+      rd[set][item] = __builtin_bit_cast(Piece<T>, __builtin_amdgcn_raw_buffer_load_b128(buffer(at.dy, at.dy_bytes), dv + item * DROWS * O * (int)sizeof(T), 0, 0));
     } else {
       const int n = dn + item * DROWS;
-      rd[item] = load_piece(n < at.left ? at.dy - o0 + (long long)n * O : dy, n < at.left ? o0 + dc : O, O);
+      rd[set][item] = load_piece(n < at.left ? at.dy - o0 + (long long)n * O : dy, n < at.left ? o0 + dc : O, O);
     }
   };
-  auto load_x = [&](int item) {
-    rx[item] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(buffer(at.x, at.x_bytes), xv + item * XROWS * (int)Kp, 0, 0));
-    rs[item] = __builtin_amdgcn_raw_buffer_load_b8(buffer(at.xs, at.left < 0 ? 0 : (long long)at.left * sstride), sv + item * XROWS * sstride, 0, 0);
+  auto load_x = [&](int set, int item) {
+    rx[set][item] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(buffer(at.x, at.x_bytes), xv + item * XROWS * (int)Kp, 0, 0));
+    rs[set][item] = __builtin_amdgcn_raw_buffer_load_b8(buffer(at.xs, at.xs_bytes), sv + item * XROWS * sstride, 0, 0);
   };
   // the work on one item in parts of three to six instructions, few enough to pass in the shadow of a product
   constexpr int QUADS = P / 4, PERQ = TERMS == 1 ? 1 : (sizeof(T) == 2 ? 1 : 0) + 3 * (TERMS - 1) + 1;
@@ -459,16 +479,16 @@ __global__ __launch_bounds__(256) void block8_wgrad_kernel(
   auto part = [&](int id, int buf) {
     if (id < DL * PERD) {
       const int item = id / PERD, n = dn + item * DROWS;
-      unsigned char* to = sm[buf] + n * B * 2 + (((dc >> 4) ^ (n & 7)) * 32) + (dc & 15) * 2;
+      unsigned char* to = dy_tile(buf, 0) + n * B * 2 + (((dc >> 4) ^ (n & 7)) * 32) + (dc & 15) * 2;
       if constexpr (TERMS == 1) {
-        *reinterpret_cast<Piece<T>*>(to) = rd[item];
+        *reinterpret_cast<Piece<T>*>(to) = rd[buf][item];
       } else {
         const int quad = id % PERD / PERQ;
         int what = id % PERQ;
         if constexpr (sizeof(T) == 2) --what;
         if (what == -1 || (sizeof(T) == 4 && what == 0)) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) r[e] = widen(rd[item].e[quad * 4 + e]);
+          for (int e = 0; e < 4; ++e) r[e] = widen(rd[buf][item].e[quad * 4 + e]);
         }
         if (what >= 0 && what % 3 == 0) {      // the next term of all four
           const uint2 c = make_uint2(__builtin_amdgcn_perm(__float_as_uint(r[1]), __float_as_uint(r[0]), 0x07060302),
@@ -479,12 +499,12 @@ __global__ __launch_bounds__(256) void block8_wgrad_kernel(
           for (int e = what % 3 * 2 - 2; e < what % 3 * 2; ++e) r[e] -= __uint_as_float(__float_as_uint(r[e]) & 0xffff0000u);
         }
       }
-      if (id % PERD == PERD - 1) load_dy(item);
+      if (id % PERD == PERD - 1) load_dy(buf, item);
     } else {
       const int j = (id - DL * PERD) / 2, h = (id - DL * PERD) % 2, n = xn + j * XROWS;
-      bf16x8* to = reinterpret_cast<bf16x8*>(sm[buf] + TERMS * TILE + n * B * 2 + (((xc >> 4) ^ (n & 7)) * 32));
-      to[h] = widen8(rx[j][2 * h], rx[j][2 * h + 1], scale_of(rs[j]));
-      if (h == 1) load_x(j);
+      bf16x8* to = reinterpret_cast<bf16x8*>(x_tile(buf) + n * B * 2 + (((xc >> 4) ^ (n & 7)) * 32));
+      to[h] = widen8(rx[buf][j][2 * h], rx[buf][j][2 * h + 1], scale_of(rs[buf][j]));
+      if (h == 1) load_x(buf, j);
     }
   };
 
@@ -519,10 +539,10 @@ __global__ __launch_bounds__(256) void block8_wgrad_kernel(
   i32x4 fx[2][TT], fd0[LEAD];
   auto frag_d = [&](int e, int buf) {
     const int sub = e / (TT * TERMS), j = e / TERMS % TT, q = e % TERMS;
-    return frag(sm[buf] + q * TILE + sub * 32 * B * 2, wo * TT + j);
+    return frag(dy_tile(buf, q) + sub * 32 * B * 2, wo * TT + j);
   };
-  auto frag_s = [&](int j, int f, int buf) { return frag(sm[buf] + f % TERMS * TILE + f / TERMS * 32 * B * 2, wo * TT + j); };
-  auto frag_x = [&](int i, int sub, int buf) { return frag(sm[buf] + TERMS * TILE + sub * 32 * B * 2, wi * TT + i); };
+  auto frag_s = [&](int j, int f, int buf) { return frag(dy_tile(buf, f % TERMS) + f / TERMS * 32 * B * 2, wo * TT + j); };
+  auto frag_x = [&](int i, int sub, int buf) { return frag(x_tile(buf) + sub * 32 * B * 2, wi * TT + i); };
   auto step = [&](int buf, int set) {      // set: which half of fx holds the step's first part
     i32x4 fd[GROUPS], fs[S * TERMS];
 #pragma unroll
@@ -578,10 +598,13 @@ __global__ __launch_bounds__(256) void block8_wgrad_kernel(
   };
 
 #pragma unroll
-  for (int i = 0; i < DL; ++i) load_dy(i);
+  for (int set = 0; set < 2; ++set) {
 #pragma unroll
-  for (int i = 0; i < XL; ++i) load_x(i);
-  advance();
+    for (int i = 0; i < DL; ++i) load_dy(set, i);
+#pragma unroll
+    for (int i = 0; i < XL; ++i) load_x(set, i);
+    advance();
+  }
 #pragma unroll
   for (int id = 0; id < PARTS; ++id) part(id, 0);
   advance();
@@ -616,7 +639,7 @@ __global__ __launch_bounds__(256) void block8_wgrad_kernel(
   }
   const Piece<float> none[TT] = {};
   const int o1 = o0 + wo * (B / 2), i1 = i0 + wi * (B / 2);
-  store_tile<float, TT, STAGE / 2>(acc, none, alpha, 0.f, &sm[0][0] + wave * (STAGE / 2), dW + blockIdx.y * slab + ((long long)m * O + o1) * I + i1,
+  store_tile<float, TT, STAGE / 2>(acc, none, alpha, 0.f, sm + wave * (STAGE / 2), dW + blockIdx.y * slab + ((long long)m * O + o1) * I + i1,
                                    I, O - o1, I - i1);
 }
 
