@@ -135,7 +135,7 @@ __device__ __forceinline__ void mfma_settle() { asm volatile("s_nop 15\n\ts_nop 
 template <class T, bool EXACT, int B>
 __global__ __launch_bounds__(256) void block8_linear_kernel(
     const unsigned char* __restrict__ x, const unsigned char* __restrict__ xs, long long xstride, long long xsstride,
-    const unsigned char* __restrict__ w, const unsigned char* __restrict__ ws, int N, int O, int nblk,
+    const unsigned char* __restrict__ w, const unsigned char* __restrict__ ws, int N, int O, int allblk, int share,
     const float* __restrict__ bias, long long bstride, float alpha, float beta, T* __restrict__ y, int tiles_n, int tiles_o) {
   constexpr int TO = B / 32, TN = B / 32, U = EXACT ? 2 : 1, SYNC = TO / 2, L = B / 32, STAGE = 2 * B * kBlock;
   __shared__ __attribute__((aligned(1024))) unsigned char sm[2][STAGE];
@@ -144,12 +144,15 @@ __global__ __launch_bounds__(256) void block8_linear_kernel(
   const int wo = wave & 1, wn = wave >> 1, l16 = lane & 15, g = lane >> 4;
   int m, tn, to;
   place(blockIdx.x, gridDim.x, tiles_n, tiles_o, m, tn, to);
-  const int n0 = tn * B, o0 = to * B, sstride = (nblk + 3) & ~3;
-  const long long K = (long long)nblk * kBlock;
-  x += m * xstride;
-  xs += m * xsstride;
-  w += (long long)m * O * K;
-  ws += (long long)m * ((O + kBlock - 1) / kBlock) * sstride;
+  const int n0 = tn * B, o0 = to * B, sstride = (allblk + 3) & ~3;
+  const long long K = (long long)allblk * kBlock;
+  // the blocks of K of this workgroup: share of them (a multiple of four: whole dwords of scales) from blockIdx.y * share on, its sums
+  // to slab blockIdx.y
+  const int first = blockIdx.y * share, nblk = allblk - first < share ? allblk - first : share;
+  x += m * xstride + (long long)first * kBlock;
+  xs += m * xsstride + first;
+  w += (long long)m * O * K + (long long)first * kBlock;
+  ws += (long long)m * ((O + kBlock - 1) / kBlock) * sstride + first;
 
   // what this lane loads: row (4 i + wave) 8 + lane / 8 of each operand's tile, rows behind the end repeat the last one;
   // offsets from the tile's first row stay below 2^30 (256 rows of at most 2^22), the step is the loads' scalar offset
@@ -304,7 +307,39 @@ __global__ __launch_bounds__(256) void block8_linear_kernel(
   }
   __syncthreads();
   const int n1 = n0 + wn * (B / 2), o1 = o0 + wo * (B / 2);
-  store_tile<T, TO, STAGE / 2>(acc, bv, alpha, beta, &sm[0][0] + wave * (STAGE / 2), y + ((long long)m * N + n1) * O + o1, O, N - n1, O - o1);
+  store_tile<T, TO, STAGE / 2>(acc, bv, alpha, beta, &sm[0][0] + wave * (STAGE / 2), y + (((long long)blockIdx.y * (gridDim.x / (tiles_n * tiles_o)) + m) * N + n1) * O + o1, O, N - n1, O - o1);
+}
+
+// y[m][e] = sum over S slabs part[s][m][e], in order, + beta bias[m][e mod O]; e < n = N O.  sum: one m whose slabs are all the members'.
+template <class T>
+__global__ __launch_bounds__(256) void block8_join_kernel(const float* __restrict__ part, int S, long long n, int O,
+                                                          const float* __restrict__ bias, long long bstride, float beta, T* __restrict__ y) {
+  const long long m = blockIdx.y, step = n * gridDim.y;
+  part += m * n;
+  y += m * n;
+  for (long long e = ((long long)blockIdx.x * 256 + threadIdx.x) * 4; e < n; e += (long long)gridDim.x * 1024) {
+    const int left = (int)(n - e < 4 ? n - e : 4);
+    Piece<float> s = load_piece(part + e, 0, left);
+    for (int i = 1; i < S; ++i) {
+      const Piece<float> v = load_piece(part + i * step + e, 0, left);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s.e[k] += v.e[k];
+    }
+    int o = bias ? (int)(e % O) : 0;
+    struct { T e[4]; } out;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      narrow(bias ? fmaf(beta, bias[m * bstride + o], s.e[k]) : s.e[k], out.e[k]);
+      if (++o == O) o = 0;
+    }
+    if (left == 4) {
+      __builtin_memcpy(y + e, &out, sizeof(out));
+    } else {
+#pragma unroll
+      for (int k = 0; k < 3; ++k)
+        if (k < left) y[e + k] = out.e[k];
+    }
+  }
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -643,26 +678,61 @@ __global__ __launch_bounds__(256) void block8_wgrad_kernel(
                                    I, O - o1, I - i1);
 }
 
-// out[e] = sum over S slabs, in order
-__global__ __launch_bounds__(256) void block8_slabs_kernel(const float* __restrict__ part, int S, long long n, float* __restrict__ out) {
-  for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < n; e += (long long)gridDim.x * 256) {
-    float s = part[e];
-    for (int i = 1; i < S; ++i) s += part[i * n + e];
-    out[e] = s;
+// out[e] = sum over S slabs, in order; two arrays in one launch: n of out, then n2 of out2, whose slabs stand behind out's
+__global__ __launch_bounds__(256) void block8_slabs_kernel(const float* __restrict__ part, int S, long long n, float* __restrict__ out,
+                                                           long long n2, float* __restrict__ out2) {
+  for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < n + n2; e += (long long)gridDim.x * 256) {
+    const bool second = e >= n;
+    const float* p = second ? part + S * n + (e - n) : part + e;
+    const long long step = second ? n2 : n;
+    float s = p[0];
+    for (int i = 1; i < S; ++i) s += p[i * step];
+    (second ? out2[e - n] : out[e]) = s;
   }
 }
 
 static int cdiv(int a, int b) { return (a + b - 1) / b; }
+static constexpr int kLinearFill = 256, kLinearLeast = 8;
+
+// 256 x 256 outputs a workgroup where that fills three quarters of the chip, else 128 x 128, and where those leave half of it idle the
+// blocks of K are shared out, eight at least to each, their sums joined by a second launch.  Measured (bf16 / fp32 results):
+// 1 x 64 x 8192 x 8192 48 / 73 us whole, 24 / 30 us in four shares, 31 / 30 us in eight; 1 x 64 x 1024 x 8192 41 / 73 us whole, 15 /
+// 19 us in eight; 1 x 512 x 4096 x 4096 28 / 45 us whole, 27 / 35 us in two, 38 / 35 us in four; shares of four blocks: 1 x 256 x 4096 x
+// 4096 32 us against 22.
+struct LinearPlan { int tile, splits, share; };
+static LinearPlan linear_plan(int M, int N, int O, int nblk) {
+  LinearPlan p{256, 1, (nblk + 3) & ~3};
+  if ((long long)M * cdiv(N, 256) * cdiv(O, 256) >= 192) return p;
+  p.tile = 128;
+  const long long tiles = (long long)M * cdiv(N, 128) * cdiv(O, 128), s = kLinearFill / tiles;
+  if (s > 1) {
+    const int most = nblk / kLinearLeast > 1 ? nblk / kLinearLeast : 1;
+    p.splits = (int)(s < most ? s : most);
+    p.share = (cdiv(nblk, p.splits) + 3) & ~3;
+    p.splits = cdiv(nblk, p.share);
+  }
+  return p;
+}
+static size_t linear_workspace(const LinearPlan& p, int M, int N, int O, int y_members) {
+  return p.splits > 1 || y_members < M ? (size_t)p.splits * M * N * O * sizeof(float) : 0;
+}
 
 template <class T, bool EXACT>
-static int linear_run(const void* x, const void* xs, long long xstride, long long xsstride, const void* w, const void* ws, int M,
-                      int N, int O, int nblk, const float* bias, long long bstride, float alpha, float beta, void* y, hipStream_t st) {
-#define HECKA_LINEAR(B) \
-  block8_linear_kernel<T, EXACT, B><<<dim3((unsigned)(M * cdiv(N, B) * cdiv(O, B))), 256, 0, st>>>( \
+static int linear_run(const LinearPlan& p, const void* x, const void* xs, long long xstride, long long xsstride, const void* w,
+                      const void* ws, int M, int N, int O, int nblk, const float* bias, long long bstride, float alpha, float beta,
+                      void* y, int y_members, float* slabs, hipStream_t st) {
+#define HECKA_LINEAR(TO, B, BIAS, OUT) \
+  block8_linear_kernel<TO, EXACT, B><<<dim3((unsigned)(M * cdiv(N, B) * cdiv(O, B)), p.splits), 256, 0, st>>>( \
       (const unsigned char*)x, (const unsigned char*)xs, xstride, xsstride, (const unsigned char*)w, (const unsigned char*)ws, N, O, \
-      nblk, bias, bstride, alpha, beta, (T*)y, cdiv(N, B), cdiv(O, B))
-  if ((long long)M * cdiv(N, 256) * cdiv(O, 256) >= 192) HECKA_LINEAR(256);
-  else HECKA_LINEAR(128);
+      nblk, p.share, BIAS, bstride, alpha, beta, OUT, cdiv(N, B), cdiv(O, B))
+  if (p.splits > 1 || y_members < M) {
+    if (p.tile == 256) HECKA_LINEAR(float, 256, nullptr, slabs);
+    else HECKA_LINEAR(float, 128, nullptr, slabs);
+    const long long n = (long long)N * O, blocks = (n + 1023) / 1024;
+    block8_join_kernel<T><<<dim3((unsigned)(blocks < 2048 ? blocks : 2048), y_members), 256, 0, st>>>(
+        slabs, y_members < M ? p.splits * M : p.splits, n, O, bias, bstride, beta, (T*)y);
+  } else if (p.tile == 256) HECKA_LINEAR(T, 256, bias, (T*)y);
+  else HECKA_LINEAR(T, 128, bias, (T*)y);
 #undef HECKA_LINEAR
   return check_launch("block8_linear");
 }
@@ -732,8 +802,8 @@ static int wgrad_run(const void* dy, const void* x, const void* xs, long long xs
   else HECKA_WGRAD(128, false);
 #undef HECKA_WGRAD
   if (cut) {
-    block8_slabs_kernel<<<dim3((unsigned)((nw + 255) / 256 < 2048 ? (nw + 255) / 256 : 2048)), 256, 0, st>>>(ws, p.splits, nw, dW);
-    if (db) block8_slabs_kernel<<<dim3((unsigned)((nb + 255) / 256 < 2048 ? (nb + 255) / 256 : 2048)), 256, 0, st>>>(ws + p.splits * nw, p.splits, nb, db);
+    const long long n2 = db ? nb : 0, blocks = (nw + n2 + 255) / 256;
+    block8_slabs_kernel<<<dim3((unsigned)(blocks < 2048 ? blocks : 2048)), 256, 0, st>>>(ws, p.splits, nw, dW, n2, db);
   }
   return check_launch("block8_wgrad");
 }
@@ -752,21 +822,32 @@ using namespace hecka;
 
 extern "C" {
 
+size_t hecka_block8_linear_workspace_bytes(int M, int N, int O, int I, int y_members) {
+  if (bad_sizes(M, N, O, I) || (y_members != M && y_members != 1)) return 0;
+  return linear_workspace(linear_plan(M, N, O, row_blocks(I)), M, N, O, y_members);
+}
+
 int hecka_block8_linear(const void* x, const void* xscales, int x_members, const void* w, const void* wscales, int M, int N, int O,
-                        int I, const float* bias, long long bstride, float alpha, float beta, void* y, int dtype, void* stream) {
+                        int I, const float* bias, long long bstride, float alpha, float beta, void* y, int dtype, int y_members,
+                        void* ws, size_t ws_bytes, void* stream) {
   if (bad_type(dtype)) return fail(HECKA_EINVAL, "block8_linear: unknown dtype%s");
   if (bad_sizes(M, N, O, I)) return fail(HECKA_EINVAL, "%sblock8_linear: bad size (N = %lld, O = %lld)", "", N, O);
   if (x_members != M && x_members != 1) return fail(HECKA_EINVAL, "%sblock8_linear: codes of %lld members for %lld", "", x_members, M);
+  if (y_members != M && (y_members != 1 || bias)) return fail(HECKA_EINVAL, "%sblock8_linear: %lld result members for %lld (their sum takes no bias)", "", y_members, M);
   if (!x || !xscales || !w || !wscales || !y) return fail(HECKA_EINVAL, "block8_linear: null pointer%s");
   if (!aligned16(x) || !aligned16(w) || (reinterpret_cast<uintptr_t>(xscales) & 3) || (reinterpret_cast<uintptr_t>(wscales) & 3))
     return fail(HECKA_EINVAL, "block8_linear: codes need 16-byte alignment, scales 4-byte%s");
-  clear_error();
   const int nblk = row_blocks(I);
+  const LinearPlan p = linear_plan(M, N, O, nblk);
+  if ((ws ? ws_bytes : 0) < linear_workspace(p, M, N, O, y_members))
+    return fail(HECKA_EWORKSPACE, "%sblock8_linear: workspace too small (%lld bytes given)", "", (long long)ws_bytes);
+  clear_error();
   const long long xst = x_members == 1 ? 0 : (long long)N * nblk * kBlock, sst = x_members == 1 ? 0 : (long long)N * scale_stride(I);
   hipStream_t st = (hipStream_t)stream;
-  return dtype == HECKA_DT_F32 ? linear_run<float, true>(x, xscales, xst, sst, w, wscales, M, N, O, nblk, bias, bstride, alpha, beta, y, st)
-         : dtype == HECKA_DT_BF16 ? linear_run<Bf16, false>(x, xscales, xst, sst, w, wscales, M, N, O, nblk, bias, bstride, alpha, beta, y, st)
-                                  : linear_run<F16, false>(x, xscales, xst, sst, w, wscales, M, N, O, nblk, bias, bstride, alpha, beta, y, st);
+#define HECKA_RUN(T, EXACT) \
+  linear_run<T, EXACT>(p, x, xscales, xst, sst, w, wscales, M, N, O, nblk, bias, bstride, alpha, beta, y, y_members, (float*)ws, st)
+  return dtype == HECKA_DT_F32 ? HECKA_RUN(float, true) : dtype == HECKA_DT_BF16 ? HECKA_RUN(Bf16, false) : HECKA_RUN(F16, false);
+#undef HECKA_RUN
 }
 
 int hecka_block8_linear_token(const void* x, int dtype, int x_members, const void* w, const void* wscales, int M, int N, int O, int I,

@@ -197,13 +197,17 @@ def _bias_rows(b):
     return b if b is None or b.stride(1) == 1 else b.contiguous()
 
 
-def _product(q, codes, scales, M, O, I, bias, alpha, beta, dtype):
-    xm = 1 if len(q.shape) == 2 else M
+def _product(q, codes, scales, M, O, I, bias, alpha, beta, dtype, total=False):
+    """[M, N, O]; total: its sum over the members [N, O] (no bias), added in fp32 and rounded once."""
     N = q.shape[-2]
-    y = torch.empty((M, N, O), device=q.device, dtype=dtype)
+    y = torch.empty((N, O) if total else (M, N, O), device=q.device, dtype=dtype)
     if y.numel():
-        _lib.call('hecka_block8_linear', q.device, q.codes.data_ptr(), q.scales.data_ptr(), xm, codes.data_ptr(), scales.data_ptr(),
-                  M, N, O, I, _ptr(bias), _bstride(bias), alpha, beta, y.data_ptr(), DTYPES[dtype])
+        ym = 1 if total else M
+        nbytes = _lib.lib().hecka_block8_linear_workspace_bytes(M, N, O, I, ym)
+        ws = torch.empty((nbytes // 4,), device=q.device, dtype=torch.float32) if nbytes else None
+        _lib.call('hecka_block8_linear', q.device, q.codes.data_ptr(), q.scales.data_ptr(), 1 if len(q.shape) == 2 else M,
+                  codes.data_ptr(), scales.data_ptr(), M, N, O, I, _ptr(bias), _bstride(bias), alpha, beta, y.data_ptr(), DTYPES[dtype],
+                  ym, _ptr(ws), nbytes)
     return y
 
 
@@ -267,17 +271,16 @@ class _Linear8(torch.autograd.Function):
         dx = dW = db = None
         want_b = has_bias and ctx.needs_input_grad[2]
         if ctx.needs_input_grad[0]:
-            shared = len(xshape) == 2
-            # members' shares of a shared input are added in fp32 and rounded once
-            part = torch.float32 if shared else xdtype
-            dx = _product(_quantize(dy)[0], codes_t, scales_t, M, I, O, None, scale, 0.0, part)
-            if shared:
-                dx = dx.sum(0).to(xdtype)
+            dx = _product(_quantize(dy)[0], codes_t, scales_t, M, I, O, None, scale, 0.0, xdtype, total=len(xshape) == 2)
         if ctx.needs_input_grad[1]:
             dW, db = _weight_grad(dy, Rows8(codes, scales, xshape, xdtype), scale, bias_scale, want_b)
             dW = dW.to(wdtype)
         elif want_b:
-            db = bias_scale * dy.sum(1, dtype=torch.float32)
+            # the column sums alone: the weight gradient of rows of one zero
+            N = dy.shape[1]
+            one = Rows8(torch.zeros((N, BLOCK), device=dy.device, dtype=torch.uint8),
+                        torch.zeros((N, scale_stride(1)), device=dy.device, dtype=torch.uint8), (N, 1), xdtype)
+            db = _weight_grad(dy, one, 0.0, bias_scale)[1]
         return dx, dW, db, None, None
 
 

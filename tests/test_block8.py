@@ -315,6 +315,46 @@ def test_shared_rows_and_their_gradient():
 
 
 @gpu
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
+@pytest.mark.parametrize('M,N,O,I', [(1, 64, 130, 5000), (2, 33, 71, 2100), (1, 17, 3, 8200), (1, 300, 8, 2048)])
+def test_long_sums_shared_out(M, N, O, I, dtype):
+    """Few tiles and many blocks of K: the slabs' sum, its bias and rounding, and the same bits on every call."""
+    from hyper_amd import _lib, block8
+    assert _lib.lib().hecka_block8_linear_workspace_bytes(M, N, O, I, M) > 0
+    x, W, b = whole((M, N, I), 1), whole((M, O, I), 2), whole((M, O), 3, 50)
+    q, w = block8.quantize(x.to(dtype).cuda()), block8.quantize_weight(W.cuda())
+    for bias in (None, b):
+        y = block8.linear(q, w, None if bias is None else bias.cuda(), scale=0.25, bias_scale=2.0)
+        want = 0.25 * torch.bmm(x.double(), W.double().transpose(1, 2).contiguous()) + (0.0 if bias is None else 2.0 * bias.double()[:, None])
+        assert torch.equal(y.cpu(), want.to(dtype))
+    x = features((M, N, I), dtype, 5).cuda()
+    assert torch.equal(block8.linear(block8.quantize(x), w), block8.linear(block8.quantize(x), w))
+
+
+@gpu
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
+@pytest.mark.parametrize('M,N,O,I', [(3, 40, 50, 201), (2, 33, 4099, 35), (7, 1, 1, 1), (40, 700, 300, 129)])
+def test_gradient_of_shared_rows_is_rounded_once(M, N, O, I, dtype):
+    """The members' sum in fp32, also where the sum over outputs is long and shared out, or the tiles are large."""
+    from hyper_amd import block8
+    x, W, dy = whole((N, I), 1), whole((M, O, I), 2), whole((M, N, O), 3)
+    xg = x.to(dtype).cuda().requires_grad_(True)
+    dx, = torch.autograd.grad(block8.linear(xg, W.cuda(), scale=0.5), xg, dy.to(dtype).cuda())
+    assert dx.dtype == dtype and torch.equal(dx.cpu(), (0.5 * torch.bmm(dy.double(), W.double()).sum(0)).to(dtype))
+
+
+@gpu
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
+def test_gradient_of_the_bias_alone(dtype):
+    from hyper_amd import block8
+    for M, N, O in ((2, 5, 7), (1, 5000, 33), (3, 130, 300)):
+        b, dy = whole((M, O), 1).cuda().requires_grad_(True), whole((M, N, O), 2).to(dtype)
+        y = block8.linear(torch.randn(M, N, 20, device='cuda', dtype=dtype), torch.randn(M, O, 20, device='cuda'), b, bias_scale=0.5)
+        db, = torch.autograd.grad(y, b, dy.cuda())
+        assert torch.equal(db.cpu().double(), 0.5 * dy.double().sum(1))
+
+
+@gpu
 def test_not_a_number_reaches_its_row_and_column_only():
     from hyper_amd import block8
     for dtype in TYPES:
@@ -456,9 +496,15 @@ def test_refusals_without_a_gpu():
     assert L.hecka_block8_weight(p, 0, 1, 8, 8, 64, p, p, p, None, None) == -1
     assert L.hecka_block8_weight(p, 0, 2, 8, 8, 63, p, p, None, None, None) == -1
     assert L.hecka_block8_weight(p, 0, 0, 8, 8, 64, p, p, None, None, None) == -1
-    assert L.hecka_block8_linear(p, p, 2, p, p, 3, 8, 8, 8, None, 0, 1.0, 0.0, p, 0, None) == -1
-    assert L.hecka_block8_linear(p, p, 1, p, p, 1, 8, 8, (1 << 22) + 1, None, 0, 1.0, 0.0, p, 0, None) == -1
-    assert L.hecka_block8_linear(odd, p, 1, p, p, 1, 8, 8, 8, None, 0, 1.0, 0.0, p, 0, None) == -1
+    assert L.hecka_block8_linear(p, p, 2, p, p, 3, 8, 8, 8, None, 0, 1.0, 0.0, p, 0, 3, None, 0, None) == -1
+    assert L.hecka_block8_linear(p, p, 1, p, p, 1, 8, 8, (1 << 22) + 1, None, 0, 1.0, 0.0, p, 0, 1, None, 0, None) == -1
+    assert L.hecka_block8_linear(odd, p, 1, p, p, 1, 8, 8, 8, None, 0, 1.0, 0.0, p, 0, 1, None, 0, None) == -1
+    assert L.hecka_block8_linear(p, p, 1, p, p, 3, 8, 8, 8, None, 0, 1.0, 0.0, p, 0, 2, None, 0, None) == -1      # a sum over some members
+    assert L.hecka_block8_linear(p, p, 1, p, p, 3, 8, 8, 8, p, 8, 1.0, 1.0, p, 0, 1, None, 0, None) == -1         # a sum with a bias
+    need = L.hecka_block8_linear_workspace_bytes(1, 64, 1024, 8192, 1)
+    assert need > 0 and need % (64 * 1024 * 4) == 0                                                               # slabs of a split K
+    assert L.hecka_block8_linear(p, p, 1, p, p, 1, 64, 1024, 8192, None, 0, 1.0, 0.0, p, 0, 1, p, need - 1, None) == -3
+    assert L.hecka_block8_linear_workspace_bytes(3, 8, 8, 8, 1) == 3 * 64 * 4 and L.hecka_block8_linear_workspace_bytes(3, 8, 8, 8, 3) == 0
     assert L.hecka_block8_linear_token(p, 0, 1, p, p, 1, 17, 8, 8, None, 0, 1.0, 0.0, p, None) == -1
     assert L.hecka_block8_wgrad(p, 0, p, p, 1, 1, 5000, 8, 8, 1.0, 1.0, p, p, None, 0, None) == -3
     assert L.hecka_block8_wgrad_workspace_bytes(1, 0, 8, 8) == 0
