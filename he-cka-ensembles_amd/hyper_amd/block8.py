@@ -41,6 +41,11 @@ def _check(t, what):
         raise TypeError('%s: float32, bfloat16 or float16, got %s' % (what, t.dtype))
 
 
+def _check_rows(q, what):
+    if not isinstance(q, Rows8):
+        raise TypeError('%s: expected Rows8, got %s' % (what, type(q).__name__))
+
+
 def _same_device(what, *ts):
     if any(t is not None and t.device != ts[0].device for t in ts):
         raise RuntimeError('%s: tensors on different devices (%s)' % (what, ', '.join(str(t.device) for t in ts if t is not None)))
@@ -55,7 +60,21 @@ class Rows8(object):
     shape and dtype of what was put in."""
 
     def __init__(self, codes, scales, shape, dtype):
-        self.codes, self.scales, self.shape, self.dtype = codes, scales, torch.Size(shape), dtype
+        shape = torch.Size(shape)
+        if len(shape) < 1 or shape[-1] == 0 or dtype not in DTYPES:
+            raise ValueError('Rows8: rows of shape %s, %s' % (tuple(shape), dtype))
+        rows = shape.numel() // shape[-1]
+        for t, name, width in ((codes, 'codes', row_blocks(shape[-1]) * BLOCK), (scales, 'scales', scale_stride(shape[-1]))):
+            if t.dtype != torch.uint8 or tuple(t.shape) != (rows, width) or not t.is_contiguous() or not t.is_cuda or t.device != codes.device:
+                raise ValueError('Rows8: %s have to be contiguous uint8 (%d, %d) on one GPU, got %s %s' % (name, rows, width, t.dtype, tuple(t.shape)))
+        self.codes, self.scales, self.shape, self.dtype = codes, scales, shape, dtype
+
+    @classmethod
+    def _made(cls, codes, scales, shape, dtype):
+        """Of tensors that quantize laid out: nothing to check."""
+        q = cls.__new__(cls)
+        q.codes, q.scales, q.shape, q.dtype = codes, scales, torch.Size(shape), dtype
+        return q
 
     @property
     def device(self):
@@ -136,7 +155,7 @@ def _quantize(x, act=0):
     if R:
         _lib.call('hecka_block8_quantize', x.device, rows.data_ptr(), DTYPES[x.dtype], R, K, ld, act, codes.data_ptr(),
                   scales.data_ptr(), _ptr(y))
-    return Rows8(codes, scales, x.shape, x.dtype), y
+    return Rows8._made(codes, scales, x.shape, x.dtype), y
 
 
 def _values(q, dtype, act=0, dy=None):
@@ -155,6 +174,7 @@ def quantize(x):
 
 def dequantize(q, dtype=None):
     """The values that a Rows8 stands for, in its own dtype or `dtype`."""
+    _check_rows(q, 'block8.dequantize')
     dtype = q.dtype if dtype is None else dtype
     if dtype not in DTYPES:
         raise TypeError('block8.dequantize: float32, bfloat16 or float16, got %s' % dtype)
@@ -226,10 +246,19 @@ def _weight_grad(dy, q, alpha, beta, want_bias=True):
     return dW, db
 
 
+def _bias_grad(dy, scale):
+    """The column sums alone, fp32 in a fixed order: those beside the weight gradient of rows of one zero."""
+    N = dy.shape[1]
+    codes = torch.zeros((N, BLOCK + scale_stride(1)), device=dy.device, dtype=torch.uint8).view(-1)
+    one = Rows8._made(codes[:N * BLOCK], codes[N * BLOCK:], (N, 1), dy.dtype)
+    return _weight_grad(dy, one, 0.0, scale)[1]
+
+
 def weight_grad(dy, rows, scale=1.0, bias_scale=1.0):
     """(dW, db) = (scale dy^T x, bias_scale sum of dy over the rows), fp32, of y = scale x W^T + bias_scale b, from dy [M, N, O] and
     x kept as Rows8 [M, N, I] (or [N, I], shared by all members)."""
     _check(dy, 'block8.weight_grad')
+    _check_rows(rows, 'block8.weight_grad')
     if dy.dim() != 3:
         raise ValueError('block8.weight_grad: dy has to be [members, N, outputs], got %s' % (tuple(dy.shape),))
     _members(rows, dy.shape[0], 'block8.weight_grad')
@@ -273,14 +302,10 @@ class _Linear8(torch.autograd.Function):
         if ctx.needs_input_grad[0]:
             dx = _product(_quantize(dy)[0], codes_t, scales_t, M, I, O, None, scale, 0.0, xdtype, total=len(xshape) == 2)
         if ctx.needs_input_grad[1]:
-            dW, db = _weight_grad(dy, Rows8(codes, scales, xshape, xdtype), scale, bias_scale, want_b)
+            dW, db = _weight_grad(dy, Rows8._made(codes, scales, xshape, xdtype), scale, bias_scale, want_b)
             dW = dW.to(wdtype)
         elif want_b:
-            # the column sums alone: the weight gradient of rows of one zero
-            N = dy.shape[1]
-            one = Rows8(torch.zeros((N, BLOCK), device=dy.device, dtype=torch.uint8),
-                        torch.zeros((N, scale_stride(1)), device=dy.device, dtype=torch.uint8), (N, 1), xdtype)
-            db = _weight_grad(dy, one, 0.0, bias_scale)[1]
+            db = _bias_grad(dy, bias_scale)
         return dx, dW, db, None, None
 
 

@@ -110,6 +110,7 @@ class BatchedLinearCheckpoint(torch.autograd.Function):
         shared = x.ndim == 2
         x, W = x.contiguous(), W.contiguous()
         N = x.shape[-2]
+        block8._sizes('Linear(checkpoint)', M, N, O, I)
         y = _bgemm(x, W, M, N, O, I, 0 if shared else N * I, O * I, False, scale, b.contiguous() if b is not None else None, bias_scale)
         q = block8.quantize(x) if ctx.needs_input_grad[1] else None
         ctx.save_for_backward(W if ctx.needs_input_grad[0] else None, *((q.codes, q.scales) if q is not None else (None, None)))
@@ -130,9 +131,9 @@ class BatchedLinearCheckpoint(torch.autograd.Function):
                 dx = dx.sum(0)
         want_b = has_bias and ctx.needs_input_grad[2]
         if ctx.needs_input_grad[1]:
-            dW, db = block8._weight_grad(dy, block8.Rows8(codes, scales, xshape, torch.float32), scale, bias_scale, want_b)
+            dW, db = block8._weight_grad(dy, block8.Rows8._made(codes, scales, xshape, torch.float32), scale, bias_scale, want_b)
         elif want_b:
-            db = bias_scale * dy.sum(1)
+            db = block8._bias_grad(dy, bias_scale)
         return dx, dW, db, None, None
 
 

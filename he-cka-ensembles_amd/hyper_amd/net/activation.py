@@ -94,7 +94,7 @@ class _Checkpointed(torch.autograd.Function):
     def backward(ctx, dy):
         from .. import block8
         shape, dtype, act = ctx.cfg
-        return block8._values(block8.Rows8(*ctx.saved_tensors, shape, dtype), dtype, act, dy.contiguous()), None
+        return block8._values(block8.Rows8._made(*ctx.saved_tensors, shape, dtype), dtype, act, dy.contiguous()), None
 
 
 def checkpointed(name, x):

@@ -571,7 +571,7 @@ int hecka_block8_linear(const void* x, const void* xscales, int x_members, const
 int hecka_block8_linear_token(const void* x, int dtype, int x_members, const void* w, const void* wscales, int M, int N, int O, int I,
                               const float* bias, long long bstride, float alpha, float beta, void* y, void* stream);
 /* dW [M, O, I] (fp32) = alpha dy^T x, db [M, O] (fp32, may be NULL) = beta sum_n dy; dy [M, N, O] (dtype), x in codes.  Exact
- * products, added in fp32, in a fixed order.  ws: hecka_block8_wgrad_workspace_bytes. */
+ * products, added in fp32, in a fixed order (fp32 and fp16: an infinity in dy gives NaN).  ws: hecka_block8_wgrad_workspace_bytes. */
 size_t hecka_block8_wgrad_workspace_bytes(int M, int N, int O, int I);
 int hecka_block8_wgrad(const void* dy, int dtype, const void* x, const void* xscales, int x_members, int M, int N, int O, int I,
                        float alpha, float beta, float* dW, float* db, void* ws, size_t ws_bytes, void* stream);

@@ -352,6 +352,10 @@ def test_gradient_of_the_bias_alone(dtype):
         y = block8.linear(torch.randn(M, N, 20, device='cuda', dtype=dtype), torch.randn(M, O, 20, device='cuda'), b, bias_scale=0.5)
         db, = torch.autograd.grad(y, b, dy.cuda())
         assert torch.equal(db.cpu().double(), 0.5 * dy.double().sum(1))
+        if dtype == torch.float32:
+            from hyper_amd.layers.linear import BatchedLinearCheckpoint
+            y = BatchedLinearCheckpoint.apply(torch.randn(M, N, 20, device='cuda'), torch.randn(M, O, 20, device='cuda'), b, 1.0, 0.5)
+            assert torch.equal(torch.autograd.grad(y, b, dy.cuda())[0], db)
 
 
 @gpu
@@ -521,11 +525,14 @@ def test_refusals_on_the_gpu():
            lambda: block8.weight_grad(torch.zeros(2, 6, 7, device='cuda'), q), lambda: block8.weight_grad(torch.zeros(3, 5, 7, device='cuda'), q),
            lambda: block8.quantize(torch.zeros(3, 0, device='cuda')), lambda: block8.quantize_weight(torch.zeros(1, 0, 3, device='cuda')),
            lambda: block8.Weight8(w.codes, w.scales, 300), lambda: block8.Weight8(w.codes, w.scales[:, :, :1], 30),
-           lambda: block8.Weight8(w.codes.float(), w.scales, 30), lambda: block8.Weight8(w.codes, w.scales, 30, w.codes_t)]
+           lambda: block8.Weight8(w.codes.float(), w.scales, 30),
+           lambda: block8.Rows8(q.codes, q.scales, (2, 6, 30), torch.float32), lambda: block8.Rows8(q.codes[:, :64], q.scales, (2, 5, 30), torch.float32),
+           lambda: block8.Rows8(q.codes, q.scales.cpu(), (2, 5, 30), torch.float32), lambda: block8.Rows8(q.codes, q.scales, (2, 5, 30), torch.float64), lambda: block8.Weight8(w.codes, w.scales, 30, w.codes_t)]
     for call in bad:
         with pytest.raises(ValueError):
             call()
-    for call in (lambda: block8.quantize(x.double()), lambda: block8.linear(x.double(), W), lambda: block8.dequantize(q, torch.float64)):
+    for call in (lambda: block8.quantize(x.double()), lambda: block8.linear(x.double(), W), lambda: block8.dequantize(q, torch.float64),
+                 lambda: block8.dequantize(x), lambda: block8.weight_grad(torch.zeros(2, 5, 7, device='cuda'), x)):
         with pytest.raises(TypeError):
             call()
     with pytest.raises(RuntimeError, match='serve'):
