@@ -4,6 +4,7 @@ There is deliberately NO fallback: if the shared library is missing or a call fa
 product path raises.  Build it with `make -C he-cka-ensembles_amd/csrc` (or `__graft_entry__.build()`).
 """
 import ctypes
+import functools
 import os
 
 _PATH = os.environ.get('HECKA_LIB_PATH') or os.path.join(os.path.dirname(os.path.abspath(__file__)), 'lib', 'libhecka.so')
@@ -141,6 +142,19 @@ def check(rc, what):
     if rc != 0:
         msg = lib().hecka_last_error()
         raise RuntimeError('libhecka %s failed (%d): %s' % (what, rc, msg.decode() if msg else '?'))
+
+
+def first_order(backward):
+    """once_differentiable, whose context and checks are left out (several microseconds) where nobody asked for a graph of the
+    gradient."""
+    import torch
+    from torch.autograd.function import once_differentiable
+    careful = once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        return careful(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
 
 
 def call(name, device, *args):

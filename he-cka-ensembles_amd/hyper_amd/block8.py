@@ -13,7 +13,6 @@ A value is off by at most half a step of its code: 2^-4 of itself, or 2^-10 of t
 Everything is fp32 / bf16 / fp16 on the GPU; there is no CPU path.  `layers.Linear(compute='e4m3')`, `layers.Linear(
 checkpoint='e4m3')` and `layers.Activation(checkpoint='e4m3')` are the layers on top."""
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -146,7 +145,6 @@ def _rows(x):
 def _quantize(x, act=0):
     if x.dim() < 1 or x.shape[-1] == 0:
         raise ValueError('block8.quantize: needs rows of at least one element, got %s' % (tuple(x.shape),))
-    x = x.detach()
     K = x.shape[-1]
     y = torch.empty(x.shape, device=x.device, dtype=x.dtype) if act else None
     rows, R, ld = _rows(x) if x.numel() else (x, 0, K)
@@ -169,7 +167,7 @@ def _values(q, dtype, act=0, dy=None):
 def quantize(x):
     """x [..., K] (any strides) as Rows8; no gradient passes."""
     _check(x, 'block8.quantize')
-    return _quantize(x)[0]
+    return _quantize(x.detach())[0]
 
 
 def dequantize(q, dtype=None):
@@ -292,7 +290,7 @@ class _Linear8(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_lib.first_order
     def backward(ctx, dy):
         codes, scales, codes_t, scales_t = ctx.saved_tensors
         xshape, xdtype, (M, O, I), wdtype, has_bias, scale, bias_scale = ctx.cfg
@@ -340,7 +338,7 @@ def linear(x, weight, bias=None, scale=1.0, bias_scale=1.0):
         _sizes(what, M, N, O, I)
         b = _bias_rows(bias.detach() if bias is not None else None)
         if isinstance(x, Rows8) or N > 16:
-            q = x if isinstance(x, Rows8) else _quantize(x)[0]
+            q = x if isinstance(x, Rows8) else _quantize(x.detach())[0]
             return _product(q, w.codes, w.scales, M, O, I, b, scale, bias_scale, q.dtype)
         x = x.detach().contiguous()
         y = torch.empty((M, N, O), device=x.device, dtype=x.dtype)

@@ -7,7 +7,6 @@ import math
 import torch
 import torch.nn.functional as F
 import torch.nn.init as init
-from torch.autograd.function import once_differentiable
 
 from .. import _lib, block8, ops
 from ..config import knobs
@@ -118,7 +117,7 @@ class BatchedLinearCheckpoint(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_lib.first_order
     def backward(ctx, dy):
         W, codes, scales = ctx.saved_tensors
         scale, bias_scale, xshape, (M, O, I), has_bias = ctx.cfg

@@ -6,7 +6,6 @@ and return their gradients as one tensor, and the forward kernel updates the run
 is selected in order; otherwise the selected members' statistics are updated with a handful of [members, C] tensor ops."""
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from ..config import knobs
@@ -277,7 +276,7 @@ class _LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_lib.first_order
     def backward(ctx, dy):
         x, mean, rstd, w = ctx.saved_tensors
         packed, has_bias, G, R = ctx.cfg

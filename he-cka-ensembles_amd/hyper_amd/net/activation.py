@@ -3,7 +3,8 @@ activation_gamma :48); stock torch elementwise ops."""
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
+
+from .. import _lib, block8
 
 _H = math.sqrt(2.0) / 2.0
 _C = _H + 0.008274364699
@@ -83,16 +84,14 @@ class _Checkpointed(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, act):
-        from .. import block8
         q, y = block8._quantize(x, act)
         ctx.save_for_backward(q.codes, q.scales)
         ctx.cfg = (q.shape, q.dtype, act)
         return y
 
     @staticmethod
-    @once_differentiable
+    @_lib.first_order
     def backward(ctx, dy):
-        from .. import block8
         shape, dtype, act = ctx.cfg
         return block8._values(block8.Rows8._made(*ctx.saved_tensors, shape, dtype), dtype, act, dy.contiguous()), None
 
@@ -101,7 +100,6 @@ def checkpointed(name, x):
     """act(x) for 'gelu' (erf form), 'silu', 'tanh', 'sigmoid' or 'crater', its input kept for the backward pass in 8-bit blocks
     (block8: a byte per element instead of 2 or 4; y is exact, only the slope is taken at the rounded input).  x: fp32 / bf16 /
     fp16 on the GPU, any shape; blocks run along the last axis."""
-    from .. import block8
     if name not in block8.ACTIVATIONS:
         raise ValueError('no 8-bit checkpoint for activation %r: please select from %s' % (name, sorted(block8.ACTIVATIONS)))
     block8._check(x, 'checkpointed')
