@@ -40,8 +40,8 @@ __device__ __forceinline__ float encodable(float x) {
   return a <= top ? x : a <= 3.402823466e38f ? copysignf(top, x) : __uint_as_float(0x7fc00000u);
 }
 
-// A lane's 32 elements of a block (Piece<T>s), the block's other elements in the lanes 16, 32 and 48 further on: codes as eight
-// dwords, and the scale byte.  Magnitudes are compared as integers (two 16-bit ones at a time), which finds NaN and infinities on
+// A lane's E elements of a block (Piece<T>s) as codes, four a dword, and the block's scale byte; across(bits) is the largest of a
+// number over the lanes that hold the block.  Magnitudes are compared as integers (two 16-bit ones at a time), which finds NaN and infinities on
 // the way; without any, and below 240 2^120, the conversion takes the elements as they are and divides by the scale itself.
 template <class T> struct Magnitude { static constexpr unsigned kLast = 0x7f70; };      // of bf16: 240 2^120
 template <> struct Magnitude<float> { static constexpr unsigned kLast = 0x7f700000; };
@@ -51,9 +51,9 @@ typedef short i16x2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 
-template <class T>
-__device__ __forceinline__ int encode32(const Piece<T> (&p)[32 / Piece<T>::N], unsigned (&codes)[8]) {
-  constexpr int D = sizeof(T) == 4 ? 32 : 16;      // dwords
+template <class T, int E, class Across>
+__device__ __forceinline__ int encode(const Piece<T> (&p)[E / Piece<T>::N], unsigned (&codes)[E / 4], const Across& across) {
+  constexpr int D = E * (int)sizeof(T) / 4;      // dwords
   const unsigned* raw = reinterpret_cast<const unsigned*>(&p[0]);
   unsigned big = 0;
 #pragma unroll
@@ -70,23 +70,18 @@ __device__ __forceinline__ int encode32(const Piece<T> (&p)[32 / Piece<T>::N], u
     const unsigned hi = big >> 16, lo = big & 0xffffu;
     big = hi > lo ? hi : lo;
   }
-  unsigned o = (unsigned)__shfl_xor((int)big, 16);
-  big = o > big ? o : big;
-  o = (unsigned)__shfl_xor((int)big, 32);
-  big = o > big ? o : big;
+  big = across(big);
   if (__any(big > Magnitude<T>::kLast)) {
-    float v[32], a = 0.f;
+    float v[E], a = 0.f;
 #pragma unroll
-    for (int k = 0; k < 32; ++k) {
+    for (int k = 0; k < E; ++k) {
       v[k] = widen(p[k / Piece<T>::N].e[k % Piece<T>::N]);
       a = fmaxf(a, finite_abs(v[k]));
       v[k] = encodable(v[k]);
     }
-    a = fmaxf(a, __shfl_xor(a, 16));
-    a = fmaxf(a, __shfl_xor(a, 32));
-    const int byte = scale_byte(a);
+    const int byte = scale_byte(__uint_as_float(across(__float_as_uint(a))));      // magnitudes order as their bits do
 #pragma unroll
-    for (int i = 0; i < 8; ++i) codes[i] = encode4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], inverse_scale(byte));
+    for (int i = 0; i < E / 4; ++i) codes[i] = encode4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], inverse_scale(byte));
     return byte;
   }
   T top;
@@ -95,7 +90,7 @@ __device__ __forceinline__ int encode32(const Piece<T> (&p)[32 / Piece<T>::N], u
   const int byte = scale_byte(widen(top));
   const float s = scale_of(byte);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < E / 4; ++i) {
     i16x2_t c = {0, 0};
 #pragma unroll
     for (int h = 0; h < 2; ++h) {

@@ -1,13 +1,55 @@
 // 8-bit blocks (block8.hpp): rows and weights to codes, codes back, and activations that keep their input in codes
 // (hecka_block8_*; contract in include/hecka.h).  All HBM bound: one read of the input, one write of each output.
 // Sixteen lanes own a block, eight elements each, so a wave covers four blocks with 16-byte loads (two per lane for fp32),
-// the maximum is four lane shuffles and the codes leave as 8 bytes per lane, 128 per block, contiguous.
+// the maximum is four lane permutes and the codes leave as 8 bytes per lane, 128 per block, contiguous.
+// Measured at 10 x 4096 x 4096 (a copy reaches 5.3 TB/s): quantise 95 us bf16, 162 us fp32 (5.2 TB/s); decode 92 / 163 us (5.4 / 5.1); gelu
+// 174 / 283 us forward and 175 / 287 us backward (4.8 / 5.3), silu 160 / 282 and 161 / 287 (5.2 / 5.3).  bf16 gelu is the one that is
+// near the vector units' rate (about forty instructions an element): with floating-point maxima and guards in place of the integer
+// ones of encode() its forward took 221 us.
 #include "block8.hpp"
 #include "hecka_host.hpp"
 
 namespace hecka {
 
-// eight elements [col, col + 8) of a row of K
+// A lane's eight elements of a block that begins at column col of a row of K: eight neighbours (one 16-byte piece), or of fp32 two
+// pieces of four, 64 apart, so that every load and store instruction covers whole lines (decoding fp32, 10 x 4096 x 4096: 163 us, and
+// 227 us with eight neighbours, whose stores are half lines each).
+template <class T>
+__device__ __forceinline__ void load_lane(const T* row, int col, int lane16, int K, Piece<T> (&p)[8 / Piece<T>::N]) {
+#pragma unroll
+  for (int j = 0; j < 8 / Piece<T>::N; ++j) p[j] = load_piece(row, col + j * 64 + lane16 * Piece<T>::N, K);
+}
+template <class T>
+__device__ __forceinline__ void store_lane(T* row, int col, int lane16, int K, const Piece<T> (&p)[8 / Piece<T>::N]) {
+#pragma unroll
+  for (int j = 0; j < 8 / Piece<T>::N; ++j) {
+    const int c = col + j * 64 + lane16 * Piece<T>::N;
+    if (c < K) store_piece(row, c, K, p[j]);
+  }
+}
+template <class T>
+__device__ __forceinline__ void load_codes(const unsigned char* block, int lane16, unsigned (&c)[2]) {
+  if constexpr (sizeof(T) == 4) {
+    const unsigned* from = reinterpret_cast<const unsigned*>(block) + lane16;
+    c[0] = from[0];
+    c[1] = from[16];
+  } else {
+    const uint2 v = *reinterpret_cast<const uint2*>(block + lane16 * 8);
+    c[0] = v.x;
+    c[1] = v.y;
+  }
+}
+template <class T>
+__device__ __forceinline__ void store_codes(unsigned char* block, int lane16, const unsigned (&c)[2]) {
+  if constexpr (sizeof(T) == 4) {
+    unsigned* to = reinterpret_cast<unsigned*>(block) + lane16;
+    to[0] = c[0];
+    to[16] = c[1];
+  } else {
+    *reinterpret_cast<uint2*>(block + lane16 * 8) = make_uint2(c[0], c[1]);
+  }
+}
+// eight neighbours [col, col + 8) of a weight's row of K
 template <class T>
 __device__ __forceinline__ void load8(const T* row, int col, int K, float* v) {
 #pragma unroll
@@ -15,16 +57,6 @@ __device__ __forceinline__ void load8(const T* row, int col, int K, float* v) {
     const Piece<T> p = load_piece(row, col + j * Piece<T>::N, K);
 #pragma unroll
     for (int i = 0; i < Piece<T>::N; ++i) v[j * Piece<T>::N + i] = widen(p.e[i]);
-  }
-}
-template <class T>
-__device__ __forceinline__ void store8(T* row, int col, int K, const float* v) {
-#pragma unroll
-  for (int j = 0; j < 8 / Piece<T>::N; ++j) {
-    Piece<T> p;
-#pragma unroll
-    for (int i = 0; i < Piece<T>::N; ++i) narrow(v[j * Piece<T>::N + i], p.e[i]);
-    if (col + j * Piece<T>::N < K) store_piece(row, col + j * Piece<T>::N, K, p);
   }
 }
 __device__ __forceinline__ float max8(const float* v) {
@@ -38,26 +70,31 @@ enum { kActNone = 0, kActGelu = 1, kActSilu = 2, kActTanh = 3, kActSigmoid = 4, 
 static constexpr float kHalfRoot = 0.70710678118654752f, kCrater = 0.70710678118654752f + 0.008274364699f;
 
 // e^x, x <= 0, from the hardware's 2^x: the exponent's rounding error, |x| 2^-25, is worked out and put back, so the result is good
-// to about 2 units in the last place (the hardware's own included); 0 from -104 down, where no float is left.
+// to about 2 units in the last place (the hardware's own included); 0 from -104 down, where no float is left.  FINE = false, for 16-bit
+// results: without the repair, 2^-18 of the result where it is largest, against their half steps of 2^-8 and 2^-11.
+template <bool FINE>
 __device__ __forceinline__ float exp_near(float x) {
   x = fmaxf(x, -104.f);
   const float t = x * 1.44269504f;
+  if (!FINE) return __builtin_amdgcn_exp2f(t);
   const float r = fmaf(x, 1.44269504f, -t) + x * 1.92596299e-8f;      // 1.44269504f + 1.92596299e-8f = log2 e
   const float p = __builtin_amdgcn_exp2f(t);
   return fmaf(p, r * 0.69314718f, p);
 }
 // sigmoid(x) and 1 - sigmoid(x), both without cancellation: q = e^-|x| <= 1
+template <bool FINE>
 __device__ __forceinline__ void sigmoid_pair(float x, float& p, float& n) {
-  const float q = exp_near(-fabsf(x)), s = __builtin_amdgcn_rcpf(1.0f + q), qs = q * s;
+  const float q = exp_near<FINE>(-fabsf(x)), s = __builtin_amdgcn_rcpf(1.0f + q), qs = q * s;
   p = x >= 0.f ? s : qs;
   n = x >= 0.f ? qs : s;
   if (x != x) p = n = x;
 }
 // normal distribution below x: 0.5 erfc(-x / sqrt 2).  erfc(z) for z >= 0 as a polynomial in 1 / (1 + p z) times e^-z^2
 // (Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26; absolute error below 1.5e-7), no cancellation on either side.
+template <bool FINE>
 __device__ __forceinline__ float normal_below(float x, float& bell) {
   const float z = fabsf(x) * kHalfRoot, t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, z, 1.0f));
-  bell = exp_near(-0.5f * x * x);
+  bell = exp_near<FINE>(-0.5f * x * x);
   float c = fmaf(1.061405429f, t, -1.453152027f);
   c = fmaf(c, t, 1.421413741f);
   c = fmaf(c, t, -0.284496736f);
@@ -66,22 +103,22 @@ __device__ __forceinline__ float normal_below(float x, float& bell) {
   return x >= 0.f ? 1.0f - half : half;
 }
 
-template <int ACT>
+template <int ACT, bool FINE>
 __device__ __forceinline__ float act_value(float x) {
   float p, n;
-  if (ACT == kActGelu) return x * normal_below(x, n);
+  if (ACT == kActGelu) return x * normal_below<FINE>(x, n);
   if (ACT == kActTanh) return tanhf(x);
-  sigmoid_pair(ACT == kActCrater ? 2.0f * kHalfRoot * (x + 1.0f) : x, p, n);      // 1 + tanh z = 2 sigmoid(2 z)
+  sigmoid_pair<FINE>(ACT == kActCrater ? 2.0f * kHalfRoot * (x + 1.0f) : x, p, n);      // 1 + tanh z = 2 sigmoid(2 z)
   return ACT == kActSilu ? x * p : ACT == kActSigmoid ? p : 2.0f * kCrater * (x * p);
 }
-template <int ACT>
+template <int ACT, bool FINE>
 __device__ __forceinline__ float act_slope(float x) {
   float p, n;
   if (ACT == kActGelu) {
-    p = normal_below(x, n);
+    p = normal_below<FINE>(x, n);
     return fmaf(x * 0.39894228f, n, p);
   }
-  sigmoid_pair(ACT == kActTanh ? 2.0f * x : ACT == kActCrater ? 2.0f * kHalfRoot * (x + 1.0f) : x, p, n);
+  sigmoid_pair<FINE>(ACT == kActTanh ? 2.0f * x : ACT == kActCrater ? 2.0f * kHalfRoot * (x + 1.0f) : x, p, n);
   if (ACT == kActTanh) return 4.0f * p * n;
   if (ACT == kActSigmoid) return p * n;
   if (ACT == kActSilu) return fmaf(x * p, n, p);
@@ -93,13 +130,12 @@ __device__ __forceinline__ float act_slope(float x) {
 // the first is worked on: one block per lane group in flight (128 bytes of codes) leaves the memory idle - decoding bf16 reached
 // 2.75 TB/s that way.
 template <bool FLAT>
-struct Place { long long row; int blk, col; };
+struct Place { long long row; int blk; };
 template <bool FLAT>
-__device__ __forceinline__ Place<FLAT> place_block(long long b, long long total, int nblk, int lane16) {
-  if constexpr (FLAT) return {0, 0, 0};
+__device__ __forceinline__ Place<FLAT> place_block(long long b, long long total, int nblk) {
+  if constexpr (FLAT) return {0, 0};
   const long long row = total <= 0xffffffffLL ? (long long)((unsigned)b / (unsigned)nblk) : b / nblk;
-  const int blk = (int)(b - row * nblk);
-  return {row, blk, blk * kBlock + lane16 * 8};
+  return {row, (int)(b - row * nblk)};
 }
 
 // rows of K elements, `ld` apart; ACT != 0: y (rows of K, contiguous) = act(x) beside the codes of x
@@ -111,32 +147,30 @@ __global__ __launch_bounds__(256) void block8_rows_kernel(const T* __restrict__ 
   const int nblk = row_blocks(K), lane16 = threadIdx.x & 15, group = threadIdx.x >> 4;
   const long long total = R * nblk;
   for (long long b0 = (long long)blockIdx.x * (16 * UNROLL) + group; b0 < total; b0 += (long long)gridDim.x * (16 * UNROLL)) {
-    float v[UNROLL][8];
+    Piece<T> p[UNROLL][8 / Piece<T>::N];
     Place<FLAT> at[UNROLL];
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
       const long long b = b0 + u * 16 < total ? b0 + u * 16 : total - 1;
-      at[u] = place_block<FLAT>(b, total, nblk, lane16);
-      if constexpr (FLAT) load8(x + b * kBlock, lane16 * 8, kBlock, v[u]);
-      else load8(x + at[u].row * ld, at[u].col, K, v[u]);
+      at[u] = place_block<FLAT>(b, total, nblk);
+      if constexpr (FLAT) load_lane(x + b * kBlock, 0, lane16, kBlock, p[u]);
+      else load_lane(x + at[u].row * ld, at[u].blk * kBlock, lane16, K, p[u]);
     }
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
       const long long b = b0 + u * 16;
       if (b >= total) break;
       if (ACT != kActNone) {
-        float a[8];
+        Piece<T> a[8 / Piece<T>::N];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) a[i] = act_value<ACT>(v[u][i]);
-        if constexpr (FLAT) store8(y + b * kBlock, lane16 * 8, kBlock, a);
-        else store8(y + at[u].row * K, at[u].col, K, a);
+        for (int i = 0; i < 8; ++i)
+          narrow(act_value<ACT, sizeof(T) == 4>(widen(p[u][i / Piece<T>::N].e[i % Piece<T>::N])), a[i / Piece<T>::N].e[i % Piece<T>::N]);
+        if constexpr (FLAT) store_lane(y + b * kBlock, 0, lane16, kBlock, a);
+        else store_lane(y + at[u].row * K, at[u].blk * kBlock, lane16, K, a);
       }
-      const int byte = scale_byte(max16(max8(v[u])));
-      const float inv = inverse_scale(byte);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[u][i] = encodable(v[u][i]);
-      *reinterpret_cast<uint2*>(codes + b * kBlock + lane16 * 8) =
-          make_uint2(encode4(v[u][0], v[u][1], v[u][2], v[u][3], inv), encode4(v[u][4], v[u][5], v[u][6], v[u][7], inv));
+      unsigned c[2];
+      const int byte = encode<T, 8>(p[u], c, [](unsigned v) { return max16(v); });
+      store_codes<T>(codes + b * kBlock, lane16, c);
       if (lane16 == 0) {
         if constexpr (FLAT) {
           scales[b] = (unsigned char)byte;
@@ -160,19 +194,19 @@ __global__ __launch_bounds__(256) void block8_values_kernel(const unsigned char*
   const int nblk = row_blocks(K), lane16 = threadIdx.x & 15, group = threadIdx.x >> 4;
   const long long total = R * nblk;
   for (long long b0 = (long long)blockIdx.x * (16 * UNROLL) + group; b0 < total; b0 += (long long)gridDim.x * (16 * UNROLL)) {
-    uint2 c[UNROLL];
+    unsigned c[UNROLL][2];
     int byte[UNROLL];
-    float d[UNROLL][8];
+    Piece<T> d[UNROLL][8 / Piece<T>::N];
     Place<FLAT> at[UNROLL];
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
       const long long b = b0 + u * 16 < total ? b0 + u * 16 : total - 1;
-      at[u] = place_block<FLAT>(b, total, nblk, lane16);
-      c[u] = *reinterpret_cast<const uint2*>(codes + b * kBlock + lane16 * 8);
+      at[u] = place_block<FLAT>(b, total, nblk);
+      load_codes<T>(codes + b * kBlock, lane16, c[u]);
       byte[u] = FLAT ? scales[b] : scales[at[u].row * ((nblk + 3) & ~3) + at[u].blk];
       if (ACT != kActNone) {
-        if constexpr (FLAT) load8(dy + b * kBlock, lane16 * 8, kBlock, d[u]);
-        else load8(dy + at[u].row * K, at[u].col, K, d[u]);
+        if constexpr (FLAT) load_lane(dy + b * kBlock, 0, lane16, kBlock, d[u]);
+        else load_lane(dy + at[u].row * K, at[u].blk * kBlock, lane16, K, d[u]);
       }
     }
 #pragma unroll
@@ -180,17 +214,17 @@ __global__ __launch_bounds__(256) void block8_values_kernel(const unsigned char*
       const long long b = b0 + u * 16;
       if (b >= total) break;
       float v[8];
-      decode4(c[u].x, scale_of(byte[u]), v);
-      decode4(c[u].y, scale_of(byte[u]), v + 4);
-      if (ACT != kActNone) {
+      decode4(c[u][0], scale_of(byte[u]), v);
+      decode4(c[u][1], scale_of(byte[u]), v + 4);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = d[u][i] * act_slope<ACT>(v[i]);
-      } else if constexpr (__is_same(T, F16)) {      // fp16's largest, 65504, is kept as 65536: back to what fp16 holds
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = fabsf(v[i]) == 65536.f ? copysignf(65504.f, v[i]) : v[i];
+      for (int i = 0; i < 8; ++i) {
+        T& e = d[u][i / Piece<T>::N].e[i % Piece<T>::N];
+        if (ACT != kActNone) v[i] = widen(e) * act_slope<ACT, sizeof(T) == 4>(v[i]);
+        else if (__is_same(T, F16) && fabsf(v[i]) == 65536.f) v[i] = copysignf(65504.f, v[i]);      // fp16's largest, 65504, is kept as 65536: back to what fp16 holds
+        narrow(v[i], e);
       }
-      if constexpr (FLAT) store8(out + b * kBlock, lane16 * 8, kBlock, v);
-      else store8(out + at[u].row * K, at[u].col, K, v);
+      if constexpr (FLAT) store_lane(out + b * kBlock, 0, lane16, kBlock, d[u]);
+      else store_lane(out + at[u].row * K, at[u].blk * kBlock, lane16, K, d[u]);
     }
   }
 }

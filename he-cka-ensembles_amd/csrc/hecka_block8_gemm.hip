@@ -391,7 +391,12 @@ __global__ __launch_bounds__(64 * W) void block8_token_kernel(const T* __restric
 #pragma unroll
     for (int i = 0; i < NT; ++i) { d[i][0] = c[i][0]; d[i][1] = c[i][1]; }
     unsigned cx[8];
-    const float sx = scale_of(encode32(px, cx)), sw = scale_of(sb);
+    const float sx = scale_of(encode<T, 32>(px, cx, [](unsigned v) {      // a block's lanes are 16 apart
+      unsigned o = (unsigned)__shfl_xor((int)v, 16);
+      v = o > v ? o : v;
+      o = (unsigned)__shfl_xor((int)v, 32);
+      return o > v ? o : v;
+    })), sw = scale_of(sb);
     load(kb + W);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {

@@ -67,6 +67,14 @@ __device__ __forceinline__ float max16(float v) {
   v = fmaxf(v, dpp<0x141>(v));
   return fmaxf(v, dpp<0x140>(v));
 }
+__device__ __forceinline__ unsigned max16(unsigned v) {
+  auto with = [&](int o) { v = (unsigned)o > v ? (unsigned)o : v; };
+  with(__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, true));
+  with(__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, true));
+  with(__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, true));
+  with(__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xf, 0xf, true));
+  return v;
+}
 __device__ __forceinline__ float lane_value(float v, int lane) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
 }
