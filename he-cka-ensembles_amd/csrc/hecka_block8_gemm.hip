@@ -97,6 +97,10 @@ __device__ __forceinline__ void store_tile(const f32x4v (&acc)[S][S], const Piec
 //   a half step of 2^-8 of a bf16 result and 2^-11 of an fp16 one - so 16-bit results take it.
 // EXACT = true (fp32 results): the codes are widened to bf16 on their way out of LDS - exact - and the bf16 instruction
 //   adds their products in fp32 (1.4e-7 at K = 8192), at half the rate.
+// Bound by the matrix instructions: 256 x 256 tiles reach 2.6 PF (fp8) and 1.36 - 1.41 PF (widened) at 8192^3, where a library's
+// plain products reach 2.70 and 1.41; 2048 x 8192 x 8192 2.25 / 1.39 PF (256 workgroups, one round: the first loads and the last
+// stores hide behind nothing).  Four waves of 128 x 128 outputs each: 256 sums a lane leave every fragment read from LDS eight
+// products, and one workgroup a CU.  128 x 128 tiles (1.47 PF at best) where those are too few for the chip (linear_plan).
 // ------------------------------------------------------------------------------------------------------------------
 template <bool EXACT> struct Raw { typedef i32x8 type; };
 template <> struct Raw<true> { typedef i32x4 type; };
@@ -348,6 +352,9 @@ __global__ __launch_bounds__(256) void block8_join_kernel(const float* __restric
 // reads 32 codes per lane and row, a block ahead, and makes the codes of x for its blocks by itself (the same codes as
 // hecka_block8_quantize: 32 elements per lane, the maximum over the four lanes of a row).  All products in bf16, exact.
 // The W waves' sums are added in order.
+// 8 x 4096 x 4096, weights from HBM: 39 us, 3.4 TB/s of codes (32 us out of the last-level cache); 1 x 4096 x 4096 11 us.  Bound by the
+// memory's latency under load: a start elsewhere in K for every workgroup changes nothing, two blocks ahead cost registers and with
+// them waves (58 us).
 // ------------------------------------------------------------------------------------------------------------------
 template <class T, int NT, int W>
 __global__ __launch_bounds__(64 * W) void block8_token_kernel(const T* __restrict__ x, long long xstride, int N, int K,
@@ -435,6 +442,9 @@ __global__ __launch_bounds__(64 * W) void block8_token_kernel(const T* __restric
 // LDS rows hold units of 16 columns (32 bytes); unit u of row n sits at u ^ (n & 7): a transposing read takes one unit of
 // sixteen rows, eight of which lie on different banks.
 // Few tiles (small O x I): the rows are cut into pieces by blockIdx.y, whose sums a second kernel adds up in order.
+// 8 x 4096 rows, 2048 x 2048: fp32 607 us (three products each: 1.36 PF), fp16 431 us (1.28 PF), bf16 284 us (0.97 PF; a plain library
+// product 1.41).  fp32 and fp16 are bound by the matrix instructions; bf16 by LDS beside them: a step's 64 KB written and 128 KB
+// read are three quarters of the time of its products, and the staging's vector instructions share the issue slots.
 // ------------------------------------------------------------------------------------------------------------------
 template <class T, int TERMS, int B, bool WHOLE>
 __global__ __launch_bounds__(256) void block8_wgrad_kernel(
@@ -699,15 +709,17 @@ __global__ __launch_bounds__(256) void block8_slabs_kernel(const float* __restri
 static int cdiv(int a, int b) { return (a + b - 1) / b; }
 static constexpr int kLinearFill = 256, kLinearLeast = 8;
 
-// 256 x 256 outputs a workgroup where that fills three quarters of the chip, else 128 x 128, and where those leave half of it idle the
-// blocks of K are shared out, eight at least to each, their sums joined by a second launch.  Measured (bf16 / fp32 results):
-// 1 x 64 x 8192 x 8192 48 / 73 us whole, 24 / 30 us in four shares, 31 / 30 us in eight; 1 x 64 x 1024 x 8192 41 / 73 us whole, 15 /
+// 256 x 256 outputs a workgroup where that gives most of the chip's CUs one (128 x 128 ones, two a CU, load twice as much), else 128 x
+// 128, and where those leave half of the chip idle the blocks of K are shared out, eight at least to each, their sums joined by a
+// second launch.  Measured (bf16 / fp32 results), large tiles against small: 1 x 2048 x 8192 x 4096, 256 large ones, 64 / 113 against 115 /
+// 132 us; 1 x 1280 x 8192 x 4096, 160, 58 / 107 against 87 / 99; 1 x 1024 x 8192 x 4096, 128, 57 / 107 against 63 / 72; 5 x 1000 x 1000 x
+// 1000, 80, 24 / 38 against 22 / 23; 12 x 1024 x 1024 x 1024, 192, 27 / 41 against 34 / 35.  Shares: 1 x 64 x 8192 x 8192 48 / 73 us whole, 24 / 30 us in four shares, 31 / 30 us in eight; 1 x 64 x 1024 x 8192 41 / 73 us whole, 15 /
 // 19 us in eight; 1 x 512 x 4096 x 4096 28 / 45 us whole, 27 / 35 us in two, 38 / 35 us in four; shares of four blocks: 1 x 256 x 4096 x
 // 4096 32 us against 22.
 struct LinearPlan { int tile, splits, share; };
-static LinearPlan linear_plan(int M, int N, int O, int nblk) {
+static LinearPlan linear_plan(int M, int N, int O, int nblk, bool exact) {
   LinearPlan p{256, 1, (nblk + 3) & ~3};
-  if ((long long)M * cdiv(N, 256) * cdiv(O, 256) >= 192) return p;
+  if ((long long)M * cdiv(N, 256) * cdiv(O, 256) >= (exact ? 224 : 112)) return p;
   p.tile = 128;
   const long long tiles = (long long)M * cdiv(N, 128) * cdiv(O, 128), s = kLinearFill / tiles;
   if (s > 1) {
@@ -773,19 +785,19 @@ static int token_run(const void* x, long long xstride, int M, int N, int K, cons
 
 struct WgradPlan { int tile, to, ti, splits, rows; };
 static WgradPlan wgrad_plan(int M, int N, int O, int I, bool whole) {
-  WgradPlan p;
-  // 256 x 256 tiles, one workgroup per CU, where they - cut into pieces of at least 512 rows - fill three quarters of the
-  // chip; else, and where dy's rows are not whole 16-byte pieces (guarded loads, for which 256 x 256 leaves no registers),
-  // 128 x 128 tiles, two per CU, in pieces of at least 256 rows
-  for (p.tile = whole ? 256 : 128;; p.tile = 128) {
-    p.to = cdiv(O, p.tile);
-    p.ti = cdiv(I, p.tile);
-    const long long tiles = (long long)M * p.to * p.ti, fill = p.tile == 256 ? 256 : 512;
-    const int most = cdiv(N, 2 * p.tile);
-    const long long s = tiles >= fill ? 1 : fill / tiles;
-    p.splits = (int)(s < most ? s : most);
-    if (p.tile == 128 || (tiles * p.splits >= 192 && O > 128 && I > 128)) break;
-  }
+  // 256 x 256 tiles, one workgroup per CU, where they fill three quarters of the chip and dy's rows are whole 16-byte pieces (guarded
+  // loads, for which 256 x 256 leaves no registers, otherwise); else 128 x 128 tiles, two per CU, and where those are too few the
+  // rows in pieces of 256 at least.  Measured (bf16 / fp32): 4 x 2000 x 2000 x 2000, 256 large tiles, 82 / 177 us, 107 / 208 us with
+  // small ones; 2 x 1024 x 2048 x 2048, 128 large tiles, 53 / 75 us cut in two, 32 / 55 us with 512 small ones; 1 x 65536 x 256 x 512 small
+  // tiles 56 / 79 us, large ones, cut into many pieces, 72 / 92 us.
+  WgradPlan p{256, cdiv(O, 256), cdiv(I, 256), 1, cdiv(N, 64) * 64};
+  if (whole && (long long)M * p.to * p.ti >= 192 && O > 128 && I > 128) return p;
+  p.tile = 128;
+  p.to = cdiv(O, 128);
+  p.ti = cdiv(I, 128);
+  const long long tiles = (long long)M * p.to * p.ti, s = tiles >= 512 ? 1 : 512 / tiles;
+  const int most = cdiv(N, 256);
+  p.splits = (int)(s < most ? s : most);
   p.rows = cdiv(cdiv(N, p.splits), 64) * 64;
   p.splits = cdiv(N, p.rows);
   return p;
@@ -827,9 +839,9 @@ using namespace hecka;
 
 extern "C" {
 
-size_t hecka_block8_linear_workspace_bytes(int M, int N, int O, int I, int y_members) {
-  if (bad_sizes(M, N, O, I) || (y_members != M && y_members != 1)) return 0;
-  return linear_workspace(linear_plan(M, N, O, row_blocks(I)), M, N, O, y_members);
+size_t hecka_block8_linear_workspace_bytes(int M, int N, int O, int I, int y_members, int dtype) {
+  if (bad_type(dtype) || bad_sizes(M, N, O, I) || (y_members != M && y_members != 1)) return 0;
+  return linear_workspace(linear_plan(M, N, O, row_blocks(I), dtype == HECKA_DT_F32), M, N, O, y_members);
 }
 
 int hecka_block8_linear(const void* x, const void* xscales, int x_members, const void* w, const void* wscales, int M, int N, int O,
@@ -843,7 +855,7 @@ int hecka_block8_linear(const void* x, const void* xscales, int x_members, const
   if (!aligned16(x) || !aligned16(w) || (reinterpret_cast<uintptr_t>(xscales) & 3) || (reinterpret_cast<uintptr_t>(wscales) & 3))
     return fail(HECKA_EINVAL, "block8_linear: codes need 16-byte alignment, scales 4-byte%s");
   const int nblk = row_blocks(I);
-  const LinearPlan p = linear_plan(M, N, O, nblk);
+  const LinearPlan p = linear_plan(M, N, O, nblk, dtype == HECKA_DT_F32);
   if ((ws ? ws_bytes : 0) < linear_workspace(p, M, N, O, y_members))
     return fail(HECKA_EWORKSPACE, "%sblock8_linear: workspace too small (%lld bytes given)", "", (long long)ws_bytes);
   clear_error();

@@ -6,8 +6,10 @@
 // HBM bound: the forward reads x and writes y once, the backward reads x and dy and writes dx once.  A row therefore stays in
 // the registers of TPR threads (16 elements each at most) between its loads and its stores, so that the variance is the
 // two-pass one (mean first, then squared distances) at no extra traffic; all statistics are fp32.  A row of up to 1024
-// elements belongs to 16, 32 or 64 lanes of a wave (its sums need no barrier), a longer one to 256 / 512 / 1024 threads; the
+// elements belongs to 8, 16, 32 or 64 lanes of a wave (its sums need no barrier), a longer one to 256 / 512 / 1024 threads; the
 // next row's loads are under way while a row is summed.
+// Measured (a copy reaches 5.3 TB/s): 2 x 16384 x 8192 bf16 209 us forward (5.1 TB/s), 335 us backward (4.8); 10 x 2048 x 2048 fp32 65 us
+// (5.2) and 112 us (4.5, the partial sums included); rows of 1001 fp16, 5 x 300: 6 and 18 us, latency.
 // The backward keeps every thread's columns of dw and db in registers over all rows of its workgroup and writes them once:
 // [workgroups per member, 2, D] partial sums, added up in a fixed order by a second kernel - no atomics, the same bits on
 // every run.
@@ -232,12 +234,15 @@ static const int kMaxNormWidth = 16384;
 
 // Threads of a row: few enough that most have work (a piece is 4 or 8 elements), enough that none has more than 16 elements
 // (forward) or 8 (backward, which holds five values for each and would leave too few waves: bf16 rows of 8192 350 us with 8
-// elements in 1024 threads, 475 us with 16 in 512).  Beyond 8192 the backward has 16 as well and loads nothing ahead.
+// elements in 1024 threads, 475 us with 16 in 512).  Beyond 8192 the backward has 16 as well and loads nothing ahead.  Up to 1024
+// elements a wave at most, whose sums need no barrier (2^25 elements of bf16, rows of 1024: 23 / 40 us forward / backward, 28 / 47 with two waves; of
+// 128: 23 / 40 us with 16 lanes, 80 / 107 with 64; of 64: 23 / 41 us with 8 lanes, 43 / 62 with 16).
 static int norm_threads(int D, int piece, bool forward) {
+  if (D <= 8 * piece) return 8;
   if (D <= 16 * piece) return 16;
   if (D <= 32 * piece) return 32;
+  if (D <= 1024) return 64;
   const int share = forward || D > 8192 ? 16 : 8;
-  if (forward ? D <= 1024 : D <= 512) return 64;
   return D <= 128 * share ? 128 : D <= 256 * share ? 256 : D <= 512 * share ? 512 : 1024;
 }
 
@@ -258,6 +263,7 @@ static int norm_dispatch(int D, bool forward, const F& f) {
 #define HECKA_NORM(TPR) \
   case TPR: return need <= 1 ? f.template run<T, TPR, 1>() : need <= 2 ? f.template run<T, TPR, 2>() : f.template run<T, TPR, 16 / N>();
   switch (t) {
+    case 8: return f.template run<T, 8, 1>();
     case 16: return f.template run<T, 16, 1>();
     case 32: return f.template run<T, 32, 1>();
     HECKA_NORM(64)

@@ -78,9 +78,14 @@ __device__ __forceinline__ unsigned max16(unsigned v) {
 __device__ __forceinline__ float lane_value(float v, int lane) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
 }
-// sum over the LANES (16, 32, 64) lanes that a row has of this wave
+// sum over the LANES (8, 16, 32, 64) lanes that a row has of this wave
 template <int LANES>
 __device__ __forceinline__ float lanes_sum(float v) {
+  if constexpr (LANES == 8) {
+    v += dpp<0xB1>(v);
+    v += dpp<0x4E>(v);
+    return v + dpp<0x141>(v);
+  }
   v = sum16(v);
   if constexpr (LANES == 16) return v;
   const float a = lane_value(v, 0) + lane_value(v, 16), b = lane_value(v, 32) + lane_value(v, 48);

@@ -102,7 +102,7 @@ SIGNATURES = {
     'hecka_block8_quantize': (_i, [_vp, _i, _ll, _i, _ll, _i, _vp, _vp, _vp, _vp]),
     'hecka_block8_values': (_i, [_vp, _vp, _vp, _i, _ll, _i, _i, _vp, _vp]),
     'hecka_block8_weight': (_i, [_vp, _i, _i, _i, _i, _ll, _vp, _vp, _vp, _vp, _vp]),
-    'hecka_block8_linear_workspace_bytes': (_sz, [_i, _i, _i, _i, _i]),
+    'hecka_block8_linear_workspace_bytes': (_sz, [_i, _i, _i, _i, _i, _i]),
     'hecka_block8_linear': (_i, [_vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _vp, _ll, ctypes.c_float, ctypes.c_float, _vp, _i, _i, _vp, _sz, _vp]),
     'hecka_block8_linear_token': (_i, [_vp, _i, _i, _vp, _vp, _i, _i, _i, _i, _vp, _ll, ctypes.c_float, ctypes.c_float, _vp, _vp]),
     'hecka_block8_wgrad_workspace_bytes': (_sz, [_i, _i, _i, _i]),

@@ -221,7 +221,7 @@ def _product(q, codes, scales, M, O, I, bias, alpha, beta, dtype, total=False):
     y = torch.empty((N, O) if total else (M, N, O), device=q.device, dtype=dtype)
     if y.numel():
         ym = 1 if total else M
-        nbytes = _lib.lib().hecka_block8_linear_workspace_bytes(M, N, O, I, ym)
+        nbytes = _lib.lib().hecka_block8_linear_workspace_bytes(M, N, O, I, ym, DTYPES[dtype])
         ws = torch.empty((nbytes // 4,), device=q.device, dtype=torch.float32) if nbytes else None
         _lib.call('hecka_block8_linear', q.device, q.codes.data_ptr(), q.scales.data_ptr(), 1 if len(q.shape) == 2 else M,
                   codes.data_ptr(), scales.data_ptr(), M, N, O, I, _ptr(bias), _bstride(bias), alpha, beta, y.data_ptr(), DTYPES[dtype],

@@ -563,7 +563,7 @@ int hecka_block8_weight(const void* W, int dtype, int M, int O, int I, long long
  * or 1 for rows that all members share) and weights in codes; y in dtype.  HECKA_DT_F32: exact products, added in fp32;
  * 16-bit: fp8 matrix instructions (about 1.5e-5 of the result before its rounding).  y_members: M, or 1 for the sum over the
  * members (no bias), added in fp32 and rounded once.  ws: hecka_block8_linear_workspace_bytes.  Sizes up to 2^22. */
-size_t hecka_block8_linear_workspace_bytes(int M, int N, int O, int I, int y_members);
+size_t hecka_block8_linear_workspace_bytes(int M, int N, int O, int I, int y_members, int dtype);
 int hecka_block8_linear(const void* x, const void* xscales, int x_members, const void* w, const void* wscales, int M, int N, int O,
                         int I, const float* bias, long long bstride, float alpha, float beta, void* y, int dtype, int y_members,
                         void* ws, size_t ws_bytes, void* stream);

@@ -320,7 +320,7 @@ def test_shared_rows_and_their_gradient():
 def test_long_sums_shared_out(M, N, O, I, dtype):
     """Few tiles and many blocks of K: the slabs' sum, its bias and rounding, and the same bits on every call."""
     from hyper_amd import _lib, block8
-    assert _lib.lib().hecka_block8_linear_workspace_bytes(M, N, O, I, M) > 0
+    assert _lib.lib().hecka_block8_linear_workspace_bytes(M, N, O, I, M, TYPES.index(dtype)) > 0
     x, W, b = whole((M, N, I), 1), whole((M, O, I), 2), whole((M, O), 3, 50)
     q, w = block8.quantize(x.to(dtype).cuda()), block8.quantize_weight(W.cuda())
     for bias in (None, b):
@@ -505,10 +505,10 @@ def test_refusals_without_a_gpu():
     assert L.hecka_block8_linear(odd, p, 1, p, p, 1, 8, 8, 8, None, 0, 1.0, 0.0, p, 0, 1, None, 0, None) == -1
     assert L.hecka_block8_linear(p, p, 1, p, p, 3, 8, 8, 8, None, 0, 1.0, 0.0, p, 0, 2, None, 0, None) == -1      # a sum over some members
     assert L.hecka_block8_linear(p, p, 1, p, p, 3, 8, 8, 8, p, 8, 1.0, 1.0, p, 0, 1, None, 0, None) == -1         # a sum with a bias
-    need = L.hecka_block8_linear_workspace_bytes(1, 64, 1024, 8192, 1)
+    need = L.hecka_block8_linear_workspace_bytes(1, 64, 1024, 8192, 1, 0)
     assert need > 0 and need % (64 * 1024 * 4) == 0                                                               # slabs of a split K
     assert L.hecka_block8_linear(p, p, 1, p, p, 1, 64, 1024, 8192, None, 0, 1.0, 0.0, p, 0, 1, p, need - 1, None) == -3
-    assert L.hecka_block8_linear_workspace_bytes(3, 8, 8, 8, 1) == 3 * 64 * 4 and L.hecka_block8_linear_workspace_bytes(3, 8, 8, 8, 3) == 0
+    assert L.hecka_block8_linear_workspace_bytes(3, 8, 8, 8, 1, 1) == 3 * 64 * 4 and L.hecka_block8_linear_workspace_bytes(3, 8, 8, 8, 3, 2) == 0
     assert L.hecka_block8_linear_token(p, 0, 1, p, p, 1, 17, 8, 8, None, 0, 1.0, 0.0, p, None) == -1
     assert L.hecka_block8_wgrad(p, 0, p, p, 1, 1, 5000, 8, 8, 1.0, 1.0, p, p, None, 0, None) == -3
     assert L.hecka_block8_wgrad_workspace_bytes(1, 0, 8, 8) == 0
