@@ -249,6 +249,8 @@ static int norm_threads(int D, int piece, bool forward) {
 // Workgroups per member: every row its own share, up to `most` in all.  Forward: eight per CU, but for long rows (whose weight
 // and bias, 8 bytes an element, a workgroup reads once) two.  Backward: enough to fill the chip once with sixteen waves per CU,
 // so that the partial sums stay a few per cent of the traffic.
+// 2^25 elements of bf16, rows of 2048, forward / backward: 24 / 42 us, with half as many 31 / 49, with twice as many 25 / 50; rows of
+// 8192: 27 / 44, 26 / 45 and 29 / 54.
 static int norm_chunks(long long G, long long R, int threads, bool forward) {
   const int rpb = threads <= 64 ? 256 / threads : 1;
   const long long most = forward ? (threads >= 1024 ? 512 : threads == 512 ? 1024 : 2048) : threads <= 256 ? (threads == 128 ? 2048 : 1024) : threads == 512 ? 512 : 256;
