@@ -138,7 +138,7 @@ __device__ __forceinline__ Place<FLAT> place_block(long long b, long long total,
   return {row, (int)(b - row * nblk)};
 }
 
-// rows of K elements, `ld` apart; ACT != 0: y (rows of K, contiguous) = act(x) beside the codes of x
+// rows of K elements, `ld` apart; ACT != 0: y (rows of K, contiguous) = act(x) beside the codes of x, or alone where codes is null
 template <class T, int ACT, bool FLAT>
 __global__ __launch_bounds__(256) void block8_rows_kernel(const T* __restrict__ x, long long R, int K, long long ld,
                                                           unsigned char* __restrict__ codes, unsigned char* __restrict__ scales,
@@ -168,6 +168,7 @@ __global__ __launch_bounds__(256) void block8_rows_kernel(const T* __restrict__ 
         if constexpr (FLAT) store_lane(y + b * kBlock, 0, lane16, kBlock, a);
         else store_lane(y + at[u].row * K, at[u].blk * kBlock, lane16, K, a);
       }
+      if (ACT != kActNone && !codes) continue;
       unsigned c[2];
       const int byte = encode<T, 8>(p[u], c, [](unsigned v) { return max16(v); });
       store_codes<T>(codes + b * kBlock, lane16, c);
@@ -358,7 +359,7 @@ int hecka_block8_quantize(const void* x, int dtype, long long R, int K, long lon
   if (bad_type(dtype)) return fail(HECKA_EINVAL, "block8_quantize: unknown dtype%s");
   if (bad_rows(R, K) || ld < K) return fail(HECKA_EINVAL, "%sblock8_quantize: bad size (%lld rows of %lld)", "", R, K);
   if (act < kActNone || act > kActCrater) return fail(HECKA_EINVAL, "%sblock8_quantize: unknown activation (%lld)", "", act);
-  if (!x || !codes || !scales || (act != kActNone && !y)) return fail(HECKA_EINVAL, "block8_quantize: null pointer%s");
+  if (!x || !codes != !scales || (act == kActNone && !codes) || (act != kActNone && !y)) return fail(HECKA_EINVAL, "block8_quantize: null pointer%s");
   if (!aligned16(codes)) return fail(HECKA_EINVAL, "block8_quantize: codes need 16-byte alignment%s");
   clear_error();
   hipStream_t st = (hipStream_t)stream;

@@ -142,17 +142,20 @@ def _rows(x):
     return flat, R, flat.stride(0)
 
 
-def _quantize(x, act=0):
+def _quantize(x, act=0, keep=True):
     if x.dim() < 1 or x.shape[-1] == 0:
         raise ValueError('block8.quantize: needs rows of at least one element, got %s' % (tuple(x.shape),))
     K = x.shape[-1]
     y = torch.empty(x.shape, device=x.device, dtype=x.dtype) if act else None
     rows, R, ld = _rows(x) if x.numel() else (x, 0, K)
-    codes = torch.empty((R, row_blocks(K) * BLOCK), device=x.device, dtype=torch.uint8)
-    scales = torch.empty((R, scale_stride(K)), device=x.device, dtype=torch.uint8)
+    codes = scales = None
+    if keep:
+        codes = torch.empty((R, row_blocks(K) * BLOCK), device=x.device, dtype=torch.uint8)
+        scales = torch.empty((R, scale_stride(K)), device=x.device, dtype=torch.uint8)
     if R:
-        _lib.call('hecka_block8_quantize', x.device, rows.data_ptr(), DTYPES[x.dtype], R, K, ld, act, codes.data_ptr(),
-                  scales.data_ptr(), _ptr(y))
+        _lib.call('hecka_block8_quantize', x.device, rows.data_ptr(), DTYPES[x.dtype], R, K, ld, act, _ptr(codes), _ptr(scales), _ptr(y))
+    if not keep:
+        return None, y
     return Rows8._made(codes, scales, x.shape, x.dtype), y
 
 
@@ -357,4 +360,7 @@ def linear(x, weight, bias=None, scale=1.0, bias_scale=1.0):
     _check_bias(what, bias, M, O)
     _same_device(what, x, weight, bias)
     _sizes(what, M, x.shape[-2], O, I)
+    if not torch.is_grad_enabled():      # nothing is kept for a backward pass
+        w = quantize_weight(weight, transposed=False)
+        return _product(_quantize(x)[0], w.codes, w.scales, M, O, I, _bias_rows(bias), float(scale), float(bias_scale), x.dtype)
     return _Linear8.apply(x, weight, _bias_rows(bias), float(scale), float(bias_scale))

@@ -200,7 +200,7 @@ class Linear(ParametersGroup):
         if self.compute == 'e4m3':
             y = block8.linear(x, W, b, self.scale, self.bias_scale)
         else:
-            y = (BatchedLinearCheckpoint if self.checkpoint else BatchedLinear).apply(x, W, b, self.scale, self.bias_scale)
+            y = (BatchedLinearCheckpoint if self.checkpoint and torch.is_grad_enabled() else BatchedLinear).apply(x, W, b, self.scale, self.bias_scale)
         if self.checkpoint and self.act_name in block8.ACTIVATIONS:
             return activation.checkpointed(self.act_name, y)
         return y if self.act is None else self.act(y)

@@ -549,7 +549,8 @@ int hecka_layernorm_bwd(const void* dy, const void* x, int dtype, const float* m
 #define HECKA_ACT_TANH 3
 #define HECKA_ACT_SIGMOID 4
 #define HECKA_ACT_CRATER 5   /* hyper/net/activation.py:10 */
-/* codes and scales of R rows of K elements, ld elements apart; act != NONE: also y [R, K] = act(x), in x's dtype. */
+/* codes and scales of R rows of K elements, ld elements apart; act != NONE: also y [R, K] = act(x), in x's dtype (codes and scales
+ * NULL: y alone). */
 int hecka_block8_quantize(const void* x, int dtype, long long R, int K, long long ld, int act, void* codes, void* scales,
                           void* y, void* stream);
 /* act == NONE: out [R, K] (dtype) = the values of the codes; else out = dy * act'(values), dy [R, K] (dtype). */

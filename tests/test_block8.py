@@ -206,6 +206,29 @@ def test_checkpointed_activation(name, dtype):
 
 
 @gpu
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
+def test_without_gradients_the_same_results_and_nothing_kept(dtype):
+    from hyper_amd import block8
+    from hyper_amd.layers import layer_norm
+    from hyper_amd.net.activation import checkpointed
+    x = features((2, 33, 300), dtype, 1).cuda().requires_grad_(True)
+    W, b = torch.randn(2, 70, 300, device='cuda', requires_grad=True), torch.randn(2, 70, device='cuda', requires_grad=True)
+    w1, b1 = torch.randn(2, 300, device='cuda', requires_grad=True), torch.randn(2, 300, device='cuda', requires_grad=True)
+    calls = [lambda n=n: checkpointed(n, x) for n in ('gelu', 'silu', 'tanh', 'sigmoid', 'crater')]
+    calls += [lambda: block8.linear(x, W, b), lambda: block8.linear(x[0], W, b, scale=0.5), lambda: layer_norm(x, w1, b1), lambda: layer_norm(x)]
+    for call in calls:
+        y = call()
+        with torch.no_grad():
+            z = call()
+        assert y.requires_grad and not z.requires_grad and torch.equal(y.detach(), z)
+        with torch.inference_mode():
+            assert torch.equal(call(), z)
+    v = x.detach().transpose(1, 2)
+    assert torch.equal(checkpointed('gelu', v), checkpointed('gelu', v.contiguous()))
+    assert checkpointed('gelu', x.detach()[:, :0]).shape == (2, 0, 300)
+
+
+@gpu
 def test_checkpointed_activation_keeps_bytes_and_takes_extremes():
     from hyper_amd.net.activation import checkpointed
     x = torch.randn(64, 4096, device='cuda', requires_grad=True)
@@ -495,6 +518,8 @@ def test_refusals_without_a_gpu():
     assert L.hecka_block8_quantize(p, 0, 1, 8, 8, 1, p, p, None, None) == -1
     assert L.hecka_block8_quantize(p, 0, 1, 8, 8, 6, p, p, p, None) == -1
     assert L.hecka_block8_quantize(p, 0, 1, 8, 8, 0, odd, p, None, None) == -1
+    assert L.hecka_block8_quantize(p, 0, 1, 8, 8, 0, None, None, None, None) == -1
+    assert L.hecka_block8_quantize(p, 0, 1, 8, 8, 1, p, None, p, None) == -1
     assert L.hecka_block8_values(p, p, None, 0, 1, 8, 1, p, None) == -1
     assert L.hecka_block8_values(p, p, None, 0, 0, 8, 0, p, None) == -1
     assert L.hecka_block8_weight(p, 0, 1, 8, 8, 64, p, p, p, None, None) == -1
