@@ -97,9 +97,10 @@ __device__ __forceinline__ void store_tile(const f32x4v (&acc)[S][S], const Piec
 //   a half step of 2^-8 of a bf16 result and 2^-11 of an fp16 one - so 16-bit results take it.
 // EXACT = true (fp32 results): the codes are widened to bf16 on their way out of LDS - exact - and the bf16 instruction
 //   adds their products in fp32 (1.4e-7 at K = 8192), at half the rate.
-// Bound by the matrix instructions: 256 x 256 tiles reach 2.6 PF (fp8) and 1.36 - 1.41 PF (widened) at 8192^3, where a library's
-// plain products reach 2.70 and 1.41; 2048 x 8192 x 8192 2.25 / 1.39 PF (256 workgroups, one round: the first loads and the last
-// stores hide behind nothing).  Four waves of 128 x 128 outputs each: 256 sums a lane leave every fragment read from LDS eight
+// Bound by the matrix instructions at the clock that the power leaves them (zeros run a fifth faster than random values), and by LDS
+// beside them: a step's 64 KB written and 128 KB read take three quarters of the time of its products.  256 x 256 tiles reach
+// 2.42 - 2.64 PF (fp8) and 1.31 - 1.40 PF (widened) at 8192^3, where a library's plain products reach 2.70 - 3.16 and 1.41 - 1.58; 2048 x
+// 8192 x 8192 2.25 / 1.39 PF (256 workgroups, one round: the first loads and the last stores hide behind nothing).  Four waves of 128 x 128 outputs each: 256 sums a lane leave every fragment read from LDS eight
 // products, and one workgroup a CU.  128 x 128 tiles (1.47 PF at best) where those are too few for the chip (linear_plan).
 // ------------------------------------------------------------------------------------------------------------------
 template <bool EXACT> struct Raw { typedef i32x8 type; };
@@ -442,9 +443,10 @@ __global__ __launch_bounds__(64 * W) void block8_token_kernel(const T* __restric
 // LDS rows hold units of 16 columns (32 bytes); unit u of row n sits at u ^ (n & 7): a transposing read takes one unit of
 // sixteen rows, eight of which lie on different banks.
 // Few tiles (small O x I): the rows are cut into pieces by blockIdx.y, whose sums a second kernel adds up in order.
-// 8 x 4096 rows, 2048 x 2048: fp32 607 us (three products each: 1.36 PF), fp16 431 us (1.28 PF), bf16 284 us (0.97 PF; a plain library
-// product 1.41).  fp32 and fp16 are bound by the matrix instructions; bf16 by LDS beside them: a step's 64 KB written and 128 KB
-// read are three quarters of the time of its products, and the staging's vector instructions share the issue slots.
+// 8192^3: fp32 1.34 PF (three products each), fp16 1.37, bf16 1.16 (a library's a^T b 1.06 - 1.17); 8 x 4096 rows, 2048 x 2048: fp32 607 -
+// 700 us, fp16 431 us, bf16 284 us.  fp32 and fp16 are bound by the matrix instructions at the clock that the power leaves them (fp32 values
+// that fit one term: 585 us); bf16 by LDS beside them: a step's 64 KB written and 128 KB read are three quarters of the time of its
+// products, and the staging's vector instructions share the issue slots.
 // ------------------------------------------------------------------------------------------------------------------
 template <class T, int TERMS, int B, bool WHOLE>
 __global__ __launch_bounds__(256) void block8_wgrad_kernel(
