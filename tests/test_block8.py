@@ -453,6 +453,35 @@ def test_far_rows_of_a_large_checkpoint():
 
 
 @gpu
+def test_far_outputs_and_far_weights():
+    """Results and gradients of more than 2^31 elements, and weights of as many: their last rows."""
+    from hyper_amd import block8
+    N, O, I, n = 140000, 16384, 40, 5
+    x, W, dy = whole((1, n, I), 1).bfloat16().cuda(), whole((1, O, I), 2).cuda(), whole((1, n, O), 3).bfloat16().cuda()
+    big = torch.zeros(1, N, I, device='cuda', dtype=torch.bfloat16)
+    big[:, -n:] = x
+    x, big = x.requires_grad_(True), big.requires_grad_(True)
+    W.requires_grad_(True)
+    y, want = block8.linear(big, W), block8.linear(x, W)
+    assert y.numel() > 2 ** 31 and torch.equal(y[:, -n:], want) and float(y[:, :-n].detach().amax()) == 0
+    far = torch.zeros_like(y)
+    far[:, -n:] = dy
+    dx, dW = torch.autograd.grad(y, (big, W), far)
+    wx, wW = torch.autograd.grad(want, (x, W), dy)
+    assert torch.equal(dx[:, -n:], wx) and float(dx[:, :-n].abs().max()) == 0 and torch.equal(dW, wW)
+    del y, far, dx, big
+    O, I = 131200, 16384
+    W = torch.zeros(1, O, I, device='cuda', dtype=torch.bfloat16)
+    W[:, -n:] = whole((1, n, I), 4).bfloat16().cuda()
+    w, few = block8.quantize_weight(W), block8.quantize_weight(W[:, -128:].contiguous())
+    assert w.codes.numel() > 2 ** 31 and torch.equal(w.codes[:, -n:], few.codes[:, -n:])
+    for rows in (1, 20):
+        x = whole((1, rows, I), 5).bfloat16().cuda()
+        y = block8.linear(x, w)
+        assert torch.equal(y[:, :, -128:], block8.linear(x, few)) and float(y[:, :, :-n].abs().max()) == 0
+
+
+@gpu
 def test_empty_batches():
     from hyper_amd import block8
     x = torch.zeros(2, 0, 30, device='cuda', requires_grad=True)

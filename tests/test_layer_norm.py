@@ -151,6 +151,25 @@ def test_shared_weight_missing_parts_and_strides():
 
 
 @gpu
+def test_rows_past_two_to_the_thirty_one_elements():
+    from hyper_amd.layers import layer_norm
+    R, D, n = 131200, 16384, 3
+    x, dy, w, b = data(1, n, D, torch.bfloat16, 6)
+    w, b = w[0].clone().requires_grad_(True), b[0].clone().requires_grad_(True)
+    far, fdy = torch.zeros(R, D, device='cuda', dtype=torch.bfloat16), torch.zeros(R, D, device='cuda', dtype=torch.bfloat16)
+    far[-n:], fdy[-n:] = x[0], dy[0]
+    x, far = x[0].requires_grad_(True), far.requires_grad_(True)
+    y, want = layer_norm(far, w, b), layer_norm(x, w, b)
+    assert y.numel() > 2 ** 31 and torch.equal(y[-n:], want) and torch.equal(y[0], b.bfloat16())
+    got, ref = torch.autograd.grad(y, (far, w, b), fdy), torch.autograd.grad(want, (x, w, b), dy[0])
+    assert torch.equal(got[0][-n:], ref[0]) and float(got[0][:-n].abs().max()) == 0
+    # the sums over rows: n terms each (the other rows' are zeros), added in another order
+    xh = (x.detach().double() - x.detach().double().mean(-1, keepdim=True)) / x.detach().double().std(-1, correction=0, keepdim=True)
+    for g, r, m in zip(got[1:], ref[1:], ((dy[0].double() * xh).abs().sum(0), dy[0].double().abs().sum(0))):
+        assert bool(((g - r).abs() <= 2 * n * 2.0 ** -24 * m.detach()).all())
+
+
+@gpu
 def test_gradient_against_differences():
     from hyper_amd.layers import layer_norm
     x, dy, w, b = data(2, 3, 24, torch.float32, 7)
