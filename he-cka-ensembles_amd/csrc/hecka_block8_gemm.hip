@@ -353,9 +353,9 @@ __global__ __launch_bounds__(256) void block8_join_kernel(const float* __restric
 // reads 32 codes per lane and row, a block ahead, and makes the codes of x for its blocks by itself (the same codes as
 // hecka_block8_quantize: 32 elements per lane, the maximum over the four lanes of a row).  All products in bf16, exact.
 // The W waves' sums are added in order.
-// 8 x 4096 x 4096, weights from HBM: 39 us, 3.4 TB/s of codes (32 us out of the last-level cache); 1 x 4096 x 4096 11 us.  Bound by the
-// memory's latency under load: a start elsewhere in K for every workgroup changes nothing, two blocks ahead cost registers and with
-// them waves (58 us).
+// 8 x 4096 x 4096, weights from HBM: 33 us, 4.0 TB/s of codes; 1 x 4096 x 4096 8.4 us; sixteen rows, 1 x 8192 x 8192, 23 us.  A kernel that
+// only reads the codes, in this order, takes 26 us of the 33 (24 in any order); the rest is work on them that the loads do not
+// cover.  A start elsewhere in K for every workgroup changes nothing, nor do two blocks ahead (34 us).
 // ------------------------------------------------------------------------------------------------------------------
 template <class T, int NT, int W>
 __global__ __launch_bounds__(64 * W) void block8_token_kernel(const T* __restrict__ x, long long xstride, int N, int K,
@@ -386,8 +386,13 @@ __global__ __launch_bounds__(64 * W) void block8_token_kernel(const T* __restric
       c[i][0] = *reinterpret_cast<const i32x4*>(pw[i] + (long long)kb * kBlock);
       c[i][1] = *reinterpret_cast<const i32x4*>(pw[i] + (long long)kb * kBlock + 16);
     }
+    if ((kb + 1) * kBlock <= K) {      // a whole block: no guards, whose branches for every piece cost a sixth of the time
 #pragma unroll
-    for (int j = 0; j < PX; ++j) px[j] = load_piece(x, kb * kBlock + g * 32 + j * Piece<T>::N, K);
+      for (int j = 0; j < PX; ++j) __builtin_memcpy(&px[j], x + kb * kBlock + g * 32 + j * Piece<T>::N, 16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < PX; ++j) px[j] = load_piece(x, kb * kBlock + g * 32 + j * Piece<T>::N, K);
+    }
     sb = ws[kb];
   };
   f32x4v acc[NT];
@@ -764,8 +769,9 @@ static int token_run(const void* x, long long xstride, int M, int N, int K, cons
                                                                            (const unsigned char*)ws, O, bias, bstride, alpha, beta, (T*)y)
   // Sixteen weight rows a wave where that makes few waves, 32 otherwise (a workgroup reads all of x, and makes its codes); K is
   // shared out to as many waves as fill the chip, two blocks each at least where there are many.  Measured (bf16, weights from HBM):
-  // 8 x 4096 x 4096, one row, 40 us with 32 rows x 4 waves, 55 us with 16 x 4; 1 x 4096 x 4096 11 us with 16 x 8, 17 us with 32 x 4;
-  // 1 x 8192 x 8192, sixteen rows, 29 us with 32 x 8, 35 us with 16 x 8; 1 x 1000 x 8192 12 us with 16 x 16, 23 us with 16 x 4.
+  // 8 x 4096 x 4096, one row, 33 us with 32 rows x 4 waves, 34 us with 32 x 8, 37 us with 16 x 4; sixteen rows 43, 45 and 56 us; 1 x 8192 x
+  // 8192, sixteen rows, 23 us with 32 x 8, 30 us with 16 x 8.  With guarded loads: 1 x 4096 x 4096 11 us with 16 x 8, 17 us with 32 x 4;
+  // 1 x 1000 x 8192 12 us with 16 x 16, 23 us with 16 x 4.
   const long long rows16 = (long long)M * cdiv(O, 16);
   const int nblk = row_blocks(K);
   if (rows16 >= 512) {
