@@ -33,7 +33,9 @@ __device__ __forceinline__ void load_lds4(const void* p, unsigned base) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
                :: "s"(__builtin_amdgcn_readfirstlane(base)), "v"(p) : "memory", "m0");
 }
-__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// until LEFT of the loads are under way at most (they end in their order)
+template <int LEFT>
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(LEFT) : "memory"); }
 __device__ __forceinline__ i32x4 buffer_of(const void* p) {      // raw buffer over the 2 GiB from p on
   const unsigned long long a = (unsigned long long)p;
   return i32x4{__builtin_amdgcn_readfirstlane((int)(unsigned)a), __builtin_amdgcn_readfirstlane((int)((a >> 32) & 0xffff)), 0x7fffffff, 0x00020000};
@@ -88,8 +90,8 @@ __device__ __forceinline__ void store_tile(const f32x4v (&acc)[S][S], const Piec
 // ------------------------------------------------------------------------------------------------------------------
 // y[m][n][o] = alpha sum_k x8[m][n][k] w8[m][o][k] + beta bias[m][o]
 //
-// A workgroup of WO x WN waves owns BO x BN outputs; per step, 128 codes (one block) of each of its rows come straight from
-// memory into LDS (no registers), one step ahead of the products.  LDS rows are 128 bytes; the 16-byte piece c of row r sits
+// A workgroup of four waves owns B x B outputs; per step, 128 codes (one block) of each of its rows come straight from memory into LDS
+// (no registers), STAGES - 1 steps ahead of the products: one, or three (linear_run).  LDS rows are 128 bytes; the 16-byte piece c of row r sits
 // at piece c ^ (r & 7), so that the sixteen rows which a fragment read touches fall on different banks.
 // The weights are the first operand, so that a lane ends up with four neighbouring outputs of one row.
 // EXACT = false: the scaled fp8 instruction takes both scales as bytes.  It adds groups of eight products aligned to the
@@ -137,13 +139,13 @@ __device__ __forceinline__ void mul_bf16(f32x4v& c, i32x4 a, i32x4 b) {
 __device__ __forceinline__ void mfma_ready() { asm volatile("s_nop 1"); }
 __device__ __forceinline__ void mfma_settle() { asm volatile("s_nop 15\n\ts_nop 15"); }
 
-template <class T, bool EXACT, int B>
+template <class T, bool EXACT, int B, int STAGES>
 __global__ __launch_bounds__(256) void block8_linear_kernel(
     const unsigned char* __restrict__ x, const unsigned char* __restrict__ xs, long long xstride, long long xsstride,
     const unsigned char* __restrict__ w, const unsigned char* __restrict__ ws, int N, int O, int allblk, int share,
     const float* __restrict__ bias, long long bstride, float alpha, float beta, T* __restrict__ y, int tiles_n, int tiles_o) {
   constexpr int TO = B / 32, TN = B / 32, U = EXACT ? 2 : 1, SYNC = TO / 2, L = B / 32, STAGE = 2 * B * kBlock;
-  __shared__ __attribute__((aligned(1024))) unsigned char sm[2][STAGE];
+  __shared__ __attribute__((aligned(1024))) unsigned char sm[STAGES][STAGE];
   __shared__ unsigned sc[2][2 * B];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wo = wave & 1, wn = wave >> 1, l16 = lane & 15, g = lane >> 4;
@@ -197,7 +199,7 @@ __global__ __launch_bounds__(256) void block8_linear_kernel(
   typedef typename Raw<EXACT>::type raw_t;
   const int swz = (g ^ (l16 & 7)) * 16, flip = (swz & 64) ? -64 : 64;
   auto raw = [&](int kb, int u, int row) {
-    const unsigned char* at = sm[kb & 1] + (row + l16) * kBlock + swz;
+    const unsigned char* at = sm[kb & (STAGES - 1)] + (row + l16) * kBlock + swz;
     if constexpr (EXACT) return *reinterpret_cast<const i32x4*>(at + u * flip);
     else return __builtin_shufflevector(*reinterpret_cast<const i32x4*>(at), *reinterpret_cast<const i32x4*>(at + flip), 0, 1, 2, 3, 4, 5, 6, 7);
   };
@@ -223,7 +225,7 @@ __global__ __launch_bounds__(256) void block8_linear_kernel(
   auto unit = [&](int kb, int u, const Unit& c, Unit& n) {
     const bool turn = u == U - 1;      // the last reads of this step's codes
     const int nkb = turn ? kb + 1 : kb, nu = turn ? 0 : u + 1;
-    const int far = kb + 2 < nblk ? kb + 2 : nblk - 1;
+    const int far = kb + STAGES < nblk ? kb + STAGES : nblk - 1;
     raw_t aw[TO], nx[TN];
     aw[0] = c.aw;
 #pragma unroll
@@ -235,7 +237,7 @@ __global__ __launch_bounds__(256) void block8_linear_kernel(
         for (int k = SYNC; k < TO; ++k) aw[k] = raw(kb, u, rw0 + k * 16);
       }
       if (i == SYNC && turn) {
-        wait_loads();      // step kb + 1, under way since the last turn
+        wait_loads<(STAGES - 2) * 2 * L>();      // step kb + 1: behind it STAGES - 2 steps are under way, of 2 L loads at least
         __syncthreads();   // and nobody reads step kb any more
       }
       if (i >= SYNC) {
@@ -259,13 +261,13 @@ __global__ __launch_bounds__(256) void block8_linear_kernel(
         const int j = e % TN;
         if constexpr (EXACT) mul_bf16<B == 256>(acc[i][j], half4(fw, e / TN), half4(c.fx[j], e / TN));
         else mul_fp8<B == 256>(acc[i][j], fw, c.fx[j], c.sw, c.sx[j]);
-        // step kb + 2 into the freed buffer: the loads one by one between the products, because a load that finds the queue full
+        // step kb + STAGES into the freed buffer: the loads one by one between the products, because a load that finds the queue full
         // holds up its wave
         if (turn && i >= SYNC) {
           constexpr int SLOTS = (TO - SYNC) * U * TN;
           const int slot = (i - SYNC) * U * TN + e;
 #pragma unroll
-          for (int part = slot * LOADS / SLOTS; part < (slot + 1) * LOADS / SLOTS; ++part) fetch(part, far, kb & 1);
+          for (int part = slot * LOADS / SLOTS; part < (slot + 1) * LOADS / SLOTS; ++part) fetch(part, far, kb & (STAGES - 1));
         }
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -275,10 +277,11 @@ __global__ __launch_bounds__(256) void block8_linear_kernel(
   };
 
 #pragma unroll
-  for (int part = 0; part < LOADS; ++part) fetch(part, 0, 0);
+  for (int step = 0; step < STAGES; ++step) {
 #pragma unroll
-  for (int part = 0; part < LOADS; ++part) fetch(part, nblk > 1 ? 1 : 0, 1);
-  wait_loads();
+    for (int part = 0; part < LOADS; ++part) fetch(part, step < nblk ? step : nblk - 1, step);
+  }
+  wait_loads<(STAGES - 1) * 2 * L>();
   __syncthreads();
   Unit p, q;
   p.sw = scale_w(0);
@@ -295,7 +298,7 @@ __global__ __launch_bounds__(256) void block8_linear_kernel(
     unit(EXACT ? kb >> 1 : kb + 1, U - 1, q, p);
   }
   if (kb < nblk * U) unit(kb, 0, p, q);
-  wait_loads();      // the last steps' repeated loads write LDS: not past the end of the workgroup
+  wait_loads<0>();      // the last steps' repeated loads write LDS: not past the end of the workgroup
   if constexpr (B == 256) {
     mfma_settle();
 #pragma unroll
@@ -715,20 +718,23 @@ __global__ __launch_bounds__(256) void block8_slabs_kernel(const float* __restri
 
 static int cdiv(int a, int b) { return (a + b - 1) / b; }
 static constexpr int kLinearFill = 256, kLinearLeast = 8;
+// rounds of the chip's 256 CUs that M matrices of R x C take in tiles of 256 x 256
+static long long large_rounds(int M, int R, int C) { return ((long long)M * cdiv(R, 256) * cdiv(C, 256) + 255) / 256; }
 
-// 256 x 256 outputs a workgroup where that gives most of the chip's CUs one (128 x 128 ones, two a CU, load twice as much), else 128 x
-// 128, and where those leave half of the chip idle the blocks of K are shared out, eight at least to each, their sums joined by a
-// second launch.  Measured (bf16 / fp32 results), large tiles against small: 1 x 2048 x 8192 x 4096, 256 large ones, 64 / 113 against 115 /
-// 132 us; 1 x 1280 x 8192 x 4096, 160, 58 / 107 against 87 / 99; 1 x 1024 x 8192 x 4096, 128, 57 / 107 against 63 / 72; 5 x 1000 x 1000 x
-// 1000, 80, 24 / 38 against 22 / 23; 12 x 1024 x 1024 x 1024, 192, 27 / 41 against 34 / 35.  Shares: 1 x 64 x 8192 x 8192 48 / 73 us whole, 24 / 30 us in four shares, 31 / 30 us in eight; 1 x 64 x 1024 x 8192 41 / 73 us whole, 15 /
+// 256 x 256 outputs a workgroup, one a CU, or 128 x 128, two a CU: a round of 256 large ones takes as long as about 512 small ones of fp8
+// products and 900 of widened codes.  Where small ones leave half of the chip idle the blocks of K are shared out, eight at least to
+// each, their sums joined by a second launch.  Measured (bf16 / fp32 results), large tiles against small: 1 x 2048 x 8192 x 4096, 256
+// large or 1024 small ones, 65 / 111 against 111 / 126 us; 1 x 1024 x 8192 x 4096, 128 or 512, 56 / 104 against 63 / 68; 5 x 1000 x 1000 x
+// 1000, 80 or 320, 24 / 38 against 21 / 23; 8 x 300 x 4096 x 4096, 256 or 768, 60 / 115 against 80 / 103; 10 x 300 x 4096 x 784, 320 or 960,
+// 44 / 68 against 38 / 36.  Shares: 1 x 64 x 8192 x 8192 48 / 73 us whole, 24 / 30 us in four shares, 31 / 30 us in eight; 1 x 64 x 1024 x 8192 41 / 73 us whole, 15 /
 // 19 us in eight; 1 x 512 x 4096 x 4096 28 / 45 us whole, 27 / 35 us in two, 38 / 35 us in four; shares of four blocks: 1 x 256 x 4096 x
 // 4096 32 us against 22.
 struct LinearPlan { int tile, splits, share; };
 static LinearPlan linear_plan(int M, int N, int O, int nblk, bool exact) {
   LinearPlan p{256, 1, (nblk + 3) & ~3};
-  if ((long long)M * cdiv(N, 256) * cdiv(O, 256) >= (exact ? 224 : 112)) return p;
-  p.tile = 128;
   const long long tiles = (long long)M * cdiv(N, 128) * cdiv(O, 128), s = kLinearFill / tiles;
+  if (large_rounds(M, N, O) * (exact ? 900 : 512) <= tiles) return p;
+  p.tile = 128;
   if (s > 1) {
     const int most = nblk / kLinearLeast > 1 ? nblk / kLinearLeast : 1;
     p.splits = (int)(s < most ? s : most);
@@ -745,18 +751,25 @@ template <class T, bool EXACT>
 static int linear_run(const LinearPlan& p, const void* x, const void* xs, long long xstride, long long xsstride, const void* w,
                       const void* ws, int M, int N, int O, int nblk, const float* bias, long long bstride, float alpha, float beta,
                       void* y, int y_members, float* slabs, hipStream_t st) {
-#define HECKA_LINEAR(TO, B, BIAS, OUT) \
-  block8_linear_kernel<TO, EXACT, B><<<dim3((unsigned)(M * cdiv(N, B) * cdiv(O, B)), p.splits), 256, 0, st>>>( \
+#define HECKA_LINEAR(TO, B, STAGES, BIAS, OUT) \
+  block8_linear_kernel<TO, EXACT, B, STAGES><<<dim3((unsigned)(M * cdiv(N, B) * cdiv(O, B)), p.splits), 256, 0, st>>>( \
       (const unsigned char*)x, (const unsigned char*)xs, xstride, xsstride, (const unsigned char*)w, (const unsigned char*)ws, N, O, \
       nblk, p.share, BIAS, bstride, alpha, beta, OUT, cdiv(N, B), cdiv(O, B))
+  // Long sums of fp8 products in 128 x 128 tiles that have a CU to themselves: three steps ahead (1 x 1024 x 4096 x 4096 28 us, one ahead 32;
+  // 1 x 64 x 8192 x 8192 22 us, 24); with widened codes and in short sums the start costs what that saves (5 x 300 x 1200 x 784 bf16 10.2 us, 10.0;
+  // fp32 14.9, 14.2).
+  constexpr int FAR = EXACT ? 2 : 4;
+  const bool far = FAR > 2 && p.share >= 16 && (long long)M * cdiv(N, 128) * cdiv(O, 128) * p.splits <= 256;
   if (p.splits > 1 || y_members < M) {
-    if (p.tile == 256) HECKA_LINEAR(float, 256, nullptr, slabs);
-    else HECKA_LINEAR(float, 128, nullptr, slabs);
+    if (p.tile == 256) HECKA_LINEAR(float, 256, 2, nullptr, slabs);
+    else if (far) HECKA_LINEAR(float, 128, FAR, nullptr, slabs);
+    else HECKA_LINEAR(float, 128, 2, nullptr, slabs);
     const long long n = (long long)N * O, blocks = (n + 1023) / 1024;
     block8_join_kernel<T><<<dim3((unsigned)(blocks < 2048 ? blocks : 2048), y_members), 256, 0, st>>>(
         slabs, y_members < M ? p.splits * M : p.splits, n, O, bias, bstride, beta, (T*)y);
-  } else if (p.tile == 256) HECKA_LINEAR(T, 256, bias, (T*)y);
-  else HECKA_LINEAR(T, 128, bias, (T*)y);
+  } else if (p.tile == 256) HECKA_LINEAR(T, 256, 2, bias, (T*)y);
+  else if (far) HECKA_LINEAR(T, 128, FAR, bias, (T*)y);
+  else HECKA_LINEAR(T, 128, 2, bias, (T*)y);
 #undef HECKA_LINEAR
   return check_launch("block8_linear");
 }
@@ -793,17 +806,17 @@ static int token_run(const void* x, long long xstride, int M, int N, int K, cons
 
 struct WgradPlan { int tile, to, ti, splits, rows; };
 static WgradPlan wgrad_plan(int M, int N, int O, int I, bool whole) {
-  // 256 x 256 tiles, one workgroup per CU, where they fill three quarters of the chip and dy's rows are whole 16-byte pieces (guarded
-  // loads, for which 256 x 256 leaves no registers, otherwise); else 128 x 128 tiles, two per CU, and where those are too few the
-  // rows in pieces of 256 at least.  Measured (bf16 / fp32): 4 x 2000 x 2000 x 2000, 256 large tiles, 82 / 177 us, 107 / 208 us with
-  // small ones; 2 x 1024 x 2048 x 2048, 128 large tiles, 53 / 75 us cut in two, 32 / 55 us with 512 small ones; 1 x 65536 x 256 x 512 small
-  // tiles 56 / 79 us, large ones, cut into many pieces, 72 / 92 us.
+  // 256 x 256 tiles, one workgroup per CU, where dy's rows are whole 16-byte pieces (guarded loads, for which 256 x 256 leaves no
+  // registers, otherwise) and a round of them does the work of 700 of 128 x 128, two per CU; where small ones are too few the rows in pieces
+  // of 256 at least.  Measured (bf16 / fp32): 4 x 2000 x 2000 x 2000, 256 large or 1024 small tiles, 82 / 177 against 107 / 208 us; 3 x 4096 x 2048
+  // x 2048, 192 or 768, 132 / 302 against 153 / 312; large ones cut into pieces, 2 x 1024 x 2048 x 2048, 53 / 75 against 32 / 55 us, 1 x
+  // 65536 x 256 x 512, 72 / 92 against 56 / 79.
   WgradPlan p{256, cdiv(O, 256), cdiv(I, 256), 1, cdiv(N, 64) * 64};
-  if (whole && (long long)M * p.to * p.ti >= 192 && O > 128 && I > 128) return p;
+  const long long tiles = (long long)M * cdiv(O, 128) * cdiv(I, 128), s = tiles >= 512 ? 1 : 512 / tiles;
+  if (whole && large_rounds(M, O, I) * 700 <= tiles) return p;
   p.tile = 128;
   p.to = cdiv(O, 128);
   p.ti = cdiv(I, 128);
-  const long long tiles = (long long)M * p.to * p.ti, s = tiles >= 512 ? 1 : 512 / tiles;
   const int most = cdiv(N, 256);
   p.splits = (int)(s < most ? s : most);
   p.rows = cdiv(cdiv(N, p.splits), 64) * 64;

@@ -339,6 +339,24 @@ def test_shared_rows_and_their_gradient():
 
 @gpu
 @pytest.mark.parametrize('dtype', TYPES, ids=str)
+@pytest.mark.parametrize('shared', [False, True])
+@pytest.mark.parametrize('M,N,O,I', [(30, 400, 1000, 300), (30, 400, 300, 1000)])
+def test_large_tiles_with_ragged_edges(M, N, O, I, shared, dtype):
+    """Tiles of 256 x 256 in y and dW, or in dx (whose sum over the members they also write)."""
+    from hyper_amd import block8
+    x, W, b, dy = whole((N, I) if shared else (M, N, I), 1), whole((M, O, I), 2), whole((M, O), 3, 50), whole((M, N, O), 4)
+    xg, Wg, bg = x.to(dtype).cuda().requires_grad_(True), W.cuda().requires_grad_(True), b.cuda().requires_grad_(True)
+    y = block8.linear(xg, Wg, bg, scale=0.25, bias_scale=2.0)
+    dx, dW, db = torch.autograd.grad(y, (xg, Wg, bg), dy.to(dtype).cuda())
+    xd = x.float().expand(M, N, I)      # sums of whole numbers below 2^24: exact in fp32 as well
+    assert torch.equal(y.detach().cpu(), (0.25 * torch.bmm(xd, W.transpose(1, 2).contiguous()) + 2.0 * b[:, None]).to(dtype))
+    want = 0.25 * torch.bmm(dy, W)
+    assert torch.equal(dx.cpu(), (want.sum(0) if shared else want).to(dtype))
+    assert torch.equal(dW.cpu(), 0.25 * torch.bmm(dy.transpose(1, 2).contiguous(), xd)) and torch.equal(db.cpu(), 2.0 * dy.sum(1))
+
+
+@gpu
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
 @pytest.mark.parametrize('M,N,O,I', [(1, 64, 130, 5000), (2, 33, 71, 2100), (1, 17, 3, 8200), (1, 300, 8, 2048)])
 def test_long_sums_shared_out(M, N, O, I, dtype):
     """Few tiles and many blocks of K: the slabs' sum, its bias and rounding, and the same bits on every call."""
@@ -358,7 +376,7 @@ def test_long_sums_shared_out(M, N, O, I, dtype):
 @pytest.mark.parametrize('dtype', TYPES, ids=str)
 @pytest.mark.parametrize('M,N,O,I', [(3, 40, 50, 201), (2, 33, 4099, 35), (7, 1, 1, 1), (40, 700, 300, 129)])
 def test_gradient_of_shared_rows_is_rounded_once(M, N, O, I, dtype):
-    """The members' sum in fp32, also where the sum over outputs is long and shared out, or the tiles are large."""
+    """The members' sum in fp32, also where the sum over outputs is long and shared out."""
     from hyper_amd import block8
     x, W, dy = whole((N, I), 1), whole((M, O, I), 2), whole((M, N, O), 3)
     xg = x.to(dtype).cuda().requires_grad_(True)
