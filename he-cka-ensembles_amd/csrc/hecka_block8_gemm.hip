@@ -931,4 +931,115 @@ int hecka_block8_wgrad(const void* dy, int dtype, const void* x, const void* xsc
                                   : wgrad_run<F16, 2>(dy, x, xscales, xst, sst, M, N, O, I, alpha, beta, dW, db, (float*)ws, st);
 }
 
+// A layer's training step in two calls, each the launches above in their order: a small layer's time is its caller's.
+namespace {
+// the parts of a buffer, each at a multiple of 256 bytes
+struct Parts {
+  char* base;
+  size_t used;
+  void* take(size_t bytes, bool wanted = true) {
+    if (!wanted) return nullptr;
+    void* p = base + used;
+    used += (bytes + 255) & ~(size_t)255;
+    return p;
+  }
+};
+struct Kept { void *xc, *xs, *tc, *ts; };      // rows x; weights transposed
+struct Sizes {
+  size_t xc, xs, wc, ws, tc, ts, dc, ds;
+  Sizes(int M, int xm, int N, int O, int I) {
+    xc = (size_t)xm * N * row_blocks(I) * kBlock;
+    xs = (size_t)xm * N * scale_stride(I);
+    wc = (size_t)M * O * row_blocks(I) * kBlock;
+    ws = (size_t)M * row_blocks(O) * scale_stride(I);
+    tc = (size_t)M * I * row_blocks(O) * kBlock;
+    ts = (size_t)M * row_blocks(I) * scale_stride(O);
+    dc = (size_t)M * N * row_blocks(O) * kBlock;
+    ds = (size_t)M * N * scale_stride(O);
+  }
+};
+Kept kept_parts(const Sizes& z, Parts& p, bool need_dx, bool need_dw) {
+  Kept k;
+  k.xc = p.take(z.xc, need_dw);
+  k.xs = p.take(z.xs, need_dw);
+  k.tc = p.take(z.tc, need_dx);
+  k.ts = p.take(z.ts, need_dx);
+  return k;
+}
+}  // namespace
+
+size_t hecka_block8_train_bytes(int what, int M, int x_members, int N, int O, int I, int dtype, int need_dx, int need_dw) {
+  if (bad_type(dtype) || bad_sizes(M, N, O, I) || (x_members != M && x_members != 1)) return 0;
+  const Sizes z(M, x_members, N, O, I);
+  Parts p{nullptr, 0};
+  if (what == 0) {
+    kept_parts(z, p, need_dx, need_dw);
+  } else if (what == 1) {
+    p.take(z.xc, !need_dw);
+    p.take(z.xs, !need_dw);
+    p.take(z.wc);
+    p.take(z.ws);
+    p.take(hecka_block8_linear_workspace_bytes(M, N, O, I, M, dtype));
+  } else {
+    p.take(z.dc, need_dx);
+    p.take(z.ds, need_dx);
+    p.take(hecka_block8_linear_workspace_bytes(M, N, I, O, x_members, dtype), need_dx);
+    p.take(hecka_block8_wgrad_workspace_bytes(M, N, O, I), need_dw);
+  }
+  return p.used;
+}
+
+int hecka_block8_train_fwd(const void* x, int dtype, int x_members, long long ld, const void* W, int wdtype, long long mstride, int M, int N,
+                           int O, int I, const float* bias, long long bstride, float alpha, float beta, int need_dx, int need_dw, void* y,
+                           void* kept, size_t kept_bytes, void* ws, size_t ws_bytes, void* stream) {
+  if (bad_type(dtype) || bad_type(wdtype)) return fail(HECKA_EINVAL, "block8_train_fwd: unknown dtype%s");
+  if (bad_sizes(M, N, O, I)) return fail(HECKA_EINVAL, "%sblock8_train_fwd: bad size (N = %lld, O = %lld)", "", N, O);
+  if (x_members != M && x_members != 1) return fail(HECKA_EINVAL, "%sblock8_train_fwd: rows of %lld members for %lld", "", x_members, M);
+  const size_t most = hecka_block8_train_bytes(0, M, x_members, N, O, I, dtype, need_dx, need_dw);
+  if ((kept ? kept_bytes : 0) < most || (ws ? ws_bytes : 0) < hecka_block8_train_bytes(1, M, x_members, N, O, I, dtype, need_dx, need_dw))
+    return fail(HECKA_EWORKSPACE, "%sblock8_train_fwd: workspace too small (%lld bytes given)", "", (long long)ws_bytes);
+  const Sizes z(M, x_members, N, O, I);
+  Parts pk{(char*)kept, 0}, pw{(char*)ws, 0};
+  Kept k = kept_parts(z, pk, need_dx, need_dw);
+  if (!need_dw) {
+    k.xc = pw.take(z.xc);
+    k.xs = pw.take(z.xs);
+  }
+  void *wc = pw.take(z.wc), *wsc = pw.take(z.ws);
+  const size_t need = hecka_block8_linear_workspace_bytes(M, N, O, I, M, dtype);
+  int rc = hecka_block8_quantize(x, dtype, (long long)x_members * N, I, ld, HECKA_ACT_NONE, k.xc, k.xs, nullptr, stream);
+  if (!rc) rc = hecka_block8_weight(W, wdtype, M, O, I, mstride, wc, wsc, k.tc, k.ts, stream);
+  if (!rc)
+    rc = hecka_block8_linear(k.xc, k.xs, x_members, wc, wsc, M, N, O, I, bias, bstride, alpha, beta, y, dtype, M, need ? pw.take(need) : nullptr, need, stream);
+  return rc;
+}
+
+int hecka_block8_train_bwd(const void* dy, int dtype, int x_members, int M, int N, int O, int I, float alpha, float beta, int need_dx,
+                           int need_dw, const void* kept, size_t kept_bytes, void* dx, float* dW, float* db, void* ws, size_t ws_bytes,
+                           void* stream) {
+  if (bad_type(dtype)) return fail(HECKA_EINVAL, "block8_train_bwd: unknown dtype%s");
+  if (bad_sizes(M, N, O, I)) return fail(HECKA_EINVAL, "%sblock8_train_bwd: bad size (N = %lld, O = %lld)", "", N, O);
+  if (x_members != M && x_members != 1) return fail(HECKA_EINVAL, "%sblock8_train_bwd: rows of %lld members for %lld", "", x_members, M);
+  if (!dy || (dx && !need_dx) || (dW && !need_dw) || (db && !dW)) return fail(HECKA_EINVAL, "block8_train_bwd: null pointer, or a gradient whose codes were not kept%s");
+  if ((kept ? kept_bytes : 0) < hecka_block8_train_bytes(0, M, x_members, N, O, I, dtype, need_dx, need_dw) ||
+      (ws ? ws_bytes : 0) < hecka_block8_train_bytes(2, M, x_members, N, O, I, dtype, dx != nullptr, dW != nullptr))
+    return fail(HECKA_EWORKSPACE, "%sblock8_train_bwd: workspace too small (%lld bytes given)", "", (long long)ws_bytes);
+  const Sizes z(M, x_members, N, O, I);
+  Parts pk{(char*)const_cast<void*>(kept), 0}, pw{(char*)ws, 0};
+  const Kept k = kept_parts(z, pk, need_dx, need_dw);
+  int rc = 0;
+  if (dx) {
+    void *dc = pw.take(z.dc), *ds = pw.take(z.ds);
+    const size_t need = hecka_block8_linear_workspace_bytes(M, N, I, O, x_members, dtype);
+    void* slabs = need ? pw.take(need) : nullptr;
+    rc = hecka_block8_quantize(dy, dtype, (long long)M * N, O, O, HECKA_ACT_NONE, dc, ds, nullptr, stream);
+    if (!rc) rc = hecka_block8_linear(dc, ds, M, k.tc, k.ts, M, N, I, O, nullptr, 0, alpha, 0.f, dx, dtype, x_members, slabs, need, stream);
+  }
+  if (dW && !rc) {
+    const size_t need = hecka_block8_wgrad_workspace_bytes(M, N, O, I);
+    rc = hecka_block8_wgrad(dy, dtype, k.xc, k.xs, x_members, M, N, O, I, alpha, beta, dW, db, need ? pw.take(need) : nullptr, need, stream);
+  }
+  return rc;
+}
+
 }  // extern "C"

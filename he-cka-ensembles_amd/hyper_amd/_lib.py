@@ -105,6 +105,9 @@ SIGNATURES = {
     'hecka_block8_linear_workspace_bytes': (_sz, [_i, _i, _i, _i, _i, _i]),
     'hecka_block8_linear': (_i, [_vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _vp, _ll, ctypes.c_float, ctypes.c_float, _vp, _i, _i, _vp, _sz, _vp]),
     'hecka_block8_linear_token': (_i, [_vp, _i, _i, _vp, _vp, _i, _i, _i, _i, _vp, _ll, ctypes.c_float, ctypes.c_float, _vp, _vp]),
+    'hecka_block8_train_bytes': (_sz, [_i, _i, _i, _i, _i, _i, _i, _i, _i]),
+    'hecka_block8_train_fwd': (_i, [_vp, _i, _i, _ll, _vp, _i, _ll, _i, _i, _i, _i, _vp, _ll, ctypes.c_float, ctypes.c_float, _i, _i, _vp, _vp, _sz, _vp, _sz, _vp]),
+    'hecka_block8_train_bwd': (_i, [_vp, _i, _i, _i, _i, _i, _i, ctypes.c_float, ctypes.c_float, _i, _i, _vp, _sz, _vp, _vp, _vp, _vp, _sz, _vp]),
     'hecka_block8_wgrad_workspace_bytes': (_sz, [_i, _i, _i, _i]),
     'hecka_block8_wgrad': (_i, [_vp, _i, _vp, _vp, _i, _i, _i, _i, _i, ctypes.c_float, ctypes.c_float, _vp, _vp, _vp, _sz, _vp]),
     'hecka_combine_slice_blocked_f32': (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _ll, _ll, _i, _i, _vp, _vp]),

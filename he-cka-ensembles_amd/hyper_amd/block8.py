@@ -182,15 +182,19 @@ def dequantize(q, dtype=None):
     return _values(q, dtype)
 
 
+def _members_apart(W):
+    """W [M, O, I] with whole members: a member's slice of a flat parameter row is read in place."""
+    M, O, I = W.shape
+    return W.contiguous() if W.stride()[1:] != (I, 1) or (M > 1 and W.stride(0) < O * I) else W
+
+
 def quantize_weight(W, transposed=True):
     """W [M, O, I] as Weight8; transposed=False leaves out what only a backward pass reads."""
     _check(W, 'block8.quantize_weight')
     if W.dim() != 3 or 0 in W.shape:
         raise ValueError('block8.quantize_weight: needs [members, outputs, inputs] without zero sizes, got %s' % (tuple(W.shape),))
-    W = W.detach()
+    W = _members_apart(W.detach())
     M, O, I = W.shape
-    if W.stride()[1:] != (I, 1) or (M > 1 and W.stride(0) < O * I):      # a member's slice of a flat parameter row is read in place
-        W = W.contiguous()
     u8 = dict(device=W.device, dtype=torch.uint8)
     codes = torch.empty((M, O, row_blocks(I) * BLOCK), **u8)
     scales = torch.empty((M, row_blocks(O), scale_stride(I)), **u8)
@@ -218,17 +222,15 @@ def _bias_rows(b):
     return b if b is None or b.stride(1) == 1 else b.contiguous()
 
 
-def _product(q, codes, scales, M, O, I, bias, alpha, beta, dtype, total=False):
-    """[M, N, O]; total: its sum over the members [N, O] (no bias), added in fp32 and rounded once."""
+def _product(q, codes, scales, M, O, I, bias, alpha, beta, dtype):
     N = q.shape[-2]
-    y = torch.empty((N, O) if total else (M, N, O), device=q.device, dtype=dtype)
+    y = torch.empty((M, N, O), device=q.device, dtype=dtype)
     if y.numel():
-        ym = 1 if total else M
-        nbytes = _lib.lib().hecka_block8_linear_workspace_bytes(M, N, O, I, ym, DTYPES[dtype])
+        nbytes = _lib.lib().hecka_block8_linear_workspace_bytes(M, N, O, I, M, DTYPES[dtype])
         ws = torch.empty((nbytes // 4,), device=q.device, dtype=torch.float32) if nbytes else None
         _lib.call('hecka_block8_linear', q.device, q.codes.data_ptr(), q.scales.data_ptr(), 1 if len(q.shape) == 2 else M,
                   codes.data_ptr(), scales.data_ptr(), M, N, O, I, _ptr(bias), _bstride(bias), alpha, beta, y.data_ptr(), DTYPES[dtype],
-                  ym, _ptr(ws), nbytes)
+                  M, _ptr(ws), nbytes)
     return y
 
 
@@ -284,30 +286,49 @@ class _Linear8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, W, b, scale, bias_scale):
         M, O, I = W.shape
-        q, _ = _quantize(x)
-        w = quantize_weight(W, transposed=ctx.needs_input_grad[0])
-        y = _product(q, w.codes, w.scales, M, O, I, b, scale, bias_scale, x.dtype)
-        # tensors that autograd frees with the graph; no saved tensor where no gradient will ask for it
-        ctx.save_for_backward(*((q.codes, q.scales) if ctx.needs_input_grad[1] else (None, None)), w.codes_t, w.scales_t)
-        ctx.cfg = (x.shape, x.dtype, W.shape, W.dtype, b is not None, scale, bias_scale)
+        N, xm, t = x.shape[-2], 1 if x.dim() == 2 else M, DTYPES[x.dtype]
+        need_dx, need_dw, _ = ctx.needs_input_grad[:3]
+        y = torch.empty((M, N, O), device=x.device, dtype=x.dtype)
+        kept = None
+        if N:
+            rows, _, ld = _rows(x)
+            W = _members_apart(W)
+            size = _lib.lib().hecka_block8_train_bytes
+            nk, nw = size(0, M, xm, N, O, I, t, need_dx, need_dw), size(1, M, xm, N, O, I, t, need_dx, need_dw)
+            if nk:
+                kept = torch.empty((nk,), device=x.device, dtype=torch.uint8)
+            ws = torch.empty((nw,), device=x.device, dtype=torch.uint8)
+            _lib.call('hecka_block8_train_fwd', x.device, rows.data_ptr(), t, xm, ld, W.data_ptr(), DTYPES[W.dtype], W.stride(0), M, N, O, I,
+                      _ptr(b), _bstride(b), scale, bias_scale, need_dx, need_dw, y.data_ptr(), _ptr(kept), nk, ws.data_ptr(), nw)
+        # a tensor that autograd frees with the graph; only the codes that a gradient will ask for
+        ctx.save_for_backward(kept)
+        ctx.cfg = (x.shape, x.dtype, W.shape, W.dtype, b is not None, scale, bias_scale, need_dx, need_dw)
         return y
 
     @staticmethod
     @_lib.first_order
     def backward(ctx, dy):
-        codes, scales, codes_t, scales_t = ctx.saved_tensors
-        xshape, xdtype, (M, O, I), wdtype, has_bias, scale, bias_scale = ctx.cfg
+        kept, = ctx.saved_tensors
+        xshape, xdtype, (M, O, I), wdtype, has_bias, scale, bias_scale, need_dx, need_dw = ctx.cfg
+        N, xm, t = dy.shape[1], 1 if len(xshape) == 2 else M, DTYPES[xdtype]
         dy = dy.contiguous()
         dx = dW = db = None
-        want_b = has_bias and ctx.needs_input_grad[2]
-        if ctx.needs_input_grad[0]:
-            dx = _product(_quantize(dy)[0], codes_t, scales_t, M, I, O, None, scale, 0.0, xdtype, total=len(xshape) == 2)
-        if ctx.needs_input_grad[1]:
-            dW, db = _weight_grad(dy, Rows8._made(codes, scales, xshape, xdtype), scale, bias_scale, want_b)
-            dW = dW.to(wdtype)
+        want_x, want_w, want_b = ctx.needs_input_grad[0], ctx.needs_input_grad[1], has_bias and ctx.needs_input_grad[2]      # may be fewer now
+        if want_x:
+            dx = torch.empty(xshape, device=dy.device, dtype=xdtype)
+        if want_w:
+            dW = torch.empty((M, O, I), device=dy.device, dtype=torch.float32)
+            db = torch.empty((M, O), device=dy.device, dtype=torch.float32) if want_b else None
         elif want_b:
             db = _bias_grad(dy, bias_scale)
-        return dx, dW, db, None, None
+        if N == 0:
+            return dx, dW.zero_().to(wdtype) if want_w else None, db.zero_() if want_b else None, None, None
+        if want_x or want_w:
+            nw = _lib.lib().hecka_block8_train_bytes(2, M, xm, N, O, I, t, want_x, want_w)
+            ws = torch.empty((nw,), device=dy.device, dtype=torch.uint8) if nw else None
+            _lib.call('hecka_block8_train_bwd', dy.device, dy.data_ptr(), t, xm, M, N, O, I, scale, bias_scale, need_dx, need_dw, kept.data_ptr(),
+                      kept.numel(), _ptr(dx), _ptr(dW), _ptr(db) if want_w else None, _ptr(ws), nw)
+        return dx, dW.to(wdtype) if want_w else None, db, None, None
 
 
 def _check_bias(what, b, M, O):

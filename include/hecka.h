@@ -576,6 +576,18 @@ int hecka_block8_linear_token(const void* x, int dtype, int x_members, const voi
 size_t hecka_block8_wgrad_workspace_bytes(int M, int N, int O, int I);
 int hecka_block8_wgrad(const void* dy, int dtype, const void* x, const void* xscales, int x_members, int M, int N, int O, int I,
                        float alpha, float beta, float* dW, float* db, void* ws, size_t ws_bytes, void* stream);
+/* A layer's training step in two calls, each the launches above one after the other: forward codes of x [x_members, N, I] (dtype, rows
+ * ld apart) and W [M, O, I] (wdtype, members mstride apart), y; backward dx (of x_members; their sum where 1), dW, db from dy [M, N, O].
+ * `kept` (256-byte aligned) carries the codes that the wanted gradients need from one to the other; the same need_dx / need_dw in
+ * both; dx, dW and db may be NULL, db only with dW.  hecka_block8_train_bytes: what = 0 kept, 1 the forward's workspace, 2 the backward's
+ * (need_dx, need_dw: of the gradients asked for). */
+size_t hecka_block8_train_bytes(int what, int M, int x_members, int N, int O, int I, int dtype, int need_dx, int need_dw);
+int hecka_block8_train_fwd(const void* x, int dtype, int x_members, long long ld, const void* W, int wdtype, long long mstride, int M, int N,
+                           int O, int I, const float* bias, long long bstride, float alpha, float beta, int need_dx, int need_dw, void* y,
+                           void* kept, size_t kept_bytes, void* ws, size_t ws_bytes, void* stream);
+int hecka_block8_train_bwd(const void* dy, int dtype, int x_members, int M, int N, int O, int I, float alpha, float beta, int need_dx,
+                           int need_dw, const void* kept, size_t kept_bytes, void* dx, float* dW, float* db, void* ws, size_t ws_bytes,
+                           void* stream);
 
 #ifdef __cplusplus
 }

@@ -386,6 +386,32 @@ def test_gradient_of_shared_rows_is_rounded_once(M, N, O, I, dtype):
 
 @gpu
 @pytest.mark.parametrize('dtype', TYPES, ids=str)
+def test_any_part_of_the_gradients(dtype):
+    """Every choice of what requires a gradient and of what is asked for gives the bits of the whole step; strided x, W in a flat row."""
+    from hyper_amd import block8
+    M, N, O, I = 2, 21, 30, 140
+    flat = torch.randn(M, O * I + 17, device='cuda')
+    x0, b0, dy = features((M, N, 2 * I), dtype, 1).cuda()[:, :, :I], torch.randn(M, O, device='cuda'), features((M, N, O), dtype, 2).cuda()
+    for shared in (False, True):
+        whole_step = None
+        for need in (7, 1, 2, 4, 3, 5, 6):
+            x = (x0[0] if shared else x0).detach().requires_grad_(bool(need & 1))
+            W = flat[:, :O * I].view(M, O, I).detach().requires_grad_(bool(need & 2))
+            b = b0.detach().requires_grad_(bool(need & 4))
+            y = block8.linear(x, W, b, scale=0.5, bias_scale=0.25)
+            for ask in range(1, 8):
+                if ask & ~need:
+                    continue
+                got = torch.autograd.grad(y, [t for i, t in enumerate((x, W, b)) if ask >> i & 1], dy, retain_graph=True)
+                if whole_step is None and ask == need == 7:
+                    whole_step = got
+                if whole_step is not None:
+                    want = [g for i, g in enumerate(whole_step) if ask >> i & 1]
+                    assert all(torch.equal(p, q) for p, q in zip(got, want)), (shared, need, ask)
+
+
+@gpu
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
 def test_gradient_of_the_bias_alone(dtype):
     from hyper_amd import block8
     for M, N, O in ((2, 5, 7), (1, 5000, 33), (3, 130, 300)):
@@ -584,6 +610,12 @@ def test_refusals_without_a_gpu():
     assert L.hecka_block8_linear_token(p, 0, 1, p, p, 1, 17, 8, 8, None, 0, 1.0, 0.0, p, None) == -1
     assert L.hecka_block8_wgrad(p, 0, p, p, 1, 1, 5000, 8, 8, 1.0, 1.0, p, p, None, 0, None) == -3
     assert L.hecka_block8_wgrad_workspace_bytes(1, 0, 8, 8) == 0
+    assert L.hecka_block8_train_bytes(0, 2, 3, 8, 8, 8, 0, 1, 1) == 0 and L.hecka_block8_train_bytes(0, 2, 2, 8, 8, 8, 0, 0, 0) == 0
+    kept, ws = (L.hecka_block8_train_bytes(i, 2, 2, 8, 8, 8, 0, 1, 1) for i in (0, 1))
+    fwd = lambda xm=2, k=kept, n=ws: L.hecka_block8_train_fwd(p, 0, xm, 8, p, 0, 64, 2, 8, 8, 8, None, 0, 1.0, 0.0, 1, 1, p, p, k, p, n, None)   # noqa: E731
+    assert fwd(xm=3) == -1 and fwd(k=kept - 1) == -3 and fwd(n=ws - 1) == -3
+    bwd = lambda dx, dw, db, need=1, k=kept, n=1 << 30: L.hecka_block8_train_bwd(p, 0, 2, 2, 8, 8, 8, 1.0, 0.0, need, need, p, k, dx, dw, db, p, n, None)   # noqa: E731
+    assert bwd(p, None, None, need=0) == -1 and bwd(None, None, p) == -1 and bwd(p, p, p, k=kept - 1) == -3 and bwd(p, p, p, n=0) == -3
 
 
 @gpu
