@@ -160,6 +160,20 @@ def first_order(backward):
     return run
 
 
+def recorded():
+    """Whether torch.jit.trace records, or forward-mode tangents may ride on the inputs: a launch that is no node of autograd's would
+    then be missing from the recording (which keeps the uninitialised result alone), or drop the tangent without a word."""
+    import torch
+    return torch._C._is_tracing() or torch.autograd.forward_ad._current_level >= 0
+
+
+def tangents(*inputs):
+    """Whether a forward-mode tangent rides on one of the inputs (those that are tensors)."""
+    import torch
+    forward_ad = torch.autograd.forward_ad
+    return forward_ad._current_level >= 0 and any(torch.is_tensor(t) and forward_ad.unpack_dual(t).tangent is not None for t in inputs)
+
+
 def call(name, device, *args):
     """Launch entry point `name` (its last argument is the stream) on `device`'s current stream, with `device` current; raises where
     it fails.  A few microseconds less of host work than entering torch.cuda.device and building a Stream object per launch."""

@@ -40,6 +40,12 @@ def _check(t, what):
         raise TypeError('%s: float32, bfloat16 or float16, got %s' % (what, t.dtype))
 
 
+def _not_traced(what):
+    """torch.jit.trace records nodes of autograd's only; codes made outside of one would be the example's."""
+    if torch._C._is_tracing():
+        raise RuntimeError('%s: torch.jit.trace cannot record it' % what)
+
+
 def _check_rows(q, what):
     if not isinstance(q, Rows8):
         raise TypeError('%s: expected Rows8, got %s' % (what, type(q).__name__))
@@ -170,12 +176,14 @@ def _values(q, dtype, act=0, dy=None):
 def quantize(x):
     """x [..., K] (any strides) as Rows8; no gradient passes."""
     _check(x, 'block8.quantize')
+    _not_traced('block8.quantize')
     return _quantize(x.detach())[0]
 
 
 def dequantize(q, dtype=None):
     """The values that a Rows8 stands for, in its own dtype or `dtype`."""
     _check_rows(q, 'block8.dequantize')
+    _not_traced('block8.dequantize')
     dtype = q.dtype if dtype is None else dtype
     if dtype not in DTYPES:
         raise TypeError('block8.dequantize: float32, bfloat16 or float16, got %s' % dtype)
@@ -191,6 +199,11 @@ def _members_apart(W):
 def quantize_weight(W, transposed=True):
     """W [M, O, I] as Weight8; transposed=False leaves out what only a backward pass reads."""
     _check(W, 'block8.quantize_weight')
+    _not_traced('block8.quantize_weight')
+    return _quantize_weight(W, transposed)
+
+
+def _quantize_weight(W, transposed=True):
     if W.dim() != 3 or 0 in W.shape:
         raise ValueError('block8.quantize_weight: needs [members, outputs, inputs] without zero sizes, got %s' % (tuple(W.shape),))
     W = _members_apart(W.detach())
@@ -259,8 +272,9 @@ def _bias_grad(dy, scale):
 
 def weight_grad(dy, rows, scale=1.0, bias_scale=1.0):
     """(dW, db) = (scale dy^T x, bias_scale sum of dy over the rows), fp32, of y = scale x W^T + bias_scale b, from dy [M, N, O] and
-    x kept as Rows8 [M, N, I] (or [N, I], shared by all members)."""
+    x kept as Rows8 [M, N, I] (or [N, I], shared by all members); no gradient passes."""
     _check(dy, 'block8.weight_grad')
+    _not_traced('block8.weight_grad')
     _check_rows(rows, 'block8.weight_grad')
     if dy.dim() != 3:
         raise ValueError('block8.weight_grad: dy has to be [members, N, outputs], got %s' % (tuple(dy.shape),))
@@ -349,10 +363,13 @@ def linear(x, weight, bias=None, scale=1.0, bias_scale=1.0):
     if isinstance(weight, Weight8):
         w = weight
         M, O, I = w.members, w.outputs, w.inputs
+        _not_traced(what)
         if not isinstance(x, Rows8):
             _check(x, what)
             if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
                 raise RuntimeError('block8.linear: weights in codes serve only (no gradients): pass the float weights to train')
+        if _lib.tangents(x, bias):
+            raise RuntimeError('block8.linear: weights in codes serve only (no tangents)')
         xm = _members(x, M, what)
         if x.shape[-1] != I:
             raise ValueError('%s: rows of %d elements for %d inputs' % (what, x.shape[-1], I))
@@ -381,7 +398,7 @@ def linear(x, weight, bias=None, scale=1.0, bias_scale=1.0):
     _check_bias(what, bias, M, O)
     _same_device(what, x, weight, bias)
     _sizes(what, M, x.shape[-2], O, I)
-    if not torch.is_grad_enabled():      # nothing is kept for a backward pass
-        w = quantize_weight(weight, transposed=False)
+    if not torch.is_grad_enabled() and not _lib.recorded():      # nothing is kept for a backward pass
+        w = _quantize_weight(weight, transposed=False)
         return _product(_quantize(x)[0], w.codes, w.scales, M, O, I, _bias_rows(bias), float(scale), float(bias_scale), x.dtype)
     return _Linear8.apply(x, weight, _bias_rows(bias), float(scale), float(bias_scale))

@@ -111,7 +111,7 @@ class BatchedLinearCheckpoint(torch.autograd.Function):
         N = x.shape[-2]
         block8._sizes('Linear(checkpoint)', M, N, O, I)
         y = _bgemm(x, W, M, N, O, I, 0 if shared else N * I, O * I, False, scale, b.contiguous() if b is not None else None, bias_scale)
-        q = block8.quantize(x) if ctx.needs_input_grad[1] else None
+        q = block8._quantize(x)[0] if ctx.needs_input_grad[1] else None
         ctx.save_for_backward(W if ctx.needs_input_grad[0] else None, *((q.codes, q.scales) if q is not None else (None, None)))
         ctx.cfg = (scale, bias_scale, tuple(x.shape), tuple(W.shape), b is not None)
         return y

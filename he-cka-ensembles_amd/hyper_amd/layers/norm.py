@@ -279,8 +279,9 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def run(*args):
         """apply, without a graph's node where nothing will ask for one (a third of a small call's time)."""
-        return _LayerNorm.apply(*args) if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:3]) else \
-            _LayerNorm.forward(None, *args)
+        if _lib.recorded() or (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:3])):
+            return _LayerNorm.apply(*args)
+        return _LayerNorm.forward(None, *args)
 
     @staticmethod
     @_lib.first_order

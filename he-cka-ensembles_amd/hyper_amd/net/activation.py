@@ -103,7 +103,7 @@ def checkpointed(name, x):
     if name not in block8.ACTIVATIONS:
         raise ValueError('no 8-bit checkpoint for activation %r: please select from %s' % (name, sorted(block8.ACTIVATIONS)))
     block8._check(x, 'checkpointed')
-    if not (torch.is_grad_enabled() and x.requires_grad):      # nothing to keep
+    if not (torch.is_grad_enabled() and x.requires_grad) and not _lib.recorded():      # nothing to keep
         return block8._quantize(x, block8.ACTIVATIONS[name], keep=False)[1]
     return _Checkpointed.apply(x, block8.ACTIVATIONS[name])
 
