@@ -80,10 +80,13 @@ __device__ __forceinline__ float exp_near(float x) {
   const float p = __builtin_amdgcn_exp2f(t);
   return fmaf(p, r * 0.69314718f, p);
 }
-// sigmoid(x) and 1 - sigmoid(x), both without cancellation: q = e^-|x| <= 1
+// sigmoid(x) and 1 - sigmoid(x), both without cancellation: q = e^-|x| <= 1.  The hardware's 1 / (1 + q), a unit in the last place off, and the
+// rounding of 1 + q are put right by one Newton step: the larger of the two is within u + 1.5 u (of q), the smaller within 5 u, u = 2^-24.
+// Three instructions: no time in fp32, 1 - 2 % in 16 bits.
 template <bool FINE>
 __device__ __forceinline__ void sigmoid_pair(float x, float& p, float& n) {
-  const float q = exp_near<FINE>(-fabsf(x)), s = __builtin_amdgcn_rcpf(1.0f + q), qs = q * s;
+  const float q = exp_near<FINE>(-fabsf(x)), d = 1.0f + q, r = __builtin_amdgcn_rcpf(d);
+  const float s = fmaf(r, fmaf(d - 1.0f - q, r, fmaf(-d, r, 1.0f)), r), qs = q * s;
   p = x >= 0.f ? s : qs;
   n = x >= 0.f ? qs : s;
   if (x != x) p = n = x;
