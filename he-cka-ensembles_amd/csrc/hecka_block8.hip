@@ -2,9 +2,10 @@
 // (hecka_block8_*; contract in include/hecka.h).  All HBM bound: one read of the input, one write of each output.
 // Sixteen lanes own a block, eight elements each, so a wave covers four blocks with 16-byte loads (two per lane for fp32),
 // the maximum is four lane permutes and the codes leave as 8 bytes per lane, 128 per block, contiguous.
-// Measured at 10 x 4096 x 4096 (a copy reaches 5.3 TB/s): quantise 95 us bf16, 162 us fp32 (5.2 TB/s); decode 92 / 163 us (5.4 / 5.1); gelu
-// 200 / 287 us forward and 184 / 288 us backward, silu 161 / 284 and 161 / 288 (5.2 / 5.3).  bf16 gelu is the one that is near the vector units'
-// rate (about forty instructions an element); with an error function good to 1.5e-7 absolutely, not relatively, it took 186 / 176 us.
+// Measured at 10 x 4096 x 4096 (a copy reaches 5.3 TB/s): quantise 95 us bf16, 162 us fp32 (5.2 TB/s); decode 92 / 163 us (5.4 / 5.1); silu, tanh
+// and sigmoid 167 / 286 us forward, 167 / 288 us backward (5.0 / 5.2), crater 168 / 180 in 16 bits; gelu fp32 287 / 288, fp16 178 / 178, bf16 217 / 200: the one that is
+// near the vector units' rate (about fifty instructions an element).  With an exponential that is good for 16 bits only (its rounded exponent not
+// put back) silu took 161, bf16 gelu 200 / 184 us.
 #include "block8.hpp"
 #include "hecka_host.hpp"
 
@@ -68,24 +69,19 @@ __device__ __forceinline__ float max8(const float* v) {
 enum { kActNone = 0, kActGelu = 1, kActSilu = 2, kActTanh = 3, kActSigmoid = 4, kActCrater = 5 };
 static constexpr float kHalfRoot = 0.70710678118654752f, kCrater = 0.70710678118654752f + 0.008274364699f;
 
-// e^x, x <= 0, from the hardware's 2^x: the exponent's rounding error, |x| 2^-25, is worked out and put back, so the result is good
-// to about 2 units in the last place (the hardware's own included); 0 from -104 down, where no float is left.  FINE = false, for 16-bit
-// results: without the repair, 2^-18 of the result where it is largest, against their half steps of 2^-8 and 2^-11.
-template <bool FINE>
-__device__ __forceinline__ float exp_near(float x) {
-  x = fmaxf(x, -104.f);
+// e^(x + low), -1e4 <= x <= 0 and |low| far below 1, from the hardware's 2^x: the exponent's rounding error, |x| 2^-25, is worked out and put back,
+// so the result is good to 3 u, u = 2^-24 (the hardware's own 2 u included); 0 where it is below 2^-126.
+__device__ __forceinline__ float exp_near(float x, float low) {
   const float t = x * 1.44269504f;
-  if (!FINE) return __builtin_amdgcn_exp2f(t);
   const float r = fmaf(x, 1.44269504f, -t) + x * 1.92596299e-8f;      // 1.44269504f + 1.92596299e-8f = log2 e
   const float p = __builtin_amdgcn_exp2f(t);
-  return fmaf(p, r * 0.69314718f, p);
+  return fmaf(p, fmaf(r, 0.69314718f, low), p);
 }
 // sigmoid(x) and 1 - sigmoid(x), both without cancellation: q = e^-|x| <= 1.  The hardware's 1 / (1 + q), a unit in the last place off, and the
 // rounding of 1 + q are put right by one Newton step: the larger of the two is within u + 1.5 u (of q), the smaller within 5 u, u = 2^-24.
 // Three instructions: no time in fp32, 1 - 2 % in 16 bits.
-template <bool FINE>
 __device__ __forceinline__ void sigmoid_pair(float x, float& p, float& n) {
-  const float q = exp_near<FINE>(-fabsf(x)), d = 1.0f + q, r = __builtin_amdgcn_rcpf(d);
+  const float q = exp_near(fmaxf(-fabsf(x), -104.f), 0.f), d = 1.0f + q, r = __builtin_amdgcn_rcpf(d);
   const float s = fmaf(r, fmaf(d - 1.0f - q, r, fmaf(-d, r, 1.0f)), r), qs = q * s;
   p = x >= 0.f ? s : qs;
   n = x >= 0.f ? qs : s;
@@ -95,11 +91,9 @@ __device__ __forceinline__ void sigmoid_pair(float x, float& p, float& n) {
 // P: degree 8, least relative error on 0 <= a <= 14.6 (1.4e-8; fitted with reweighted least squares, 0.265 is the best of a search); the
 // evaluation in fp32 is within 6e-7 (10 u).  a^2 is rounded, and what that takes from the exponent put back: at a = 13 it is 42 u of the result.
 // Beyond 20 both factors are zero as fp32 numbers.
-template <bool FINE>
 __device__ __forceinline__ float normal_below(float x, float& bell) {
   const float a = fminf(fabsf(x), 20.f), t = __builtin_amdgcn_rcpf(fmaf(0.265f, a, 1.0f)), h = a * a;
-  bell = exp_near<FINE>(-0.5f * h);
-  if (FINE) bell = fmaf(bell, -0.5f * fmaf(a, a, -h), bell);
+  bell = exp_near(-0.5f * h, -0.5f * fmaf(a, a, -h));
   float c = fmaf(0.0305863377f, t, -0.143120438f);
   c = fmaf(c, t, 0.215588495f);
   c = fmaf(c, t, -0.113883875f);
@@ -112,22 +106,22 @@ __device__ __forceinline__ float normal_below(float x, float& bell) {
   return x >= 0.f ? 1.0f - half : half;
 }
 
-template <int ACT, bool FINE>
+template <int ACT>
 __device__ __forceinline__ float act_value(float x) {
   float p, n;
-  if (ACT == kActGelu) return x * normal_below<FINE>(x, n);
+  if (ACT == kActGelu) return x * normal_below(x, n);
   if (ACT == kActTanh) return tanhf(x);
-  sigmoid_pair<FINE>(ACT == kActCrater ? 2.0f * kHalfRoot * (x + 1.0f) : x, p, n);      // 1 + tanh z = 2 sigmoid(2 z)
+  sigmoid_pair(ACT == kActCrater ? 2.0f * kHalfRoot * (x + 1.0f) : x, p, n);      // 1 + tanh z = 2 sigmoid(2 z)
   return ACT == kActSilu ? x * p : ACT == kActSigmoid ? p : 2.0f * kCrater * (x * p);
 }
-template <int ACT, bool FINE>
+template <int ACT>
 __device__ __forceinline__ float act_slope(float x) {
   float p, n;
   if (ACT == kActGelu) {
-    p = normal_below<FINE>(x, n);
+    p = normal_below(x, n);
     return fmaf(x * 0.39894228f, n, p);
   }
-  sigmoid_pair<FINE>(ACT == kActTanh ? 2.0f * x : ACT == kActCrater ? 2.0f * kHalfRoot * (x + 1.0f) : x, p, n);
+  sigmoid_pair(ACT == kActTanh ? 2.0f * x : ACT == kActCrater ? 2.0f * kHalfRoot * (x + 1.0f) : x, p, n);
   if (ACT == kActTanh) return 4.0f * p * n;
   if (ACT == kActSigmoid) return p * n;
   if (ACT == kActSilu) return fmaf(x * p, n, p);
@@ -173,7 +167,7 @@ __global__ __launch_bounds__(256) void block8_rows_kernel(const T* __restrict__ 
         Piece<T> a[8 / Piece<T>::N];
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          narrow(act_value<ACT, sizeof(T) == 4>(widen(p[u][i / Piece<T>::N].e[i % Piece<T>::N])), a[i / Piece<T>::N].e[i % Piece<T>::N]);
+          narrow(act_value<ACT>(widen(p[u][i / Piece<T>::N].e[i % Piece<T>::N])), a[i / Piece<T>::N].e[i % Piece<T>::N]);
         if constexpr (FLAT) store_lane(y + b * kBlock, 0, lane16, kBlock, a);
         else store_lane(y + at[u].row * K, at[u].blk * kBlock, lane16, K, a);
       }
@@ -229,7 +223,7 @@ __global__ __launch_bounds__(256) void block8_values_kernel(const unsigned char*
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         T& e = d[u][i / Piece<T>::N].e[i % Piece<T>::N];
-        if (ACT != kActNone) v[i] = widen(e) * act_slope<ACT, sizeof(T) == 4>(v[i]);
+        if (ACT != kActNone) v[i] = widen(e) * act_slope<ACT>(v[i]);
         else if (__is_same(T, F16) && fabsf(v[i]) == 65536.f) v[i] = copysignf(65504.f, v[i]);      // fp16's largest, 65504, is kept as 65536: back to what fp16 holds
         narrow(v[i], e);
       }

@@ -78,3 +78,17 @@ def test_above_zero_a_rounding_or_two_and_no_more(name):
     at = x.double()
     off = (checkpointed(name, x).double() - values64(name, at)).abs() / values64(name, at).clamp(min=1e-30)
     assert bool((off <= ((2.0 if name == 'silu' else 1.0) + 3 * torch.exp(-at) + 1e-3) * U).all()), float((off / U).max())
+
+
+@gpu
+@pytest.mark.parametrize('dtype', TYPES[1:], ids=str)
+@pytest.mark.parametrize('name', NAMES + ['tanh'])
+def test_a_16_bit_result_is_the_fp32_one_rounded(name, dtype):
+    """One arithmetic for all types: for every finite 16-bit argument the fp32 result, rounded once - y and, of 8-bit values, the slope."""
+    from hyper_amd.net.activation import checkpointed
+    x = torch.arange(-2 ** 15, 2 ** 15, dtype=torch.int32).to(torch.int16).view(dtype)
+    x = x[torch.isfinite(x)].cuda()
+    assert torch.equal(checkpointed(name, x).float().nan_to_num(), checkpointed(name, x.float()).to(dtype).float().nan_to_num())
+    s, f = x[x.abs() < 100].requires_grad_(True), x[x.abs() < 100].float().requires_grad_(True)
+    g, h = (torch.autograd.grad(checkpointed(name, t), t, torch.ones_like(t))[0] for t in (s, f))
+    assert torch.equal(g, h.to(dtype))
