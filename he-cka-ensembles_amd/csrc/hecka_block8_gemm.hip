@@ -94,11 +94,11 @@ __device__ __forceinline__ void store_tile(const f32x4v (&acc)[S][S], const Piec
 // (no registers), STAGES - 1 steps ahead of the products: one, or three (linear_run).  LDS rows are 128 bytes; the 16-byte piece c of row r sits
 // at piece c ^ (r & 7), so that the sixteen rows which a fragment read touches fall on different banks.
 // The weights are the first operand, so that a lane ends up with four neighbouring outputs of one row.
-// EXACT = false: the scaled fp8 instruction takes both scales as bytes.  It adds groups of eight products aligned to the
-//   largest, keeping 13 bits below its leading one (measured; 1.5e-5 of the result for normal values, whatever K), against
-//   a half step of 2^-8 of a bf16 result and 2^-11 of an fp16 one - so 16-bit results take it.
-// EXACT = true (fp32 results): the codes are widened to bf16 on their way out of LDS - exact - and the bf16 instruction
-//   adds their products in fp32 (1.4e-7 at K = 8192), at half the rate.
+// EXACT = true: the codes are widened to bf16 on their way out of LDS - exact - and the bf16 instruction adds their products in fp32
+//   (1.4e-7 at K = 8192).
+// EXACT = false (HECKA_BLOCK8_FP8, 16-bit results only): the scaled fp8 instruction takes both scales as bytes, at nearly twice the
+//   rate.  It adds groups of eight products aligned to the largest, keeping 13 bits below its leading one (measured; 1.5e-5 of the
+//   result for normal values, whatever K), against a half step of 2^-8 of a bf16 result and 2^-11 of an fp16 one: a choice of the caller's.
 // Bound by the matrix instructions at the clock that the power leaves them (zeros run a fifth faster than random values), and by LDS
 // beside them: a step's 64 KB written and 128 KB read take three quarters of the time of its products.  256 x 256 tiles reach
 // 2.42 - 2.64 PF (fp8) and 1.31 - 1.40 PF (widened) at 8192^3, where a library's plain products reach 2.70 - 3.16 and 1.41 - 1.58; 2048 x
@@ -723,7 +723,7 @@ static long long large_rounds(int M, int R, int C) { return ((long long)M * cdiv
 
 // 256 x 256 outputs a workgroup, one a CU, or 128 x 128, two a CU: a round of 256 large ones takes as long as about 512 small ones of fp8
 // products and 900 of widened codes.  Where small ones leave half of the chip idle the blocks of K are shared out, eight at least to
-// each, their sums joined by a second launch.  Measured (bf16 / fp32 results), large tiles against small: 1 x 2048 x 8192 x 4096, 256
+// each, their sums joined by a second launch.  Measured (fp8 / widened codes), large tiles against small: 1 x 2048 x 8192 x 4096, 256
 // large or 1024 small ones, 65 / 111 against 111 / 126 us; 1 x 1024 x 8192 x 4096, 128 or 512, 56 / 104 against 63 / 68; 5 x 1000 x 1000 x
 // 1000, 80 or 320, 24 / 38 against 21 / 23; 8 x 300 x 4096 x 4096, 256 or 768, 60 / 115 against 80 / 103; 10 x 300 x 4096 x 784, 320 or 960,
 // 44 / 68 against 38 / 36.  Shares: 1 x 64 x 8192 x 8192 48 / 73 us whole, 24 / 30 us in four shares, 31 / 30 us in eight; 1 x 64 x 1024 x 8192 41 / 73 us whole, 15 /
@@ -756,8 +756,8 @@ static int linear_run(const LinearPlan& p, const void* x, const void* xs, long l
       (const unsigned char*)x, (const unsigned char*)xs, xstride, xsstride, (const unsigned char*)w, (const unsigned char*)ws, N, O, \
       nblk, p.share, BIAS, bstride, alpha, beta, OUT, cdiv(N, B), cdiv(O, B))
   // Long sums of fp8 products in 128 x 128 tiles that have a CU to themselves: three steps ahead (1 x 1024 x 4096 x 4096 28 us, one ahead 32;
-  // 1 x 64 x 8192 x 8192 22 us, 24); with widened codes and in short sums the start costs what that saves (5 x 300 x 1200 x 784 bf16 10.2 us, 10.0;
-  // fp32 14.9, 14.2).
+  // 1 x 64 x 8192 x 8192 22 us, 24); with widened codes and in short sums the start costs what that saves (5 x 300 x 1200 x 784 fp8 10.2 us, 10.0;
+  // widened 14.9, 14.2).
   constexpr int FAR = EXACT ? 2 : 4;
   const bool far = FAR > 2 && p.share >= 16 && (long long)M * cdiv(N, 128) * cdiv(O, 128) * p.splits <= 256;
   if (p.splits > 1 || y_members < M) {
@@ -846,6 +846,12 @@ static int wgrad_run(const void* dy, const void* x, const void* xs, long long xs
   return check_launch("block8_wgrad");
 }
 
+// whether `dtype` asks for the fp8 instruction, and that taken off it (left there, and so no known type, with fp32, whose products are exact)
+static bool take_fp8(int& dtype) {
+  if (dtype != (HECKA_DT_BF16 | HECKA_BLOCK8_FP8) && dtype != (HECKA_DT_F16 | HECKA_BLOCK8_FP8)) return false;
+  dtype &= ~HECKA_BLOCK8_FP8;
+  return true;
+}
 static bool bad_type(int dtype) { return dtype != HECKA_DT_F32 && dtype != HECKA_DT_BF16 && dtype != HECKA_DT_F16; }
 // sizes for which every index that the kernels keep in 32 bits fits: sizes below 2^22, tiles below 2^31
 static bool bad_sizes(int M, int N, int O, int I) {
@@ -861,13 +867,15 @@ using namespace hecka;
 extern "C" {
 
 size_t hecka_block8_linear_workspace_bytes(int M, int N, int O, int I, int y_members, int dtype) {
+  const bool fp8 = take_fp8(dtype);
   if (bad_type(dtype) || bad_sizes(M, N, O, I) || (y_members != M && y_members != 1)) return 0;
-  return linear_workspace(linear_plan(M, N, O, row_blocks(I), dtype == HECKA_DT_F32), M, N, O, y_members);
+  return linear_workspace(linear_plan(M, N, O, row_blocks(I), !fp8), M, N, O, y_members);
 }
 
 int hecka_block8_linear(const void* x, const void* xscales, int x_members, const void* w, const void* wscales, int M, int N, int O,
                         int I, const float* bias, long long bstride, float alpha, float beta, void* y, int dtype, int y_members,
                         void* ws, size_t ws_bytes, void* stream) {
+  const bool fp8 = take_fp8(dtype);
   if (bad_type(dtype)) return fail(HECKA_EINVAL, "block8_linear: unknown dtype%s");
   if (bad_sizes(M, N, O, I)) return fail(HECKA_EINVAL, "%sblock8_linear: bad size (N = %lld, O = %lld)", "", N, O);
   if (x_members != M && x_members != 1) return fail(HECKA_EINVAL, "%sblock8_linear: codes of %lld members for %lld", "", x_members, M);
@@ -876,7 +884,7 @@ int hecka_block8_linear(const void* x, const void* xscales, int x_members, const
   if (!aligned16(x) || !aligned16(w) || (reinterpret_cast<uintptr_t>(xscales) & 3) || (reinterpret_cast<uintptr_t>(wscales) & 3))
     return fail(HECKA_EINVAL, "block8_linear: codes need 16-byte alignment, scales 4-byte%s");
   const int nblk = row_blocks(I);
-  const LinearPlan p = linear_plan(M, N, O, nblk, dtype == HECKA_DT_F32);
+  const LinearPlan p = linear_plan(M, N, O, nblk, !fp8);
   if ((ws ? ws_bytes : 0) < linear_workspace(p, M, N, O, y_members))
     return fail(HECKA_EWORKSPACE, "%sblock8_linear: workspace too small (%lld bytes given)", "", (long long)ws_bytes);
   clear_error();
@@ -884,7 +892,8 @@ int hecka_block8_linear(const void* x, const void* xscales, int x_members, const
   hipStream_t st = (hipStream_t)stream;
 #define HECKA_RUN(T, EXACT) \
   linear_run<T, EXACT>(p, x, xscales, xst, sst, w, wscales, M, N, O, nblk, bias, bstride, alpha, beta, y, y_members, (float*)ws, st)
-  return dtype == HECKA_DT_F32 ? HECKA_RUN(float, true) : dtype == HECKA_DT_BF16 ? HECKA_RUN(Bf16, false) : HECKA_RUN(F16, false);
+  if (fp8) return dtype == HECKA_DT_BF16 ? HECKA_RUN(Bf16, false) : HECKA_RUN(F16, false);
+  return dtype == HECKA_DT_F32 ? HECKA_RUN(float, true) : dtype == HECKA_DT_BF16 ? HECKA_RUN(Bf16, true) : HECKA_RUN(F16, true);
 #undef HECKA_RUN
 }
 
@@ -969,6 +978,8 @@ Kept kept_parts(const Sizes& z, Parts& p, bool need_dx, bool need_dw) {
 }  // namespace
 
 size_t hecka_block8_train_bytes(int what, int M, int x_members, int N, int O, int I, int dtype, int need_dx, int need_dw) {
+  const int products = dtype;      // with the choice of the instruction
+  take_fp8(dtype);
   if (bad_type(dtype) || bad_sizes(M, N, O, I) || (x_members != M && x_members != 1)) return 0;
   const Sizes z(M, x_members, N, O, I);
   Parts p{nullptr, 0};
@@ -979,11 +990,11 @@ size_t hecka_block8_train_bytes(int what, int M, int x_members, int N, int O, in
     p.take(z.xs, !need_dw);
     p.take(z.wc);
     p.take(z.ws);
-    p.take(hecka_block8_linear_workspace_bytes(M, N, O, I, M, dtype));
+    p.take(hecka_block8_linear_workspace_bytes(M, N, O, I, M, products));
   } else {
     p.take(z.dc, need_dx);
     p.take(z.ds, need_dx);
-    p.take(hecka_block8_linear_workspace_bytes(M, N, I, O, x_members, dtype), need_dx);
+    p.take(hecka_block8_linear_workspace_bytes(M, N, I, O, x_members, products), need_dx);
     p.take(hecka_block8_wgrad_workspace_bytes(M, N, O, I), need_dw);
   }
   return p.used;
@@ -992,11 +1003,13 @@ size_t hecka_block8_train_bytes(int what, int M, int x_members, int N, int O, in
 int hecka_block8_train_fwd(const void* x, int dtype, int x_members, long long ld, const void* W, int wdtype, long long mstride, int M, int N,
                            int O, int I, const float* bias, long long bstride, float alpha, float beta, int need_dx, int need_dw, void* y,
                            void* kept, size_t kept_bytes, void* ws, size_t ws_bytes, void* stream) {
+  const int products = dtype;
+  take_fp8(dtype);
   if (bad_type(dtype) || bad_type(wdtype)) return fail(HECKA_EINVAL, "block8_train_fwd: unknown dtype%s");
   if (bad_sizes(M, N, O, I)) return fail(HECKA_EINVAL, "%sblock8_train_fwd: bad size (N = %lld, O = %lld)", "", N, O);
   if (x_members != M && x_members != 1) return fail(HECKA_EINVAL, "%sblock8_train_fwd: rows of %lld members for %lld", "", x_members, M);
   const size_t most = hecka_block8_train_bytes(0, M, x_members, N, O, I, dtype, need_dx, need_dw);
-  if ((kept ? kept_bytes : 0) < most || (ws ? ws_bytes : 0) < hecka_block8_train_bytes(1, M, x_members, N, O, I, dtype, need_dx, need_dw))
+  if ((kept ? kept_bytes : 0) < most || (ws ? ws_bytes : 0) < hecka_block8_train_bytes(1, M, x_members, N, O, I, products, need_dx, need_dw))
     return fail(HECKA_EWORKSPACE, "%sblock8_train_fwd: workspace too small (%lld bytes given)", "", (long long)ws_bytes);
   const Sizes z(M, x_members, N, O, I);
   Parts pk{(char*)kept, 0}, pw{(char*)ws, 0};
@@ -1006,23 +1019,25 @@ int hecka_block8_train_fwd(const void* x, int dtype, int x_members, long long ld
     k.xs = pw.take(z.xs);
   }
   void *wc = pw.take(z.wc), *wsc = pw.take(z.ws);
-  const size_t need = hecka_block8_linear_workspace_bytes(M, N, O, I, M, dtype);
+  const size_t need = hecka_block8_linear_workspace_bytes(M, N, O, I, M, products);
   int rc = hecka_block8_quantize(x, dtype, (long long)x_members * N, I, ld, HECKA_ACT_NONE, k.xc, k.xs, nullptr, stream);
   if (!rc) rc = hecka_block8_weight(W, wdtype, M, O, I, mstride, wc, wsc, k.tc, k.ts, stream);
   if (!rc)
-    rc = hecka_block8_linear(k.xc, k.xs, x_members, wc, wsc, M, N, O, I, bias, bstride, alpha, beta, y, dtype, M, need ? pw.take(need) : nullptr, need, stream);
+    rc = hecka_block8_linear(k.xc, k.xs, x_members, wc, wsc, M, N, O, I, bias, bstride, alpha, beta, y, products, M, need ? pw.take(need) : nullptr, need, stream);
   return rc;
 }
 
 int hecka_block8_train_bwd(const void* dy, int dtype, int x_members, int M, int N, int O, int I, float alpha, float beta, int need_dx,
                            int need_dw, const void* kept, size_t kept_bytes, void* dx, float* dW, float* db, void* ws, size_t ws_bytes,
                            void* stream) {
+  const int products = dtype;
+  take_fp8(dtype);
   if (bad_type(dtype)) return fail(HECKA_EINVAL, "block8_train_bwd: unknown dtype%s");
   if (bad_sizes(M, N, O, I)) return fail(HECKA_EINVAL, "%sblock8_train_bwd: bad size (N = %lld, O = %lld)", "", N, O);
   if (x_members != M && x_members != 1) return fail(HECKA_EINVAL, "%sblock8_train_bwd: rows of %lld members for %lld", "", x_members, M);
   if (!dy || (dx && !need_dx) || (dW && !need_dw) || (db && !dW)) return fail(HECKA_EINVAL, "block8_train_bwd: null pointer, or a gradient whose codes were not kept%s");
   if ((kept ? kept_bytes : 0) < hecka_block8_train_bytes(0, M, x_members, N, O, I, dtype, need_dx, need_dw) ||
-      (ws ? ws_bytes : 0) < hecka_block8_train_bytes(2, M, x_members, N, O, I, dtype, dx != nullptr, dW != nullptr))
+      (ws ? ws_bytes : 0) < hecka_block8_train_bytes(2, M, x_members, N, O, I, products, dx != nullptr, dW != nullptr))
     return fail(HECKA_EWORKSPACE, "%sblock8_train_bwd: workspace too small (%lld bytes given)", "", (long long)ws_bytes);
   const Sizes z(M, x_members, N, O, I);
   Parts pk{(char*)const_cast<void*>(kept), 0}, pw{(char*)ws, 0};
@@ -1030,10 +1045,10 @@ int hecka_block8_train_bwd(const void* dy, int dtype, int x_members, int M, int 
   int rc = 0;
   if (dx) {
     void *dc = pw.take(z.dc), *ds = pw.take(z.ds);
-    const size_t need = hecka_block8_linear_workspace_bytes(M, N, I, O, x_members, dtype);
+    const size_t need = hecka_block8_linear_workspace_bytes(M, N, I, O, x_members, products);
     void* slabs = need ? pw.take(need) : nullptr;
     rc = hecka_block8_quantize(dy, dtype, (long long)M * N, O, O, HECKA_ACT_NONE, dc, ds, nullptr, stream);
-    if (!rc) rc = hecka_block8_linear(dc, ds, M, k.tc, k.ts, M, N, I, O, nullptr, 0, alpha, 0.f, dx, dtype, x_members, slabs, need, stream);
+    if (!rc) rc = hecka_block8_linear(dc, ds, M, k.tc, k.ts, M, N, I, O, nullptr, 0, alpha, 0.f, dx, products, x_members, slabs, need, stream);
   }
   if (dW && !rc) {
     const size_t need = hecka_block8_wgrad_workspace_bytes(M, N, O, I);

@@ -18,6 +18,7 @@ from . import _lib
 
 BLOCK = 128
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+FP8 = 0x100          # added to a 16-bit type: products by the fp8 matrix instruction
 ACTIVATIONS = {'gelu': 1, 'silu': 2, 'tanh': 3, 'sigmoid': 4, 'crater': 5}
 _MOST = 1 << 22      # sizes of a product
 
@@ -235,14 +236,23 @@ def _bias_rows(b):
     return b if b is None or b.stride(1) == 1 else b.contiguous()
 
 
-def _product(q, codes, scales, M, O, I, bias, alpha, beta, dtype):
+def _products(what, products, dtype):
+    """The library's number for results of `dtype` by the wanted products."""
+    if products not in ('exact', 'fp8'):
+        raise ValueError("%s: products are 'exact' or 'fp8', got %r" % (what, products))
+    if products == 'fp8' and dtype == torch.float32:
+        raise ValueError('%s: the fp8 instruction is for bfloat16 and float16; float32 results are exact products' % what)
+    return DTYPES[dtype] + (FP8 if products == 'fp8' else 0)
+
+
+def _product(q, codes, scales, M, O, I, bias, alpha, beta, dtype, number):
     N = q.shape[-2]
     y = torch.empty((M, N, O), device=q.device, dtype=dtype)
     if y.numel():
-        nbytes = _lib.lib().hecka_block8_linear_workspace_bytes(M, N, O, I, M, DTYPES[dtype])
+        nbytes = _lib.lib().hecka_block8_linear_workspace_bytes(M, N, O, I, M, number)
         ws = torch.empty((nbytes // 4,), device=q.device, dtype=torch.float32) if nbytes else None
         _lib.call('hecka_block8_linear', q.device, q.codes.data_ptr(), q.scales.data_ptr(), 1 if len(q.shape) == 2 else M,
-                  codes.data_ptr(), scales.data_ptr(), M, N, O, I, _ptr(bias), _bstride(bias), alpha, beta, y.data_ptr(), DTYPES[dtype],
+                  codes.data_ptr(), scales.data_ptr(), M, N, O, I, _ptr(bias), _bstride(bias), alpha, beta, y.data_ptr(), number,
                   M, _ptr(ws), nbytes)
     return y
 
@@ -294,13 +304,13 @@ def _sizes(what, M, N, O, I):
 
 
 class _Linear8(torch.autograd.Function):
-    """y[m] = scale x8[m] W8[m]^T + bias_scale b[m].  Keeps the codes of x and W (a byte per element each) and nothing else; the
+    """y[m] = scale x8[m] W8[m]^T + bias_scale b[m]; t: _products' number.  Keeps the codes of x and W (a byte per element each) and nothing else; the
     backward's products are dx = scale dy8 W8 and dW = scale dy^T x8 (dy as it is, x from the checkpoint)."""
 
     @staticmethod
-    def forward(ctx, x, W, b, scale, bias_scale):
+    def forward(ctx, x, W, b, scale, bias_scale, t):
         M, O, I = W.shape
-        N, xm, t = x.shape[-2], 1 if x.dim() == 2 else M, DTYPES[x.dtype]
+        N, xm = x.shape[-2], 1 if x.dim() == 2 else M
         need_dx, need_dw, _ = ctx.needs_input_grad[:3]
         y = torch.empty((M, N, O), device=x.device, dtype=x.dtype)
         kept = None
@@ -316,15 +326,15 @@ class _Linear8(torch.autograd.Function):
                       _ptr(b), _bstride(b), scale, bias_scale, need_dx, need_dw, y.data_ptr(), _ptr(kept), nk, ws.data_ptr(), nw)
         # a tensor that autograd frees with the graph; only the codes that a gradient will ask for
         ctx.save_for_backward(kept)
-        ctx.cfg = (x.shape, x.dtype, W.shape, W.dtype, b is not None, scale, bias_scale, need_dx, need_dw)
+        ctx.cfg = (x.shape, x.dtype, W.shape, W.dtype, b is not None, scale, bias_scale, need_dx, need_dw, t)
         return y
 
     @staticmethod
     @_lib.first_order
     def backward(ctx, dy):
         kept, = ctx.saved_tensors
-        xshape, xdtype, (M, O, I), wdtype, has_bias, scale, bias_scale, need_dx, need_dw = ctx.cfg
-        N, xm, t = dy.shape[1], 1 if len(xshape) == 2 else M, DTYPES[xdtype]
+        xshape, xdtype, (M, O, I), wdtype, has_bias, scale, bias_scale, need_dx, need_dw, t = ctx.cfg
+        N, xm = dy.shape[1], 1 if len(xshape) == 2 else M
         dy = dy.contiguous()
         dx = dW = db = None
         want_x, want_w, want_b = ctx.needs_input_grad[0], ctx.needs_input_grad[1], has_bias and ctx.needs_input_grad[2]      # may be fewer now
@@ -336,13 +346,13 @@ class _Linear8(torch.autograd.Function):
         elif want_b:
             db = _bias_grad(dy, bias_scale)
         if N == 0:
-            return dx, dW.zero_().to(wdtype) if want_w else None, db.zero_() if want_b else None, None, None
+            return dx, dW.zero_().to(wdtype) if want_w else None, db.zero_() if want_b else None, None, None, None
         if want_x or want_w:
             nw = _lib.lib().hecka_block8_train_bytes(2, M, xm, N, O, I, t, want_x, want_w)
             ws = torch.empty((nw,), device=dy.device, dtype=torch.uint8) if nw else None
             _lib.call('hecka_block8_train_bwd', dy.device, dy.data_ptr(), t, xm, M, N, O, I, scale, bias_scale, need_dx, need_dw, kept.data_ptr(),
                       kept.numel(), _ptr(dx), _ptr(dW), _ptr(db) if want_w else None, _ptr(ws), nw)
-        return dx, dW.to(wdtype) if want_w else None, db, None, None
+        return dx, dW.to(wdtype) if want_w else None, db, None, None, None
 
 
 def _check_bias(what, b, M, O):
@@ -353,12 +363,15 @@ def _check_bias(what, b, M, O):
         raise ValueError('%s: bias has to be float32 (%d, %d), got %s %s' % (what, M, O, b.dtype, tuple(b.shape)))
 
 
-def linear(x, weight, bias=None, scale=1.0, bias_scale=1.0):
+def linear(x, weight, bias=None, scale=1.0, bias_scale=1.0, products='exact'):
     """y[m] = scale x[m] W[m]^T + bias_scale b[m] in 8-bit blocks; x [M, N, I], or [N, I] shared by all members; bias fp32 [M, O].
 
     weight: a float tensor [M, O, I] - training: its codes are made here, x's are the checkpoint; or a Weight8 - serving: no
     gradients, x may be Rows8 (then the result has the dtype it was made from), and up to 16 rows take one launch that makes the
-    codes of x on the way.  fp32 x: products exact, added in fp32; bf16 / fp16 x: fp8 matrix instructions."""
+    codes of x on the way.
+
+    products: 'exact' - of the blocks' values, added in fp32 - or, for bf16 / fp16 x, 'fp8' - the fp8 matrix instruction, nearly twice as
+    fast, which cuts each product 13 bits below the largest of eight (1.5e-5 of the result); up to 16 rows served are exact with either."""
     what = 'block8.linear'
     if isinstance(weight, Weight8):
         w = weight
@@ -377,10 +390,11 @@ def linear(x, weight, bias=None, scale=1.0, bias_scale=1.0):
         _same_device(what, x, w, bias)
         N = x.shape[-2]
         _sizes(what, M, N, O, I)
+        number = _products(what, products, x.dtype)
         b = _bias_rows(bias.detach() if bias is not None else None)
         if isinstance(x, Rows8) or N > 16:
             q = x if isinstance(x, Rows8) else _quantize(x.detach())[0]
-            return _product(q, w.codes, w.scales, M, O, I, b, scale, bias_scale, q.dtype)
+            return _product(q, w.codes, w.scales, M, O, I, b, scale, bias_scale, q.dtype, number)
         x = x.detach().contiguous()
         y = torch.empty((M, N, O), device=x.device, dtype=x.dtype)
         if N:
@@ -398,7 +412,8 @@ def linear(x, weight, bias=None, scale=1.0, bias_scale=1.0):
     _check_bias(what, bias, M, O)
     _same_device(what, x, weight, bias)
     _sizes(what, M, x.shape[-2], O, I)
+    number = _products(what, products, x.dtype)
     if not torch.is_grad_enabled() and not _lib.recorded():      # nothing is kept for a backward pass
         w = _quantize_weight(weight, transposed=False)
-        return _product(_quantize(x)[0], w.codes, w.scales, M, O, I, _bias_rows(bias), float(scale), float(bias_scale), x.dtype)
-    return _Linear8.apply(x, weight, _bias_rows(bias), float(scale), float(bias_scale))
+        return _product(_quantize(x)[0], w.codes, w.scales, M, O, I, _bias_rows(bias), float(scale), float(bias_scale), x.dtype, number)
+    return _Linear8.apply(x, weight, _bias_rows(bias), float(scale), float(bias_scale), number)

@@ -140,13 +140,14 @@ class BatchedLinearCheckpoint(torch.autograd.Function):
 class Linear(ParametersGroup):
     """checkpoint='e4m3' (not in the reference's signature): what the layer keeps for its backward pass - its input and, for the
     activations that block8 knows, the activation's - is kept in 8-bit blocks; results are the same, gradients are taken at the
-    blocks' values.  compute='e4m3': the products themselves run on 8-bit blocks of x, W and the gradient (block8.linear; x fp32, bf16
-    or fp16), whose codes of x are the checkpoint."""
+    blocks' values.  compute='e4m3': the products themselves are of 8-bit blocks of x, W and the gradient (block8.linear; x fp32, bf16
+    or fp16), whose codes of x are the checkpoint; compute='fp8': the same for bf16 and fp16 x by the fp8 matrix instruction, faster and
+    less exact (block8.linear's products)."""
 
     def __init__(self, in_features, out_features, bias=True, act=None, gamma=1.0, param_scale='torch', track=True, compute='fp32',
                  checkpoint=None):
-        if compute not in ('fp32', 'e4m3'):
-            raise ValueError("compute is 'fp32' or 'e4m3', got %r" % (compute,))
+        if compute not in ('fp32', 'e4m3', 'fp8'):
+            raise ValueError("compute is 'fp32', 'e4m3' or 'fp8', got %r" % (compute,))
         if checkpoint not in (None, 'e4m3'):
             raise ValueError("checkpoint is None or 'e4m3', got %r" % (checkpoint,))
         self.compute, self.checkpoint = compute, checkpoint
@@ -197,8 +198,8 @@ class Linear(ParametersGroup):
         else:
             raise ValueError('Bad x dimension. Got %d' % x.ndim)
         b = viewed['bias'] if self.bias else None
-        if self.compute == 'e4m3':
-            y = block8.linear(x, W, b, self.scale, self.bias_scale)
+        if self.compute != 'fp32':
+            y = block8.linear(x, W, b, self.scale, self.bias_scale, 'fp8' if self.compute == 'fp8' else 'exact')
         else:
             y = (BatchedLinearCheckpoint if self.checkpoint and torch.is_grad_enabled() else BatchedLinear).apply(x, W, b, self.scale, self.bias_scale)
         if self.checkpoint and self.act_name in block8.ACTIVATIONS:
@@ -207,7 +208,7 @@ class Linear(ParametersGroup):
 
     def extra_repr(self):
         return 'in_features=%d, out_features=%d, activation=%s%s%s' % (
-            self.in_features, self.out_features, self.act, ', compute=e4m3' if self.compute != 'fp32' else '',
+            self.in_features, self.out_features, self.act, ', compute=%s' % self.compute if self.compute != 'fp32' else '',
             ', checkpoint=e4m3' if self.checkpoint else '')
 
 

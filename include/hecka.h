@@ -543,6 +543,7 @@ int hecka_layernorm_bwd(const void* dy, const void* x, int dtype, const float* m
  * 65536 comes back as 65504 in fp16).  Codes [R, Kp], Kp = K up to whole blocks (zero codes behind K), 16-byte
  * aligned; scale bytes q + 127 [R, S], S = Kp / 128 up to a multiple of 4 (127 behind the last block).
  * Weights [M, O, I] share one s over 128 x 128 elements: codes [M, O, Ip], scale bytes [M, ceil(O / 128), S(I)]. */
+#define HECKA_BLOCK8_FP8 0x100 /* added to the dtype of 16-bit results: products by the fp8 matrix instruction (hecka_block8_linear) */
 #define HECKA_ACT_NONE 0
 #define HECKA_ACT_GELU 1     /* erf form */
 #define HECKA_ACT_SILU 2
@@ -561,8 +562,9 @@ int hecka_block8_values(const void* codes, const void* scales, const void* dy, i
 int hecka_block8_weight(const void* W, int dtype, int M, int O, int I, long long mstride, void* codes, void* scales, void* codes_t,
                         void* scales_t, void* stream);
 /* y[m][n][o] = alpha sum_i x[m][n][i] w[m][o][i] + beta bias[m][o] (bias fp32, members bstride elements apart, may be NULL) of rows in codes (x_members: M,
- * or 1 for rows that all members share) and weights in codes; y in dtype.  HECKA_DT_F32: exact products, added in fp32;
- * 16-bit: fp8 matrix instructions (about 1.5e-5 of the result before its rounding).  y_members: M, or 1 for the sum over the
+ * or 1 for rows that all members share) and weights in codes; y in dtype.  Products are exact and added in fp32;
+ * HECKA_DT_BF16 | HECKA_BLOCK8_FP8, and HECKA_DT_F16: by the fp8 matrix instruction, nearly twice as fast, which cuts each product 13 bits below the
+ * largest of eight (about 1.5e-5 of the result before its rounding).  y_members: M, or 1 for the sum over the
  * members (no bias), added in fp32 and rounded once.  ws: hecka_block8_linear_workspace_bytes.  Sizes up to 2^22. */
 size_t hecka_block8_linear_workspace_bytes(int M, int N, int O, int I, int y_members, int dtype);
 int hecka_block8_linear(const void* x, const void* xscales, int x_members, const void* w, const void* wscales, int M, int N, int O,
@@ -579,7 +581,7 @@ int hecka_block8_wgrad(const void* dy, int dtype, const void* x, const void* xsc
 /* A layer's training step in two calls, each the launches above one after the other: forward codes of x [x_members, N, I] (dtype, rows
  * ld apart) and W [M, O, I] (wdtype, members mstride apart), y; backward dx (of x_members; their sum where 1), dW, db from dy [M, N, O].
  * `kept` (256-byte aligned) carries the codes that the wanted gradients need from one to the other; the same need_dx / need_dw in
- * both; dx, dW and db may be NULL, db only with dW.  hecka_block8_train_bytes: what = 0 kept, 1 the forward's workspace, 2 the backward's
+ * both; dx, dW and db may be NULL, db only with dW.  dtype | HECKA_BLOCK8_FP8 as above, for y and dx; dW is the same.  hecka_block8_train_bytes: what = 0 kept, 1 the forward's workspace, 2 the backward's
  * (need_dx, need_dw: of the gradients asked for). */
 size_t hecka_block8_train_bytes(int what, int M, int x_members, int N, int O, int I, int dtype, int need_dx, int need_dw);
 int hecka_block8_train_fwd(const void* x, int dtype, int x_members, long long ld, const void* W, int wdtype, long long mstride, int M, int N,
