@@ -121,10 +121,24 @@ __device__ __forceinline__ void mfma_fp8(f32x4v& c, i32x8 a, i32x8 b, unsigned s
 __device__ __forceinline__ void mfma_bf16(f32x4v& c, i32x4 a, i32x4 b) {
   asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }
-// A sum in ordinary registers: settled (mfma_settle) before the compiler can touch it.
+// Sums in ordinary registers, from zero and further: settled before anything else can touch them.
+__device__ __forceinline__ void first_columns(f32x4v& c, i32x4 a, i32x4 b) {
+  asm volatile("s_nop 3\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %2, 0" : "=&v"(c) : "v"(a), "v"(b));
+}
 __device__ __forceinline__ void add_columns(f32x4v& c, i32x4 a, i32x4 b) {
   asm volatile("s_nop 3\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
 }
+__device__ __forceinline__ void settle_columns(f32x4v& c) { asm volatile("s_nop 15\n\ts_nop 3" : "+v"(c)); }
+
+// A sum of any number of terms as accurate as one of a few: hi + lo, lo what the additions to hi have rounded off (exactly worked out: Knuth's
+// two-sum).  Once hi is not finite lo is NaN and hi the answer.
+struct Long { float hi, lo; };
+__device__ __forceinline__ void add(Long& s, float t) {
+  const float sum = s.hi + t, part = sum - s.hi;
+  s.lo += (s.hi - (sum - part)) + (t - part);
+  s.hi = sum;
+}
+__device__ __forceinline__ float value(const Long& s) { return s.lo == s.lo ? s.hi + s.lo : s.hi; }
 // The same by the compiler's own means, which waits for what needs it: for the smaller tiles, whose sums leave it registers.
 template <bool OWN>
 __device__ __forceinline__ void mul_fp8(f32x4v& c, i32x8 a, i32x8 b, unsigned sa, unsigned sb) {
@@ -446,8 +460,9 @@ __global__ __launch_bounds__(64 * W) void block8_token_kernel(const T* __restric
 // The sum runs down the rows of both operands.  A step stages 32 rows n of each in LDS as bf16, row major, and the
 // transposing LDS read hands every lane four rows of its column at a time.  x8's codes are widened times their scale (exact);
 // dy is split exactly into TERMS bf16 terms by cutting (bf16 1, fp16 2, fp32 3 terms of eight significant bits), every term
-// multiplies x: the products are exact and added in fp32.  db: the sums of dy are one more product with a column of ones, made
-// by the waves that hold the first columns i.
+// multiplies x: the products are exact and added in fp32.  db: a step's sums of dy are one more product with a column of ones, made
+// by the waves that hold the first columns i; the steps' sums are added with what the additions round off (Long), so that db is as good over a
+// million rows as over 64: within 1e-7 of the 2-norm at 20000 rows, 2.2e-7 in one chain, at the same time.
 // LDS rows hold units of 16 columns (32 bytes); unit u of row n sits at u ^ (n & 7): a transposing read takes one unit of
 // sixteen rows, eight of which lie on different banks.
 // Few tiles (small O x I): the rows are cut into pieces by blockIdx.y, whose sums a second kernel adds up in order.
@@ -577,9 +592,9 @@ __global__ __launch_bounds__(256) void block8_wgrad_kernel(
   // wave has tiles mine, mine + 2 tiles_i, ... - with many tiles_i one at most.
   constexpr int OWN = TT / 2;
   const int mine = db ? ti * 2 + wi : TT;
-  f32x4v accb[OWN];
+  Long sums[OWN];      // a step's rows are added by the matrix instruction, the steps by add(): the rows may be millions
 #pragma unroll
-  for (int n = 0; n < OWN; ++n) accb[n] = f32x4v{0.f, 0.f, 0.f, 0.f};
+  for (int n = 0; n < OWN; ++n) sums[n] = Long{0.f, 0.f};
   const i32x4 ones = {0x3f803f80, 0x3f803f80, 0x3f803f80, 0x3f803f80};
 
   // fragment of 16 columns (unit u) of a tile: rows 4 g .. 4 g + 3 and 16 more down
@@ -622,16 +637,22 @@ __global__ __launch_bounds__(256) void block8_wgrad_kernel(
       if (S == 2 && e < TT) fx[1][e] = frag_x(e, 1, buf);
       if (e == TURN) {
         if (mine < TT) {      // before the step's buffer is given up
+          f32x4v c;
+          first_columns(c, ones, fs[0]);
 #pragma unroll
-          for (int f = 0; f < S * TERMS; ++f) add_columns(accb[0], ones, fs[f]);
+          for (int f = 1; f < S * TERMS; ++f) add_columns(c, ones, fs[f]);
+          settle_columns(c);
+          add(sums[0], c[0]);
 #pragma unroll
           for (int n = 1; n < OWN; ++n) {
             if (mine + n * 2 * tiles_i < TT) {
+              first_columns(c, ones, frag_s(mine + n * 2 * tiles_i, 0, buf));
 #pragma unroll
-              for (int f = 0; f < S * TERMS; ++f) add_columns(accb[n], ones, frag_s(mine + n * 2 * tiles_i, f, buf));
+              for (int f = 1; f < S * TERMS; ++f) add_columns(c, ones, frag_s(mine + n * 2 * tiles_i, f, buf));
+              settle_columns(c);
+              add(sums[n], c[0]);
             }
           }
-          mfma_settle();
         }
         __syncthreads();
       }
@@ -694,7 +715,7 @@ __global__ __launch_bounds__(256) void block8_wgrad_kernel(
 #pragma unroll
     for (int n = 0; n < OWN; ++n) {
       const int t = mine + n * 2 * tiles_i, o = o0 + (wo * TT + t) * 16 + l16;
-      if (t < TT && o < O) to_db[o] = beta * accb[n][0];
+      if (t < TT && o < O) to_db[o] = beta * value(sums[n]);
     }
   }
   const Piece<float> none[TT] = {};
@@ -703,16 +724,16 @@ __global__ __launch_bounds__(256) void block8_wgrad_kernel(
                                    I, O - o1, I - i1);
 }
 
-// out[e] = sum over S slabs, in order; two arrays in one launch: n of out, then n2 of out2, whose slabs stand behind out's
+// out[e] = sum over S slabs, in order, what its additions round off included; two arrays in one launch: n of out, then n2 of out2, whose slabs stand behind out's
 __global__ __launch_bounds__(256) void block8_slabs_kernel(const float* __restrict__ part, int S, long long n, float* __restrict__ out,
                                                            long long n2, float* __restrict__ out2) {
   for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < n + n2; e += (long long)gridDim.x * 256) {
     const bool second = e >= n;
     const float* p = second ? part + S * n + (e - n) : part + e;
     const long long step = second ? n2 : n;
-    float s = p[0];
-    for (int i = 1; i < S; ++i) s += p[i * step];
-    (second ? out2[e - n] : out[e]) = s;
+    Long s{p[0], 0.f};
+    for (int i = 1; i < S; ++i) add(s, p[i * step]);
+    (second ? out2[e - n] : out[e]) = value(s);
   }
 }
 
