@@ -4,7 +4,7 @@ only).
 
     q = quantize(x)                          # Rows8: a checkpoint of x in a byte per element
     dequantize(q)                            # the values that it stands for
-    w = quantize_weight(W)                   # Weight8: laid out once by a program that serves
+    w = quantize_weight(W, transposed=False) # Weight8: laid out once by a program that serves
     y = linear(x, w, bias)                   # x (or Rows8) times w^T
     y = linear(x, W, bias)                   # W a float tensor: training - gradients for x, W and bias
     dW, db = weight_grad(dy, q)              # the weight gradient from the checkpoint
@@ -95,8 +95,9 @@ class Rows8(object):
 
 class Weight8(object):
     """Weights [M, O, I] in 8-bit blocks of 128 x 128.  codes [M, O, Ip] (uint8 or float8_e4m3fn, contiguous), scales uint8 [M,
-    ceil(O / 128), S(I)]: byte e stands for 2^(e - 127).  codes_t [M, I, Op] / scales_t: the same codes transposed, which the
-    input gradient multiplies with (None where there is no backward pass)."""
+    ceil(O / 128), S(I)]: byte e, 1 to 254, stands for 2^(e - 127).  codes_t [M, I, Op] / scales_t (or None): the same codes transposed, for a
+    program that multiplies with W as well as with W^T, by Weight8(w.codes_t, w.scales_t, w.outputs).  linear reads codes and scales alone, and
+    its training makes codes of its own."""
 
     def __init__(self, codes, scales, inputs, codes_t=None, scales_t=None):
         for t, n in ((codes, 'codes'), (codes_t, 'codes_t')):
@@ -111,8 +112,8 @@ class Weight8(object):
             raise ValueError('Weight8: codes_t and scales_t come together')
         want = [(scales, (M, row_blocks(O), scale_stride(inputs)))]
         if codes_t is not None:
-            if tuple(codes_t.shape) != (M, inputs, row_blocks(O) * BLOCK):
-                raise ValueError('Weight8: codes_t has the wrong shape %s' % (tuple(codes_t.shape),))
+            if tuple(codes_t.shape) != (M, inputs, row_blocks(O) * BLOCK) or codes_t.device != codes.device:
+                raise ValueError('Weight8: codes_t has the wrong shape or device, %s on %s' % (tuple(codes_t.shape), codes_t.device))
             want.append((scales_t, (M, row_blocks(inputs), scale_stride(O))))
         for t, shape in want:
             if t.dtype != torch.uint8 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != codes.device:
@@ -198,7 +199,7 @@ def _members_apart(W):
 
 
 def quantize_weight(W, transposed=True):
-    """W [M, O, I] as Weight8; transposed=False leaves out what only a backward pass reads."""
+    """W [M, O, I] as Weight8; transposed=False leaves out codes_t and scales_t, half of its bytes, which linear does not read."""
     _check(W, 'block8.quantize_weight')
     _not_traced('block8.quantize_weight')
     return _quantize_weight(W, transposed)

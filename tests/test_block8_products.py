@@ -156,3 +156,18 @@ def test_refusals_on_the_gpu():
                  lambda: block8.linear(block8.quantize(x), w, products='fp8'), lambda: block8.linear(x.half(), W, products='e4m3')):
         with pytest.raises(ValueError):
             call()
+
+
+@gpu
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
+def test_transposed_codes_multiply_with_the_weights_themselves(dtype):
+    """quantize_weight's codes_t as a Weight8: the product that the input gradient is, bit for bit; without them half of the bytes."""
+    from hyper_amd import block8
+    for M, N, O, I in ((2, 40, 300, 140), (2, 3, 300, 140)):
+        x, W, dy = features((M, N, I), dtype, 1).cuda().requires_grad_(True), torch.randn(M, O, I, device='cuda'), features((M, N, O), dtype, 2).cuda()
+        dx, = torch.autograd.grad(block8.linear(x, W, scale=0.5), x, dy)
+        w = block8.quantize_weight(W)
+        back = block8.Weight8(w.codes_t, w.scales_t, w.outputs)
+        assert torch.equal(block8.linear(block8.quantize(dy), back, scale=0.5), dx)
+        alone = block8.quantize_weight(W, transposed=False)
+        assert alone.codes_t is None and alone.scales_t is None and alone.nbytes() == w.codes.numel() + w.scales.numel()
