@@ -6,8 +6,8 @@
 // HBM bound: the forward reads x and writes y once, the backward reads x and dy and writes dx once.  A row therefore stays in
 // the registers of TPR threads (16 elements each at most) between its loads and its stores, so that the variance is the
 // two-pass one (mean first, then squared distances) at no extra traffic; all statistics are fp32.  A row of up to 1024
-// elements belongs to 8, 16, 32 or 64 lanes of a wave (its sums need no barrier), a longer one to 256 / 512 / 1024 threads; the
-// next row's loads are under way while a row is summed.
+// elements belongs to 8, 16, 32 or 64 lanes of a wave (its sums need no barrier), a longer one to 128 (forward only), 256, 512 or 1024
+// threads; the next row's loads are under way while a row is summed.
 // Measured (a copy reaches 5.3 TB/s): 2 x 16384 x 8192 bf16 209 us forward (5.1 TB/s), 335 us backward (4.8); 10 x 2048 x 2048 fp32 65 us
 // (5.2) and 112 us (4.5, the partial sums included); rows of 1001 fp16, 5 x 300: 6 and 18 us, latency.
 // The backward keeps every thread's columns of dw and db in registers over all rows of its workgroup and writes them once:
@@ -253,32 +253,40 @@ static int norm_threads(int D, int piece, bool forward) {
 // 8192: 27 / 44, 26 / 45 and 29 / 54.
 static int norm_chunks(long long G, long long R, int threads, bool forward) {
   const int rpb = threads <= 64 ? 256 / threads : 1;
-  const long long most = forward ? (threads >= 1024 ? 512 : threads == 512 ? 1024 : 2048) : threads <= 256 ? (threads == 128 ? 2048 : 1024) : threads == 512 ? 512 : 256;
+  const long long most = forward ? (threads >= 1024 ? 512 : threads == 512 ? 1024 : 2048) : threads <= 256 ? 1024 : threads == 512 ? 512 : 256;
   const long long want = (R + rpb - 1) / rpb, share = most / G < 1 ? 1 : most / G;
   return (int)(want < share ? want : share);
 }
 
 template <class T, class F>
-static int norm_dispatch(int D, bool forward, const F& f) {
+static int norm_dispatch(int D, const F& f) {
   constexpr int N = Piece<T>::N;
-  const int t = norm_threads(D, N, forward), need = (D + t * N - 1) / (t * N);      // pieces per thread: 1, 2 or (fp32) 4
-#define HECKA_NORM(TPR) \
-  case TPR: return need <= 1 ? f.template run<T, TPR, 1>() : need <= 2 ? f.template run<T, TPR, 2>() : f.template run<T, TPR, 16 / N>();
+  const int t = norm_threads(D, N, F::kForward), need = (D + t * N - 1) / (t * N);      // pieces per thread
   switch (t) {
     case 8: return f.template run<T, 8, 1>();
     case 16: return f.template run<T, 16, 1>();
     case 32: return f.template run<T, 32, 1>();
-    HECKA_NORM(64)
-    HECKA_NORM(128)
-    HECKA_NORM(256)
-    HECKA_NORM(512)
-    HECKA_NORM(1024)
-    default: return HECKA_EINVAL;
+    case 64: return need <= 1 ? f.template run<T, 64, 1>() : need <= 2 ? f.template run<T, 64, 2>() : f.template run<T, 64, 16 / N>();
   }
-#undef HECKA_NORM
+  if constexpr (F::kForward) {      // more than half of 16 elements a thread
+    switch (t) {
+      case 128: return f.template run<T, 128, 16 / N>();
+      case 256: return f.template run<T, 256, 16 / N>();
+      case 512: return f.template run<T, 512, 16 / N>();
+      case 1024: return f.template run<T, 1024, 16 / N>();
+    }
+  } else {                          // more than half of 8, or of 16 beyond 8192
+    switch (t) {
+      case 256: return f.template run<T, 256, 8 / N>();
+      case 512: return f.template run<T, 512, 8 / N>();
+      case 1024: return D <= 8192 ? f.template run<T, 1024, 8 / N>() : f.template run<T, 1024, 16 / N>();
+    }
+  }
+  return HECKA_EINVAL;
 }
 
 struct NormFwd {
+  static constexpr bool kForward = true;
   const void* x; long long G, R; int D; const float *w, *b; long long wstride; float eps; void* y; float *mean, *rstd; hipStream_t st;
   template <class T, int TPR, int NV> int run() const {
     const int chunks = norm_chunks(G, R, TPR, true);
@@ -288,6 +296,7 @@ struct NormFwd {
   }
 };
 struct NormBwd {
+  static constexpr bool kForward = false;
   const void *dy, *x; const float *mean, *rstd; long long G, R; int D; const float* w; long long wstride; void* dx; float *dw, *db; long long gstride; float* ws; hipStream_t st;
   template <class T, int TPR, int NV> int run() const {
     constexpr bool AHEAD = NV * Piece<T>::N <= 8;
@@ -303,9 +312,8 @@ struct NormBwd {
 };
 
 template <class F>
-static int norm_type(int dtype, int D, bool forward, const F& f) {
-  return dtype == HECKA_DT_F32 ? norm_dispatch<float>(D, forward, f)
-         : dtype == HECKA_DT_BF16 ? norm_dispatch<Bf16>(D, forward, f) : norm_dispatch<F16>(D, forward, f);
+static int norm_type(int dtype, int D, const F& f) {
+  return dtype == HECKA_DT_F32 ? norm_dispatch<float>(D, f) : dtype == HECKA_DT_BF16 ? norm_dispatch<Bf16>(D, f) : norm_dispatch<F16>(D, f);
 }
 
 static int norm_check(const char* what, int dtype, int G, long long R, int D) {
@@ -326,7 +334,7 @@ int hecka_layernorm_fwd(const void* x, int dtype, int G, long long R, int D, con
   if (int rc = norm_check("layernorm_fwd", dtype, G, R, D)) return rc;
   if (!x || !y || !mean != !rstd) return fail(HECKA_EINVAL, "layernorm_fwd: null pointer%s");
   clear_error();
-  return norm_type(dtype, D, true, NormFwd{x, G, R, D, weight, bias, wstride, eps, y, mean, rstd, (hipStream_t)stream});
+  return norm_type(dtype, D, NormFwd{x, G, R, D, weight, bias, wstride, eps, y, mean, rstd, (hipStream_t)stream});
 }
 
 size_t hecka_layernorm_bwd_workspace_bytes(int G, long long R, int D) {
@@ -345,7 +353,7 @@ int hecka_layernorm_bwd(const void* dy, const void* x, int dtype, const float* m
   if ((dweight || dbias) && (ws ? ws_bytes : 0) < hecka_layernorm_bwd_workspace_bytes(G, R, D))
     return fail(HECKA_EWORKSPACE, "%slayernorm_bwd: workspace too small (%lld bytes given)", "", (long long)ws_bytes);
   clear_error();
-  return norm_type(dtype, D, false, NormBwd{dy, x, mean, rstd, G, R, D, weight, wstride, dx, dweight, dbias, gstride, (float*)ws,
+  return norm_type(dtype, D, NormBwd{dy, x, mean, rstd, G, R, D, weight, wstride, dx, dweight, dbias, gstride, (float*)ws,
                                      (hipStream_t)stream});
 }
 

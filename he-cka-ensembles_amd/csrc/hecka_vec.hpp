@@ -61,12 +61,6 @@ __device__ __forceinline__ float sum16(float v) {
   v += dpp<0x141>(v);
   return v + dpp<0x140>(v);
 }
-__device__ __forceinline__ float max16(float v) {
-  v = fmaxf(v, dpp<0xB1>(v));
-  v = fmaxf(v, dpp<0x4E>(v));
-  v = fmaxf(v, dpp<0x141>(v));
-  return fmaxf(v, dpp<0x140>(v));
-}
 __device__ __forceinline__ unsigned max16(unsigned v) {
   auto with = [&](int o) { v = (unsigned)o > v ? (unsigned)o : v; };
   with(__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, true));
