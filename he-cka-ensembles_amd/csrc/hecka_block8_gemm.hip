@@ -830,7 +830,7 @@ static WgradPlan wgrad_plan(int M, int N, int O, int I, bool whole) {
   // 256 x 256 tiles, one workgroup per CU, where dy's rows are whole 16-byte pieces (guarded loads, for which 256 x 256 leaves no
   // registers, otherwise) and a round of them does the work of 700 of 128 x 128, two per CU; where small ones are too few the rows in pieces
   // of 256 at least.  Measured (bf16 / fp32): 4 x 2000 x 2000 x 2000, 256 large or 1024 small tiles, 82 / 177 against 107 / 208 us; 3 x 4096 x 2048
-  // x 2048, 192 or 768, 132 / 302 against 153 / 312; large ones cut into pieces, 2 x 1024 x 2048 x 2048, 53 / 75 against 32 / 55 us, 1 x
+  // x 2048, 192 or 768, 132 / 302 against 153 / 312; ragged rows of dy, 4 x 2000 x 2001 x 2000, 324 / 259; large ones cut into pieces, 2 x 1024 x 2048 x 2048, 53 / 75 against 32 / 55 us, 1 x
   // 65536 x 256 x 512, 72 / 92 against 56 / 79.
   WgradPlan p{256, cdiv(O, 256), cdiv(I, 256), 1, cdiv(N, 64) * 64};
   const long long tiles = (long long)M * cdiv(O, 128) * cdiv(I, 128), s = tiles >= 512 ? 1 : 512 / tiles;

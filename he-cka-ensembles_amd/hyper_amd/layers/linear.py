@@ -139,8 +139,8 @@ class BatchedLinearCheckpoint(torch.autograd.Function):
 @register_gen_module('linear')
 class Linear(ParametersGroup):
     """checkpoint='e4m3' (not in the reference's signature): what the layer keeps for its backward pass - its input and, for the
-    activations that block8 knows, the activation's - is kept in 8-bit blocks; results are the same, gradients are taken at the
-    blocks' values.  compute='e4m3': the products themselves are of 8-bit blocks of x, W and the gradient (block8.linear; x fp32, bf16
+    activations that block8 knows, the activation's - is kept in 8-bit blocks; products are those of the layer without it, the
+    activation its own kernel's (equal but for its last places), gradients are taken at the blocks' values.  compute='e4m3': the products themselves are of 8-bit blocks of x, W and the gradient (block8.linear; x fp32, bf16
     or fp16), whose codes of x are the checkpoint; compute='fp8': the same for bf16 and fp16 x by the fp8 matrix instruction, faster and
     less exact (block8.linear's products)."""
 

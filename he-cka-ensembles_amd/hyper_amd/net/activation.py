@@ -98,8 +98,8 @@ class _Checkpointed(torch.autograd.Function):
 
 def checkpointed(name, x):
     """act(x) for 'gelu' (erf form), 'silu', 'tanh', 'sigmoid' or 'crater', its input kept for the backward pass in 8-bit blocks
-    (block8: a byte per element instead of 2 or 4; y is exact, only the slope is taken at the rounded input).  x: fp32 / bf16 /
-    fp16 on the GPU, any shape; blocks run along the last axis."""
+    (block8: a byte per element instead of 2 or 4; y is the function of x itself, only the slope is taken at the rounded
+    input).  x: fp32 / bf16 / fp16 on the GPU, any shape; blocks run along the last axis."""
     if name not in block8.ACTIVATIONS:
         raise ValueError('no 8-bit checkpoint for activation %r: please select from %s' % (name, sorted(block8.ACTIVATIONS)))
     block8._check(x, 'checkpointed')
